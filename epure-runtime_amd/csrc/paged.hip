@@ -1,0 +1,538 @@
+// Rotary positions, and the rows of a paged key-value cache: written (turned
+// and quantised on the way) and read back.  Declared in
+// include/epure_paged.h; attention over the cache is attend.hip.
+//
+// One kernel shape serves all three: a row is one head's D values of one
+// token, a lane holds 16 of them as two 16-byte chunks, and D / 16 lanes
+// (rounded up to a power of two) hold a row.  With pairs (i, i + dim / 2) a
+// lane's two chunks are the two halves of its pairs, so a turn needs nothing
+// from another lane, and a row's largest magnitude is a few lane exchanges
+// within 16 lanes.  All of it is bound by the bytes of the rows.
+#include "ep_common.h"
+#include "ep_internal.h"
+#include "ep_paged.h"
+
+namespace ep {
+namespace {
+
+struct Turn {
+    const float *cos_t, *sin_t;
+    int64_t max_pos;
+    int dim;          // 0: no rotation
+    int interleaved;
+    float sign;       // -1: the inverse
+};
+
+struct Rows {
+    const void *ptr;
+    int64_t sb, ss, sh;
+    int heads;
+};
+
+// Element index (within its row) of value e of a lane: chunk a, then chunk b.
+struct Chunks {
+    int a, b;
+    EP_DEV int at(int e) const { return e < 8 ? a + e : b + e - 8; }
+};
+
+// Lane u's chunks where whole chunks can be loaded: the two halves of the
+// pairs (i, i + dim / 2), else 16 adjacent values.
+EP_DEV Chunks chunks_of(int u, const Turn &t, bool turned)
+{
+    if (turned && !t.interleaved && u < t.dim / 16)
+        return {8 * u, 8 * u + t.dim / 2};
+    return {16 * u, 16 * u + 8};
+}
+
+template <typename T>
+EP_DEV float to_f32(T v);
+template <>
+EP_DEV float to_f32<float>(float v) { return v; }
+template <>
+EP_DEV float to_f32<f16_t>(f16_t v) { return (float)v; }
+template <>
+EP_DEV float to_f32<uint16_t>(uint16_t v) { return bf16_to_f32(v); }
+
+template <typename T>
+EP_DEV T from_f32(float v);
+template <>
+EP_DEV float from_f32<float>(float v) { return v; }
+template <>
+EP_DEV f16_t from_f32<f16_t>(float v) { return (f16_t)v; }
+template <>
+EP_DEV uint16_t from_f32<uint16_t>(float v) { return f32_to_bf16(v); }
+
+// 8 values from or to 16-byte aligned (32 for f32) memory.
+template <typename T>
+EP_DEV void load8(const T *p, float *v)
+{
+    T r[8];
+    __builtin_memcpy(r, __builtin_assume_aligned(p, 16), sizeof r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v[i] = to_f32<T>(r[i]);
+}
+template <typename T>
+EP_DEV void store8(T *p, const float *v)
+{
+    T r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        r[i] = from_f32<T>(v[i]);
+    __builtin_memcpy(__builtin_assume_aligned(p, 16), r, sizeof r);
+}
+
+// (a cos - b sin, b cos + a sin), each product rounded before the sum: the
+// result is the one of elementary f32 operations, whatever the compiler
+// would contract (an 8-bit code next to a rounding border depends on it).
+EP_DEV void turn_pair(float a, float b, float c, float s, float &ta, float &tb)
+{
+#pragma clang fp contract(off)
+    const float ac = a * c, bs = b * s, bc = b * c, as = a * s;
+    ta = ac - bs;
+    tb = bc + as;
+}
+
+// The 16 values of lane u of the row at x, turned by position p (in the
+// tables) where `turned`.  VEC: chunks are loaded whole (D and, with a turn,
+// dim / 2 in whole chunks, everything 16-byte aligned); else value by value.
+template <typename T, bool VEC>
+EP_DEV Chunks load_row(const T *x, int D, int u, const Turn &t, bool turned, int64_t p, float *v)
+{
+    if constexpr (VEC) {
+        const Chunks ch = chunks_of(u, t, turned);
+        load8(x + ch.a, v);
+        load8(x + ch.b, v + 8);
+        if (turned && 16 * u < t.dim) {
+            const float *cs = t.cos_t + p * (t.dim / 2) + 8 * u, *sn = t.sin_t + p * (t.dim / 2) + 8 * u;
+            float c[8], s[8];
+            load8(cs, c);
+            load8(sn, s);
+            if (t.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    turn_pair(v[2 * i], v[2 * i + 1], c[i], t.sign * s[i], v[2 * i], v[2 * i + 1]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    turn_pair(v[i], v[i + 8], c[i], t.sign * s[i], v[i], v[i + 8]);
+            }
+        }
+        return ch;
+    } else {
+        const Chunks ch{16 * u, 16 * u + 8};
+        const int half = t.dim / 2;
+        for (int e = 0; e < 16; ++e) {
+            const int d = 16 * u + e;
+            v[e] = d < D ? to_f32<T>(x[d]) : 0.0f;
+            if (turned && d < t.dim) {
+                const bool second = t.interleaved ? (d & 1) : d >= half;
+                const int i = t.interleaved ? d >> 1 : (second ? d - half : d);
+                const int other = t.interleaved ? d ^ 1 : (second ? d - half : d + half);
+                const float y = to_f32<T>(x[other]), c = t.cos_t[p * half + i], s = t.sign * t.sin_t[p * half + i];
+                float ta, tb;
+                if (second)
+                    turn_pair(y, v[e], c, s, ta, tb);
+                else
+                    turn_pair(v[e], y, c, s, ta, tb);
+                v[e] = second ? tb : ta;
+            }
+        }
+        return ch;
+    }
+}
+
+template <typename T, bool VEC>
+EP_DEV void store_row(T *y, int D, const Chunks &ch, const float *v)
+{
+    if constexpr (VEC) {
+        store8(y + ch.a, v);
+        store8(y + ch.b, v + 8);
+    } else {
+        for (int e = 0; e < 16; ++e)
+            if (ch.at(e) < D)
+                y[ch.at(e)] = from_f32<T>(v[e]);
+    }
+}
+
+// Largest over the lanes (a power of two, at most 16) that hold a row:
+// quads, then lane mirrors within 8 and 16 (every lane of the row takes
+// part; lanes of one row are adjacent and aligned).
+EP_DEV uint32_t row_max(uint32_t m, int lanes)
+{
+    auto step = [&](uint32_t o) { m = m > o ? m : o; };
+    if (lanes > 1)
+        step(__builtin_amdgcn_update_dpp(0, m, 0xb1, 0xf, 0xf, false));   // quad_perm [1,0,3,2]
+    if (lanes > 2)
+        step(__builtin_amdgcn_update_dpp(0, m, 0x4e, 0xf, 0xf, false));   // quad_perm [2,3,0,1]
+    if (lanes > 4)
+        step(__builtin_amdgcn_update_dpp(0, m, 0x141, 0xf, 0xf, false));  // row_half_mirror
+    if (lanes > 8)
+        step(__builtin_amdgcn_update_dpp(0, m, 0x140, 0xf, 0xf, false));  // row_mirror
+    return m;
+}
+
+EP_DEV float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Scale and codes of a lane's 16 values of a row whose largest |x| has the
+// bits `m` (as integers, magnitudes order NaN above infinity above the rest).
+EP_DEV float quantise(const float *v, uint32_t m, int dtype, uint32_t *codes)
+{
+    if (m >= 0x7f800000u) {
+        codes[0] = codes[1] = codes[2] = codes[3] = 0;
+        return __uint_as_float(0x7fc00000u);
+    }
+    if (dtype == EP_I8) {
+        const float top = fmaxf(__uint_as_float(m), pow2(-100));
+        const float inv = 127.0f / top;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float q = fminf(fmaxf(rintf(v[4 * i + j] * inv), -127.0f), 127.0f);
+                w |= ((uint32_t)(int)q & 0xffu) << (8 * j);
+            }
+            codes[i] = w;
+        }
+        return top / 127.0f;
+    }
+    // 448 = 0.875 * 2^9: m = f * 2^n with f in [0.5, 1) fits 448 * 2^e from
+    // e = n - 9 where f <= 0.875, else from n - 8.  Zero and subnormal m end
+    // at the least e.
+    const int n = (int)(m >> 23) - 126;
+    int e = (m & 0x7fffffu) <= 0x600000u ? n - 9 : n - 8;
+    e = e > -100 ? e : -100;
+    const float inv = pow2(-e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i] * inv, v[4 * i + 1] * inv, 0, false);
+        codes[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2] * inv, v[4 * i + 3] * inv, w, true);
+    }
+    return pow2(e);
+}
+
+struct Token {
+    int64_t b, s, p;
+};
+
+EP_DEV Token token_at(const PagedTokens &t, int64_t i)
+{
+    Token k;
+    k.b = i / t.S;
+    k.s = i - k.b * t.S;
+    k.p = t.pos[k.b * t.pos_sb + k.s * t.pos_ss];
+    return k;
+}
+
+// Which row a lane group of `lanes` works on: (token, head) of 256 / lanes
+// rows a workgroup.
+EP_DEV bool row_at(int64_t rows, int heads, int lanes, int64_t &token, int &head, int &u)
+{
+    const int64_t r = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    u = threadIdx.x & (lanes - 1);
+    if (r >= rows)
+        return false;
+    token = r / heads;
+    head = (int)(r - token * heads);
+    return true;
+}
+
+struct RotateArgs {
+    Rows q, k;
+    Turn turn;
+    PagedTokens tok;
+    void *q_out, *k_out;
+    int64_t rows;
+    int D, lanes;
+};
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) rotate_kernel(RotateArgs a)
+{
+    int64_t token;
+    int head, u;
+    if (!row_at(a.rows, a.q.heads + a.k.heads, a.lanes, token, head, u) || 16 * u >= a.D)
+        return;
+    const Token t = token_at(a.tok, token);
+    const bool is_q = head < a.q.heads;
+    const Rows &x = is_q ? a.q : a.k;
+    const int h = is_q ? head : head - a.q.heads;
+    T *y = (T *)(is_q ? a.q_out : a.k_out) + (token * x.heads + h) * a.D;
+    float v[16];
+    const bool ok = t.p >= 0 && t.p < a.turn.max_pos;
+    const Chunks ch = load_row<T, VEC>((const T *)x.ptr + t.b * x.sb + t.s * x.ss + h * x.sh, a.D, u, a.turn, ok, t.p, v);
+    if (!ok) {
+        const float fill = t.p < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            v[e] = fill;
+    }
+    store_row<T, VEC>(y, a.D, ch, v);
+}
+
+struct AppendArgs {
+    Rows q, k, v;
+    Turn turn;
+    PagedTokens tok;
+    PagedCache c;
+    void *q_out;
+    int64_t rows;
+    int lanes;
+};
+
+// The slot (row of [n_pages][page], times heads later) of position p, or
+// false: padding, past the table, or not a page.
+EP_DEV bool slot_of(const PagedTokens &t, const PagedCache &c, int64_t b, int64_t p, int64_t &page, int &row)
+{
+    if (p < 0 || (p >> c.page_shift) >= t.width)
+        return false;
+    page = t.table[b * t.table_stride + (p >> c.page_shift)];
+    row = (int)(p & (c.page - 1));
+    return page >= 0 && page < c.n_pages;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) append_kernel(AppendArgs a)
+{
+    int64_t token;
+    int head, u;
+    const int D = a.c.D, Hq = a.q.heads, Hk = a.c.heads;
+    if (!row_at(a.rows, Hq + 2 * Hk, a.lanes, token, head, u))
+        return;
+    const Token t = token_at(a.tok, token);
+    const bool mine = 16 * u < D;   // lanes past the row only take part in its maximum
+    const bool is_q = head < Hq, is_v = head >= Hq + Hk;
+    const Rows &x = is_q ? a.q : is_v ? a.v : a.k;
+    const int h = is_q ? head : is_v ? head - Hq - Hk : head - Hq;
+    const bool turns = !is_v && a.turn.dim > 0;
+    const bool known = t.p >= 0 && (!turns || t.p < a.turn.max_pos);
+    float v[16];
+    Chunks ch{0, 0};
+    if (mine)
+        ch = load_row<T, VEC>((const T *)x.ptr + t.b * x.sb + t.s * x.ss + h * x.sh, D, u, a.turn, turns && known, t.p, v);
+    if (!mine || !known) {
+        const float fill = t.p < 0 || !mine ? 0.0f : __uint_as_float(0x7fc00000u);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            v[e] = fill;
+    }
+    if (is_q) {
+        if (mine)
+            store_row<T, VEC>((T *)a.q_out + (token * Hq + h) * D, D, ch, v);
+        return;
+    }
+    int64_t page = 0;
+    int row = 0;
+    if (!known || !slot_of(a.tok, a.c, t.b, t.p, page, row))   // one answer for all lanes of a row
+        return;
+    const int64_t at = (page * Hk + h) * a.c.page + row;
+    void *dst = is_v ? a.c.v : a.c.k;
+    if (a.c.dtype == EP_F16 || a.c.dtype == EP_BF16) {
+        if (mine) {
+            if (a.c.dtype == EP_F16)
+                store_row<f16_t, true>((f16_t *)dst + at * D, D, ch, v);
+            else
+                store_row<uint16_t, true>((uint16_t *)dst + at * D, D, ch, v);
+        }
+        return;
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const uint32_t b = __float_as_uint(v[e]) & 0x7fffffffu;
+        m = m > b ? m : b;
+    }
+    m = row_max(m, a.lanes);
+    uint32_t codes[4];
+    const float s = quantise(v, m, a.c.dtype, codes);
+    if (mine) {
+        uint8_t *p = (uint8_t *)dst + at * D;
+        __builtin_memcpy(__builtin_assume_aligned(p + ch.a, 8), codes, 8);
+        __builtin_memcpy(__builtin_assume_aligned(p + ch.b, 8), codes + 2, 8);
+    }
+    if (u == 0)
+        (is_v ? a.c.v_scale : a.c.k_scale)[at] = s;
+}
+
+struct ReadArgs {
+    PagedTokens tok;
+    PagedCache c;
+    void *k_out, *v_out;
+    int64_t rows;
+    int lanes;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) read_kernel(ReadArgs a)
+{
+    int64_t token;
+    int head, u;
+    const int D = a.c.D, Hk = a.c.heads;
+    if (!row_at(a.rows, 2 * Hk, a.lanes, token, head, u) || 16 * u >= D)
+        return;
+    const Token t = token_at(a.tok, token);
+    const bool is_v = head >= Hk;
+    const int h = is_v ? head - Hk : head;
+    float v[16];
+    int64_t page;
+    int row;
+    if (slot_of(a.tok, a.c, t.b, t.p, page, row)) {
+        const int64_t at = (page * Hk + h) * a.c.page + row;
+        const void *src = is_v ? a.c.v : a.c.k;
+        if (a.c.dtype == EP_F16 || a.c.dtype == EP_BF16) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (a.c.dtype == EP_F16)
+                    load8((const f16_t *)src + at * D + 16 * u + 8 * i, v + 8 * i);
+                else
+                    load8((const uint16_t *)src + at * D + 16 * u + 8 * i, v + 8 * i);
+            }
+        } else {
+            const float s = (is_v ? a.c.v_scale : a.c.k_scale)[at];
+            const u32x4_t w = *(const u32x4_t *)((const uint8_t *)src + at * D + 16 * u);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                decode4(w[i], a.c.dtype, v + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                v[e] *= s;
+        }
+    } else {
+        const float fill = t.p < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            v[e] = fill;
+    }
+    store_row<T, true>((T *)(is_v ? a.v_out : a.k_out) + (token * Hk + h) * D, D, {16 * u, 16 * u + 8}, v);
+}
+
+bool aligned(const void *p, int64_t n) { return ((uintptr_t)p % n) == 0; }
+
+// A lane's chunks of these rows can be loaded whole.
+bool whole_chunks(const ep_heads *x, int64_t B, int64_t S)
+{
+    const int n = x->dtype == EP_F32 ? 4 : 8;   // values in 16 bytes
+    return aligned(x->ptr, 16) && (B == 1 || x->stride_b % n == 0) && (S == 1 || x->stride_s % n == 0) &&
+           (x->heads == 1 || x->stride_h % n == 0);
+}
+
+int lanes_of(int64_t D)
+{
+    int n = 1;
+    while (n * 16 < D)
+        n *= 2;
+    return n;
+}
+
+// D and the rotated part in whole chunks (in pairs of them where a lane's
+// two chunks are the halves of its pairs, and the rest in 16s).
+bool whole_rows(int64_t D, const ep_rotation *rot)
+{
+    return D % 16 == 0 && (!rot || (rot->dim % 16 == 0 && aligned(rot->cos_t, 16) && aligned(rot->sin_t, 16)));
+}
+
+Rows rows_of(const ep_heads *x)
+{
+    return x && x->ptr ? Rows{x->ptr, x->stride_b, x->stride_s, x->stride_h, x->heads} : Rows{nullptr, 0, 0, 0, 0};
+}
+
+Turn turn_of(const ep_rotation *rot, int inverse)
+{
+    if (!rot)
+        return Turn{nullptr, nullptr, 0, 0, 0, 1.0f};
+    return Turn{rot->cos_t, rot->sin_t, rot->max_pos, rot->dim, rot->interleaved, inverse ? -1.0f : 1.0f};
+}
+
+int grid_of(int64_t rows, int lanes, unsigned &grid)
+{
+    const int64_t per = 256 / lanes, n = (rows + per - 1) / per;
+    if (n > 0x7fffffff)
+        return set_error(EP_DECLINE_SHAPE, "%lld rows are more than one launch takes", (long long)rows);
+    grid = (unsigned)n;
+    return EP_OK;
+}
+
+template <bool VEC>
+void rotate_typed(int dtype, unsigned grid, const RotateArgs &a, hipStream_t st)
+{
+    if (dtype == EP_F32)
+        rotate_kernel<float, VEC><<<grid, 256, 0, st>>>(a);
+    else if (dtype == EP_F16)
+        rotate_kernel<f16_t, VEC><<<grid, 256, 0, st>>>(a);
+    else
+        rotate_kernel<uint16_t, VEC><<<grid, 256, 0, st>>>(a);
+}
+
+template <bool VEC>
+void append_typed(int dtype, unsigned grid, const AppendArgs &a, hipStream_t st)
+{
+    if (dtype == EP_F32)
+        append_kernel<float, VEC><<<grid, 256, 0, st>>>(a);
+    else if (dtype == EP_F16)
+        append_kernel<f16_t, VEC><<<grid, 256, 0, st>>>(a);
+    else
+        append_kernel<uint16_t, VEC><<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace
+
+int launch_rotate(const ep_heads *q, const ep_heads *k, const ep_rotation *rot, const PagedTokens &tok, int64_t D,
+                  int inverse, void *q_out, void *k_out, hipStream_t stream)
+{
+    RotateArgs a{rows_of(q), rows_of(k), turn_of(rot, inverse), tok, q_out, k_out, 0, (int)D, lanes_of(D)};
+    a.rows = tok.B * tok.S * (a.q.heads + a.k.heads);
+    unsigned grid;
+    const int rc = grid_of(a.rows, a.lanes, grid);
+    if (rc != EP_OK || a.rows == 0)
+        return rc;
+    const bool vec = whole_rows(D, rot) && whole_chunks(q, tok.B, tok.S) && aligned(q_out, 16) &&
+                     (!a.k.ptr || (whole_chunks(k, tok.B, tok.S) && aligned(k_out, 16)));
+    if (vec)
+        rotate_typed<true>(q->dtype, grid, a, stream);
+    else
+        rotate_typed<false>(q->dtype, grid, a, stream);
+    EP_HIP_CHECK(hipGetLastError());
+    return EP_OK;
+}
+
+int launch_kv_append(const ep_heads *q, const ep_heads *k, const ep_heads *v, const ep_rotation *rot,
+                     const PagedTokens &tok, const PagedCache &c, void *q_out, hipStream_t stream)
+{
+    AppendArgs a{rows_of(q), rows_of(k), rows_of(v), turn_of(rot, 0), tok, c, q_out, 0, lanes_of(c.D)};
+    a.rows = tok.B * tok.S * (a.q.heads + 2 * c.heads);
+    unsigned grid;
+    const int rc = grid_of(a.rows, a.lanes, grid);
+    if (rc != EP_OK || a.rows == 0)
+        return rc;
+    const bool vec = whole_rows(c.D, rot) && whole_chunks(k, tok.B, tok.S) && whole_chunks(v, tok.B, tok.S) &&
+                     (!a.q.ptr || (whole_chunks(q, tok.B, tok.S) && aligned(q_out, 16)));
+    if (vec)
+        append_typed<true>(k->dtype, grid, a, stream);
+    else
+        append_typed<false>(k->dtype, grid, a, stream);
+    EP_HIP_CHECK(hipGetLastError());
+    return EP_OK;
+}
+
+int launch_kv_read(const PagedTokens &tok, const PagedCache &c, void *k_out, void *v_out, int out_dtype,
+                   hipStream_t stream)
+{
+    ReadArgs a{tok, c, k_out, v_out, tok.B * tok.S * 2 * c.heads, lanes_of(c.D)};
+    unsigned grid;
+    const int rc = grid_of(a.rows, a.lanes, grid);
+    if (rc != EP_OK || a.rows == 0)
+        return rc;
+    if (!aligned(k_out, 16) || !aligned(v_out, 16))
+        return set_error(EP_DECLINE_SHAPE, "cache read: outputs must be 16-byte aligned");
+    if (out_dtype == EP_F32)
+        read_kernel<float><<<grid, 256, 0, stream>>>(a);
+    else if (out_dtype == EP_F16)
+        read_kernel<f16_t><<<grid, 256, 0, stream>>>(a);
+    else
+        read_kernel<uint16_t><<<grid, 256, 0, stream>>>(a);
+    EP_HIP_CHECK(hipGetLastError());
+    return EP_OK;
+}
+
+}  // namespace ep

@@ -1,5 +1,6 @@
 """epure (MI355X build) -- the fused codebook dequant-matmul behind every
-packed linear, on hand-written gfx950 HIP kernels.
+packed linear, on hand-written gfx950 HIP kernels, and what a served batch
+needs between the linears (rotary positions, a paged key-value cache, attention).
 
 Public names follow the reference package (epure/__init__.py:31-37) for the
 parts this build covers: the packed store, linear and embedding, the fine-tuning
@@ -14,6 +15,7 @@ from .finetune import (
     trainable_forward,
     verify_frozen,
 )
+from .paged import PagedKVCache, Rotary, rope_frequencies
 from .runtime import (
     ExpertHolder,
     PackedEmbedding,
@@ -31,5 +33,6 @@ __all__ = [
     "apply_packed", "tie_packed_lm_head",
     "make_trainable", "packed_weights", "snapshot_indices", "verify_frozen",
     "trainable_forward", "ScaleTuner", "container",
+    "Rotary", "rope_frequencies", "PagedKVCache",
     "__version__",
 ]

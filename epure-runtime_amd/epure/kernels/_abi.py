@@ -16,13 +16,39 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__
                         LIB_NAME)
 
 ABI_VERSION = 1
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, E4M3, I8 = 0, 1, 2, 3, 4
 FLAG_ACCUMULATE = 1
 OK = 0
 
 _DT = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+# element types of a paged cache
+CACHE_DT = {torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3, torch.int8: I8}
 
 _c_i64, _c_int, _p, _sz = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
+
+
+# Descriptors of include/epure_paged.h.
+class Heads(ctypes.Structure):
+    _fields_ = [("ptr", _p), ("dtype", _c_int), ("heads", _c_int), ("stride_b", _c_i64), ("stride_s", _c_i64),
+                ("stride_h", _c_i64)]
+
+
+class Tokens(ctypes.Structure):
+    _fields_ = [("B", _c_i64), ("S", _c_i64), ("positions", _p), ("pos_stride_b", _c_i64),
+                ("pos_stride_s", _c_i64), ("table", _p), ("table_stride", _c_i64), ("width", _c_i64)]
+
+
+class KVCache(ctypes.Structure):
+    _fields_ = [("k", _p), ("v", _p), ("k_scale", _p), ("v_scale", _p), ("dtype", _c_int), ("heads", _c_int),
+                ("page", _c_int), ("D", _c_int), ("n_pages", _c_i64)]
+
+
+class Rotation(ctypes.Structure):
+    _fields_ = [("cos_t", _p), ("sin_t", _p), ("max_pos", _c_i64), ("dim", _c_int), ("interleaved", _c_int)]
+
+
+_heads, _tokens = ctypes.POINTER(Heads), ctypes.POINTER(Tokens)
+_cache, _rotation = ctypes.POINTER(KVCache), ctypes.POINTER(Rotation)
 
 _SIGS = {
     "ep_abi_version": (_c_int, []),
@@ -103,6 +129,14 @@ _SIGS = {
         _c_int, _c_int, _c_int, _c_int, _c_int,  # max_pos, levels, group, scale_dtype, cb_dtype
         ctypes.c_float, ctypes.c_float, ctypes.c_float,  # eps, qk_eps, att_scale
         _p, _p]),                                # trace, stream
+    # include/epure_paged.h
+    "ep_rotate": (_c_int, [_heads, _heads, _rotation, _tokens, _c_i64, _c_int, _p, _p, _p]),
+    "ep_kv_append": (_c_int, [_heads, _heads, _heads, _rotation, _tokens, _cache, _p, _p]),
+    "ep_kv_read": (_c_int, [_tokens, _cache, _p, _p, _c_int, _p]),
+    "ep_paged_attention_workspace": (_sz, [_heads, _tokens, _cache]),
+    "ep_paged_attention": (_c_int, [
+        _heads, _tokens, _cache, ctypes.c_float, _c_i64,  # q, tokens, cache, scale, window
+        _p, _p, _sz, _p]),                       # out, workspace, bytes, stream
 }
 
 XSRC_PLAIN, XSRC_RMSNORM, XSRC_SWIGLU = 0, 1, 2
