@@ -1,0 +1,646 @@
+// Attention of new tokens over a paged key-value cache: the kernel template
+// (attend.hip plans and joins; attend_gen_*.hip instantiate).
+//
+//   out[r] = sum_j softmax_j(scale q[r] . k[j]) v[j],   first(r) <= j <= last(r)
+//
+// The rows of one matrix tile are the query heads that share a cache head,
+// over all new tokens of a sequence (a "unit" is up to 16 MT of them); a
+// segment is one unit on one cache head, cut into tiles of 32 positions.
+//
+// A wave takes whole tiles straight from memory to registers, with nothing
+// exchanged between lanes on the way:
+//   S^T = K Q^T: lane (n = lane & 15, g = lane >> 4) gives key row 16 t + n,
+//     values 8 g .. 8 g + 7 of each 32 (8-bit caches: 16 g .. of each 64,
+//     taken as two steps), and gets the scores of positions
+//     16 t + 4 g + i of query row n.
+//   O^T = V^T P^T: that is the layout of the second product's B operand if
+//     its k index 8 g + 4 t + i means position 16 t + 4 g + i.  The A operand
+//     then wants, for output n, eight positions of one column: lane n takes
+//     CW adjacent columns of those eight rows (16 lanes read one whole row),
+//     and the CW products of columns CW n + t, t = 0 .. CW - 1, need only the
+//     16-bit halves of two rows put side by side.
+// A row's maximum, sum and output live in the four lanes of one n, so the
+// running softmax costs two lane exchanges a tile.
+//
+// Rounding: scores, softmax and sums are f32; the weights enter the second
+// product as two 16-bit terms (w and what its rounding lost), which leaves
+// 2^-16 of each and costs matrix instructions that a bandwidth-bound loop
+// has to spare.  8-bit codes are exact in either 16-bit type; their scales
+// multiply scores and weights.  In f16 the weights are 2^15 exp(s - max), so
+// that a long tail of small ones stays above f16's least number.
+#pragma once
+
+#include "ep_common.h"
+#include "ep_internal.h"
+#include "ep_paged.h"
+
+namespace ep {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+constexpr int kAttTile = 32;             // positions a wave takes at a time
+constexpr int kAttWaves = 4;             // waves of a workgroup: they take tiles in turn
+constexpr int kAttOut = 0x40000000;      // an offset past every descriptor below: reads zeros
+
+struct AttendArgs {
+    const void *q;
+    int64_t q_sb, q_ss, q_sh;
+    PagedTokens tok;
+    PagedCache c;
+    float scale;             // of the scores, times log2(e)
+    int window;              // 1 .. cap
+    int cap;                 // positions that the table has pages for
+    void *out;
+    int G, rows;             // query heads a cache head; rows of a sequence on one cache head (S G)
+    int blocks;              // units of a sequence
+    int64_t units;
+    int workers;             // workgroups that share all tiles evenly; 0: one workgroup a segment
+    int slot_rows;           // rows kept of a piece: min(rows, 16 MT)
+    int2 *desc;              // [segments]: first slot, pieces
+    float2 *part_ml;         // [2 workers][slot_rows]: maximum, sum
+    float *part_o;           // [2 workers][slot_rows][D]
+};
+
+EP_DEV int dpp_row_max(int v)
+{
+    const auto step = [&](int o) { v = v > o ? v : o; };
+    step(__builtin_amdgcn_update_dpp(0, v, 0x128, 0xf, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x124, 0xf, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, false));
+    step(__builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, false));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// Position of token (b, s): in [0, cap), -1 for padding, cap past the table.
+EP_DEV int attend_position(const AttendArgs &a, int64_t b, int s)
+{
+    const int64_t p = a.tok.pos[b * a.tok.pos_sb + s * a.tok.pos_ss];
+    return p < 0 ? -1 : p >= a.cap ? a.cap : (int)p;
+}
+
+EP_DEV int first_seen(const AttendArgs &a, int p) { return p >= a.window ? p - a.window + 1 : 0; }
+
+// Tiles that the rows of unit u reach (one at least: its outputs are written
+// with that tile).
+template <int RM>
+EP_DEV uint32_t unit_tiles(const AttendArgs &a, int64_t u)
+{
+    const int64_t b = u / a.blocks;
+    const int r0 = (int)(u - b * a.blocks) * RM, r1 = min(r0 + RM, a.rows);
+    int lo = a.cap, hi = -1;
+    for (int s = r0 / a.G; s <= (r1 - 1) / a.G; ++s) {
+        const int p = attend_position(a, b, s);
+        if (p >= 0 && p < a.cap) {
+            hi = max(hi, p);
+            lo = min(lo, first_seen(a, p));
+        }
+    }
+    return hi < 0 ? 1u : (uint32_t)(hi / kAttTile - lo / kAttTile + 1);
+}
+
+// 16-bit arithmetic of a product's operands.
+struct OpBf16 {
+    static constexpr int kDtype = EP_BF16;
+    static constexpr float kShift = 0.0f;
+    static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
+    static EP_DEV f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c)
+    {
+        bf16x8_t x, y;
+        __builtin_memcpy(&x, &a, 16);
+        __builtin_memcpy(&y, &b, 16);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+    }
+    // Two values rounded to 16 bits, and the rest of each rounded likewise.
+    static EP_DEV uint32_t pack(float x, float y)
+    {
+        typedef float f32x2_t __attribute__((ext_vector_type(2)));
+        const bf16x2_t h = __builtin_convertvector((f32x2_t){x, y}, bf16x2_t);
+        uint32_t u;
+        __builtin_memcpy(&u, &h, 4);
+        return u;
+    }
+    static EP_DEV float low(uint32_t u) { return __uint_as_float(u << 16); }
+    static EP_DEV float high(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+};
+struct OpF16 {
+    static constexpr int kDtype = EP_F16;
+    static constexpr float kShift = 15.0f;
+    static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
+    static EP_DEV f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c)
+    {
+        f16x8_t x, y;
+        __builtin_memcpy(&x, &a, 16);
+        __builtin_memcpy(&y, &b, 16);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+    }
+    static EP_DEV uint32_t pack(float x, float y)
+    {
+        const f16x2_t h = {(f16_t)x, (f16_t)y};
+        uint32_t u;
+        __builtin_memcpy(&u, &h, 4);
+        return u;
+    }
+    static EP_DEV float low(uint32_t u) { return (float)as_f16x2(u)[0]; }
+    static EP_DEV float high(uint32_t u) { return (float)as_f16x2(u)[1]; }
+};
+
+// Two 8-bit codes of w (bytes B, B + 1 with HI = B / 2) as f32.
+template <int CODE, bool HI>
+EP_DEV void codes2(uint32_t w, float &x, float &y)
+{
+    if constexpr (CODE == EP_I8) {
+        x = (float)(int8_t)(w >> (HI ? 16 : 0));
+        y = (float)(int8_t)(w >> (HI ? 24 : 8));
+    } else {
+        typedef float f32x2_t __attribute__((ext_vector_type(2)));
+        const f32x2_t v = __builtin_amdgcn_cvt_pk_f32_fp8(w, HI);
+        x = v[0];
+        y = v[1];
+    }
+}
+
+// The upper halves of two f32 side by side: codes are exact in bf16.
+EP_DEV uint32_t high_halves(float x, float y)
+{
+    return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+}
+
+// Eight codes as an operand.
+template <typename OP, int CODE>
+EP_DEV u32x4_t decode8(uint32_t w0, uint32_t w1)
+{
+    u32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float x, y;
+        if (i & 1)
+            codes2<CODE, true>(i < 2 ? w0 : w1, x, y);
+        else
+            codes2<CODE, false>(i < 2 ? w0 : w1, x, y);
+        if constexpr (OP::kDtype == EP_BF16)
+            r[i] = high_halves(x, y);
+        else
+            r[i] = OP::pack(x, y);
+    }
+    return r;
+}
+
+EP_DEV __amdgpu_buffer_rsrc_t tile_rsrc(const void *base, int64_t byte, bool ok, int bytes)
+{
+    return buffer_rsrc((const char *)base + (ok ? byte : 0), ok ? (uint32_t)bytes : 0u);
+}
+
+// QOP: type of the queries; CODE: EP_I8, EP_E4M3, or QOP's type.  KS: steps of
+// 32 values of a head, CW: output columns a lane (16 CW >= D), MT: 16-row
+// tiles of query rows.
+template <typename QOP, int CODE, int KS, int CW, int MT>
+__global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
+{
+    constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
+    constexpr int ES = k8 ? 1 : 2, KL = k8 ? KS / 2 : KS, RM = 16 * MT, DP = 16 * CW, VW = CW * ES / 4;
+    static_assert(!k8 || KS % 2 == 0, "8-bit keys are read in chunks of two steps");
+    using VOP = typename std::conditional<k8, OpBf16, QOP>::type;
+    __shared__ float s_o[kAttWaves][16][DP + 4];
+    __shared__ float s_m[kAttWaves][RM], s_l[kAttWaves][RM];
+    __shared__ int s_p[RM];
+
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int H = a.c.heads, D = a.c.D;
+    const float nan = __uint_as_float(0x7fc00000u);
+
+    // Offsets of this lane's key chunks and value rows within half a tile.
+    int koff[2], voff[4];
+    const int kbase = n * D * ES + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int d = (KL - 2 + i) * (k8 ? 64 : 32) + g * (k8 ? 16 : 8);
+        koff[i] = d < D ? kbase + (KL - 2 + i) * 64 : kAttOut;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        voff[i] = CW * n < D ? ((4 * g + i) * D + CW * n) * ES : kAttOut;
+
+    // ---- one piece: tiles [t0, t1) of a segment, counted from its first;
+    // t1 < 0: all of them.  slot < 0: the outputs are written.
+    auto piece = [&](int64_t u, int h, int t0, int t1, int slot) {
+        const int64_t b = u / a.blocks;
+        const int r0 = (int)(u - b * a.blocks) * RM;
+        int first[MT], last[MT];
+        u32x4_t q[MT][KS];
+        int lo = -a.cap, hi = -1, in_lo = 0, in_hi = -a.cap;     // over the rows: seen by any (lo negated), by all
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const int row = r0 + 16 * mt + n;
+            const int s = min(row, a.rows - 1) / a.G, gq = row - s * a.G;
+            const int p = row < a.rows ? attend_position(a, b, s) : -1;
+            const bool some = p >= 0 && p < a.cap;
+            first[mt] = some ? first_seen(a, p) : a.cap;
+            last[mt] = some ? p : -1;
+            lo = max(lo, some ? -first[mt] : -a.cap);
+            hi = max(hi, last[mt]);
+            in_lo = max(in_lo, some ? first[mt] : 0);
+            in_hi = max(in_hi, some ? -p : -a.cap);
+            const char *src = (const char *)a.q + 2 * (b * a.q_sb + s * a.q_ss + (int64_t)(h * a.G + gq) * a.q_sh);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const int d = k8 ? 64 * (k / 2) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g;
+                q[mt][k] = row < a.rows && d < D ? *(const u32x4_t *)(src + 2 * d) : (u32x4_t){0, 0, 0, 0};
+            }
+            if (wave == 0 && g == 0)
+                s_p[16 * mt + n] = p;
+        }
+        lo = -dpp_row_max(lo);
+        hi = dpp_row_max(hi);
+        in_lo = dpp_row_max(in_lo);
+        in_hi = -dpp_row_max(in_hi);
+        const bool ragged = lo != in_lo || hi != in_hi;     // rows differ in what they see
+        const int tile0 = hi < 0 ? 0 : lo / kAttTile;
+        const int end = t1 < 0 ? (hi < 0 ? 1 : hi / kAttTile + 1) : tile0 + t1;
+
+        // ---- loads
+        const int32_t *table = a.tok.table + b * a.tok.table_stride;
+        auto load_ids = [&](int j) {
+            const int64_t at = (int64_t)(j * kAttTile + 16 * (lane & 1)) >> a.c.page_shift;
+            return a.tok.width > 0 ? table[at < a.tok.width ? at : a.tok.width - 1] : -1;
+        };
+        u32x4_t kr[2][KL];
+        uint32_t vr[8][VW];
+        float ks[8], vs[8];
+        bool good[2];
+        int64_t at[2];       // row of each half's first position
+        auto locate = [&](int ids, int j) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int64_t id = __builtin_amdgcn_readlane(ids, t);
+                good[t] = j < end && id >= 0 && id < a.c.n_pages;
+                at[t] = (id * H + h) * a.c.page + ((j * kAttTile + 16 * t) & (a.c.page - 1));
+            }
+        };
+        auto load_scales = [&](const float *src, float *out) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const auto w = __builtin_amdgcn_raw_buffer_load_b128(tile_rsrc(src, at[t] * 4, good[t], 64), 16 * g, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    out[4 * t + i] = __uint_as_float(w[i]);
+            }
+        };
+        auto load_k = [&]() {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const auto r = tile_rsrc(a.c.k, at[t] * D * ES, good[t], 16 * D * ES);
+#pragma unroll
+                for (int k = 0; k < KL; ++k)
+                    kr[t][k] = __builtin_amdgcn_raw_buffer_load_b128(
+                        r, k >= KL - 2 ? koff[k - (KL - 2)] : kbase + 64 * k, 0, 0);
+            }
+            if constexpr (k8)
+                load_scales(a.c.k_scale, ks);
+        };
+        auto load_v = [&]() {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const auto r = tile_rsrc(a.c.v, at[t] * D * ES, good[t], 16 * D * ES);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t *dst = vr[4 * t + i];
+                    if constexpr (VW == 1)
+                        dst[0] = __builtin_amdgcn_raw_buffer_load_b32(r, voff[i], 0, 0);
+                    else if constexpr (VW == 2) {
+                        const auto w = __builtin_amdgcn_raw_buffer_load_b64(r, voff[i], 0, 0);
+                        dst[0] = w[0];
+                        dst[1] = w[1];
+                    } else
+#pragma unroll
+                        for (int c = 0; c < VW; c += 4) {
+                            const auto w = __builtin_amdgcn_raw_buffer_load_b128(r, voff[i] + 4 * c, 0, 0);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                dst[c + x] = w[x];
+                        }
+                }
+            }
+            if constexpr (k8)
+                load_scales(a.c.v_scale, vs);
+        };
+
+        // ---- the running softmax
+        float m[MT], l[MT];
+        f32x4_t o[MT][CW];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt] = -INFINITY;
+            l[mt] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < CW; ++t)
+                o[mt][t] = (f32x4_t){0, 0, 0, 0};
+        }
+        int j = tile0 + t0 + wave;
+        int ids = load_ids(j);
+        locate(ids, j);
+        ids = load_ids(j + kAttWaves);
+        load_k();
+        load_v();
+        for (; j < end; j += kAttWaves) {
+            const int j0 = j * kAttTile;
+            const bool bad0 = !good[0], bad1 = !good[1];
+            f32x4_t sc[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    sc[mt][t] = (f32x4_t){0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    u32x4_t f;
+                    if constexpr (k8)
+                        f = decode8<QOP, CODE>(kr[t][k / 2][2 * (k & 1)], kr[t][k / 2][2 * (k & 1) + 1]);
+                    else
+                        f = kr[t][k];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+                        sc[mt][t] = QOP::mfma(f, q[mt][k], sc[mt][t]);
+                }
+            float x[MT][8];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[mt][e] = sc[mt][e / 4][e % 4] * (k8 ? ks[e] * a.scale : a.scale);
+            // the next tile's keys (none past the end: empty descriptors)
+            locate(ids, j + kAttWaves);
+            ids = load_ids(j + 2 * kAttWaves);
+            load_k();
+
+            // A tile that some row sees in part (or that names a page the pool
+            // lacks: its scores are NaN) masks its scores one by one.
+            const bool edge = j0 < in_lo || j0 + kAttTile - 1 > in_hi || bad0 || bad1;
+            uint32_t seen[MT];
+            if (edge) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    seen[mt] = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int p = j0 + 16 * (e / 4) + 4 * g + e % 4;
+                        const bool in = p >= first[mt] && p <= last[mt];
+                        seen[mt] |= (uint32_t)in << e;
+                        x[mt][e] = !in ? -INFINITY : (e < 4 ? bad0 : bad1) ? nan : x[mt][e];
+                    }
+                }
+            }
+            u32x4_t ph[MT], pl[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                float top = x[mt][0];
+#pragma unroll
+                for (int e = 1; e < 8; ++e)
+                    top = fmaxf(top, x[mt][e]);
+                top = fmaxf(m[mt], xor32_max(xor16_max(top)));
+                const float base = top == -INFINITY ? 0.0f : top;
+                if (__any(top > m[mt])) {
+                    const float keep = __builtin_amdgcn_exp2f(m[mt] - base);
+                    l[mt] *= keep;
+#pragma unroll
+                    for (int t = 0; t < CW; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            o[mt][t][i] *= keep;
+                }
+                m[mt] = top;
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(x[mt][e] - (base - VOP::kShift));
+                    l[mt] += w[e];
+                    if constexpr (k8)
+                        w[e] = edge && !(seen[mt] >> e & 1) ? 0.0f : w[e] * vs[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    ph[mt][e] = VOP::pack(w[2 * e], w[2 * e + 1]);
+                    pl[mt][e] = VOP::pack(w[2 * e] - VOP::low(ph[mt][e]), w[2 * e + 1] - VOP::high(ph[mt][e]));
+                }
+            }
+            // Values: what no row sees becomes zero (its weights are zero, and
+            // zero times a NaN is NaN); what some rows see and others not is
+            // taken out if it is not finite, and added where it is seen.
+            uint32_t keep[4];
+            if (edge)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int p = j0 + 16 * (e / 2) + 4 * g + 2 * (e % 2);
+                    keep[e] = (p >= lo && p <= hi ? 0xffffu : 0u) | (p + 1 >= lo && p + 1 <= hi ? 0xffff0000u : 0u);
+                }
+#pragma unroll
+            for (int t = 0; t < CW; ++t) {
+                u32x4_t f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (k8) {
+                        float v0[2], v1[2];
+                        if (t & 2) {
+                            codes2<CODE, true>(vr[2 * e][t / 4], v0[0], v0[1]);
+                            codes2<CODE, true>(vr[2 * e + 1][t / 4], v1[0], v1[1]);
+                        } else {
+                            codes2<CODE, false>(vr[2 * e][t / 4], v0[0], v0[1]);
+                            codes2<CODE, false>(vr[2 * e + 1][t / 4], v1[0], v1[1]);
+                        }
+                        f[e] = high_halves(v0[t & 1], v1[t & 1]);
+                    } else {
+                        f[e] = __builtin_amdgcn_perm(vr[2 * e + 1][t / 2], vr[2 * e][t / 2],
+                                                     t & 1 ? 0x07060302u : 0x05040100u);
+                    }
+                }
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        f[e] &= keep[e];
+                    if (CODE != EP_I8 && ragged) {
+                        u32x4_t odd;
+                        uint32_t some = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t z = ((f[e] & VOP::kExp) == VOP::kExp ? 0xffffu : 0u) |
+                                               ((f[e] >> 16 & VOP::kExp) == VOP::kExp ? 0xffff0000u : 0u);
+                            odd[e] = z & (VOP::kOne | VOP::kOne << 16);
+                            f[e] &= ~z;
+                            some |= z;
+                        }
+                        if (__any(some != 0))
+#pragma unroll
+                            for (int mt = 0; mt < MT; ++mt) {
+                                u32x4_t one;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    one[e] = (seen[mt] >> (2 * e) & 1 ? VOP::kOne : 0u) |
+                                             (seen[mt] >> (2 * e + 1) & 1 ? VOP::kOne << 16 : 0u);
+                                const f32x4_t hits = VOP::mfma(odd, one, (f32x4_t){0, 0, 0, 0});
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    o[mt][t][i] = hits[i] > 0.0f ? nan : o[mt][t][i];
+                            }
+                    }
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+                    o[mt][t] = VOP::mfma(f, pl[mt], VOP::mfma(f, ph[mt], o[mt][t]));
+            }
+            load_v();
+        }
+
+        // ---- the waves' parts of the piece
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            l[mt] = xor32_sum(xor16_sum(l[mt]));
+            if (g == 0) {
+                s_m[wave][16 * mt + n] = m[mt];
+                s_l[wave][16 * mt + n] = l[mt];
+            }
+        }
+        __syncthreads();
+        const int rows = min(RM, a.rows - r0);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float top = s_m[0][16 * mt + n];
+#pragma unroll
+            for (int w = 1; w < kAttWaves; ++w)
+                top = fmaxf(top, s_m[w][16 * mt + n]);
+            const float f = __builtin_amdgcn_exp2f(m[mt] - (top == -INFINITY ? 0.0f : top));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < CW; t += 4)
+                    *(f32x4_t *)&s_o[wave][n][CW * (4 * g + i) + t] =
+                        (f32x4_t){o[mt][t][i] * f, o[mt][t + 1][i] * f, o[mt][t + 2][i] * f, o[mt][t + 3][i] * f};
+            __syncthreads();
+            for (int e = threadIdx.x; e < 16 * DP / 4; e += 64 * kAttWaves) {
+                const int row = e / (DP / 4), d = 4 * (e % (DP / 4)), r = 16 * mt + row;
+                if (r >= rows || d >= D)
+                    continue;
+                float mx = s_m[0][r], sum = 0.0f;
+#pragma unroll
+                for (int w = 1; w < kAttWaves; ++w)
+                    mx = fmaxf(mx, s_m[w][r]);
+                const float mu = mx == -INFINITY ? 0.0f : mx;
+                f32x4_t y = {0, 0, 0, 0};
+#pragma unroll
+                for (int w = 0; w < kAttWaves; ++w) {
+                    sum += s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - mu);
+                    y += *(const f32x4_t *)&s_o[w][row][d];
+                }
+                if (slot >= 0) {
+                    const int64_t at = (int64_t)slot * a.slot_rows + r;
+                    *(f32x4_t *)(a.part_o + at * D + d) = y;
+                    if (d == 0)
+                        a.part_ml[at] = make_float2(mx, sum);
+                    continue;
+                }
+                const int p = s_p[r], s = (r0 + r) / a.G, gq = r0 + r - s * a.G;
+                const float inv = 1.0f / sum;      // no weight at all (every score -inf) gives NaN
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    y[i] = p < 0 ? 0.0f : p >= a.cap || sum == 0.0f ? nan : y[i] * inv;
+                uint2 w;
+                w.x = QOP::pack(y[0], y[1]);
+                w.y = QOP::pack(y[2], y[3]);
+                *(uint2 *)((char *)a.out + 2 * (((b * a.tok.S + s) * H * a.G + h * a.G + gq) * D + d)) = w;
+            }
+            __syncthreads();
+        }
+    };
+
+    // ---- an even share of all tiles, in the order unit, cache head, tile.
+    // Every wave counts the units' tiles by itself, 64 units at a time.
+    uint32_t tiles = 0, upto = 0;        // of the lane's unit; of all units up to it in this block of 64
+    int64_t u0 = -1;
+    auto load_units = [&](int64_t from) {
+        u0 = from;
+        tiles = from + lane < a.units ? unit_tiles<RM>(a, from + lane) : 0u;
+        upto = tiles;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const uint32_t v = __shfl_up(upto, d, 64);
+            upto += lane >= d ? v : 0u;
+        }
+    };
+    int64_t total = 0;
+    if (a.workers)
+        for (int64_t from = 0; from < a.units; from += 64) {
+            load_units(from);
+            total += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * H;
+        }
+    else
+        total = 1;                       // a piece: the whole segment
+    const int64_t per = a.workers ? max((total + a.workers - 1) / a.workers, (int64_t)kAttWaves) : 1;
+    const int64_t begin = a.workers ? blockIdx.x * per : 0, stop = min(begin + per, total);
+    int64_t before = 0;                  // tiles ahead of this block of units
+    if (begin < stop && u0 > 0)
+        load_units(0);
+    for (int64_t f = begin; f < stop;) {
+        int64_t u = blockIdx.x / (unsigned)H, next = stop;
+        int h = (int)(blockIdx.x - u * H), t0 = 0, t1 = -1, slot = -1;
+        if (a.workers) {
+            uint64_t hit;
+            while (!(hit = __ballot(before + (int64_t)upto * H > f))) {
+                before += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * H;
+                if (u0 + 64 >= a.units)      // not reached while positions stay as they are
+                    return;
+                load_units(u0 + 64);
+            }
+            const int i = __builtin_ctzll(hit);
+            const uint32_t nt = (uint32_t)__builtin_amdgcn_readlane((int)tiles, i);
+            const int64_t seg0 = before + (int64_t)((uint32_t)__builtin_amdgcn_readlane((int)upto, i) - nt) * H;
+            u = u0 + i;
+            h = (int)((f - seg0) / nt);
+            const int64_t head0 = seg0 + (int64_t)h * nt;              // the segment's first tile
+            t0 = (int)(f - head0);
+            t1 = (int)min((int64_t)nt, stop - head0);
+            const int64_t w0 = head0 / per, w1 = min((head0 + nt - 1) / per, (int64_t)a.workers - 1);
+            if (t0 == 0 && threadIdx.x == 0)
+                a.desc[u * H + h] = make_int2((int)(2 * w0 + (head0 % per != 0)), (int)(w1 - w0 + 1));
+            // a worker's piece is kept in its first slot if it begins the worker's share, else in its second
+            slot = t0 == 0 && t1 == (int)nt ? -1 : 2 * (int)blockIdx.x + (f != begin);
+            next = head0 + t1;
+        }
+        piece(u, h, t0, t1, slot);
+        f = next;
+    }
+}
+
+// Instantiations of one pair of types, by D and rows (attend_gen_*.hip).
+template <typename QOP, int CODE, int MT>
+void attend_by_size(const AttendArgs &a, unsigned grid, hipStream_t st)
+{
+    constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
+    const int D = a.c.D;
+    if (D <= 64)
+        attend_kernel<QOP, CODE, 2, 4, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+    else if (!k8 && D <= 96)
+        attend_kernel<QOP, CODE, k8 ? 4 : 3, 8, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+    else if (D <= 128)
+        attend_kernel<QOP, CODE, 4, 8, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+    else if (D <= 192)
+        attend_kernel<QOP, CODE, 6, 16, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+    else
+        attend_kernel<QOP, CODE, 8, 16, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+}
+
+template <typename QOP, int CODE>
+void attend_by_rows(const AttendArgs &a, int mt, unsigned grid, hipStream_t st)
+{
+    if (mt == 1)
+        attend_by_size<QOP, CODE, 1>(a, grid, st);
+    else
+        attend_by_size<QOP, CODE, 2>(a, grid, st);
+}
+
+void attend_bf16(const AttendArgs &a, int mt, unsigned grid, hipStream_t st);
+void attend_f16(const AttendArgs &a, int mt, unsigned grid, hipStream_t st);
+void attend_i8(const AttendArgs &a, int q_dtype, int mt, unsigned grid, hipStream_t st);
+void attend_e4m3(const AttendArgs &a, int q_dtype, int mt, unsigned grid, hipStream_t st);
+
+}  // namespace ep

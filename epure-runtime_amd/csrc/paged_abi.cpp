@@ -186,6 +186,8 @@ int ep_paged_attention(const ep_heads *q, const ep_tokens *tokens, const ep_kv_c
         return EP_OK;
     if (!out)
         return set_error(EP_ERR_ARG, "attention: null output");
+    if (!aligned16(out) || !aligned16(workspace))
+        return set_error(EP_DECLINE_SHAPE, "attention: output and workspace must be 16-byte aligned");
     return launch_attend(q, tokens_of(tokens), c, scale, window, out, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
