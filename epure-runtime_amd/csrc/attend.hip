@@ -9,75 +9,68 @@ namespace ep {
 namespace {
 
 // Joins the pieces of a segment that several workers took, one query row a
-// workgroup: weights exp2(m_k - max) of the pieces' sums and outputs.
+// workgroup: D / 4 lanes take a piece, the next ones the next, each with its
+// own running maximum, so that sums, maxima and outputs load together.
 template <typename OP>
 __global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int RM)
 {
-    __shared__ float s_w[256], s_red[8];
+    __shared__ float s_m[64], s_l[64];
     __shared__ f32x4_t s_y[256];
-    const int Hq = a.c.heads * a.G, D = a.c.D, tid = threadIdx.x;
-    const int64_t token = blockIdx.x / (unsigned)Hq;
-    const int head = (int)(blockIdx.x - token * Hq), h = head / a.G, gq = head - h * a.G;
-    const int64_t b = token / a.tok.S;
-    const int s = (int)(token - b * a.tok.S), row = s * a.G + gq, block = row / RM, r = row - block * RM;
+    const uint32_t Hq = a.c.heads * a.G, D = a.c.D, tid = threadIdx.x;
+    const uint32_t token = blockIdx.x / Hq, head = blockIdx.x - token * Hq, h = head / a.G, gq = head - h * a.G;
+    const uint32_t b = token / (uint32_t)a.tok.S, s = token - b * (uint32_t)a.tok.S;
+    const uint32_t row = s * a.G + gq, block = row / RM, r = row - block * RM;
     const int2 d = a.desc[(b * a.blocks + block) * a.c.heads + h];
+    const int p = attend_position(a, b, s);
     if (d.y <= 1)       // one worker wrote the output
         return;
-    // piece 0 is in slot d.x, piece k in the first slot of its worker
-    auto slot = [&](int k) { return ((int64_t)(k == 0 ? d.x : (d.x & ~1) + 2 * k)) * a.slot_rows + r; };
-    auto block_max = [&](float v) {
-        v = wave_max(v);
-        if ((tid & 63) == 0)
-            s_red[tid >> 6] = v;
-        __syncthreads();
-        v = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-        __syncthreads();
-        return v;
-    };
-    float top = -INFINITY;
-    for (int k = tid; k < d.y; k += 256)
-        top = fmaxf(top, a.part_ml[slot(k)].x);
-    top = block_max(top);
-    const float base = top == -INFINITY ? 0.0f : top;
-    const int quads = D / 4, groups = 256 / quads, grp = tid / quads, c = 4 * (tid - grp * quads);
+    const uint32_t quads = D / 4, groups = 256 / quads, grp = tid / quads, c = 4 * (tid - grp * quads);
+    float m = -INFINITY, l = 0.0f;
     f32x4_t y = {0, 0, 0, 0};
-    float sum = 0.0f;
-    for (int k0 = 0; k0 < d.y; k0 += 256) {
-        if (k0 + tid < d.y) {
-            const float2 ml = a.part_ml[slot(k0 + tid)];
-            s_w[tid] = __builtin_amdgcn_exp2f(ml.x - base);
-            sum += ml.y * s_w[tid];
-        }
-        __syncthreads();
-        const int n = min(256, d.y - k0);
-        if (grp < groups)
-            for (int k = grp; k < n; k += groups) {
-                const f32x4_t v = *(const f32x4_t *)(a.part_o + slot(k0 + k) * D + c);
+    auto add = [&](float m2, float l2, f32x4_t y2) {
+        const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+        m = top;
+        l = l * f + l2 * f2;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    y[i] = fmaf(v[i], s_w[k], y[i]);
+        for (int i = 0; i < 4; ++i)
+            y[i] = y[i] * f + y2[i] * f2;
+    };
+    if (grp < groups)
+        for (int k0 = grp; k0 < d.y; k0 += 4 * groups) {
+            float2 ml[4];
+            f32x4_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // piece 0 is in slot d.x, piece k in the first slot of its worker; past the end the last again
+                const int k = min(k0 + i * (int)groups, d.y - 1);
+                const int64_t at = (int64_t)(k == 0 ? d.x : (d.x & ~1) + 2 * k) * a.slot_rows + r;
+                ml[i] = a.part_ml[at];
+                v[i] = *(const f32x4_t *)(a.part_o + at * D + c);
             }
-        __syncthreads();
-    }
-    sum = wave_sum(sum);
-    if ((tid & 63) == 0)
-        s_red[tid >> 6] = sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (k0 + i * (int)groups < d.y)
+                    add(ml[i].x, ml[i].y, v[i]);
+        }
     s_y[tid] = y;
+    if (grp < groups && c == 0) {
+        s_m[grp] = m;
+        s_l[grp] = l;
+    }
     __syncthreads();
     if (grp != 0)
         return;
-    sum = (s_red[0] + s_red[1]) + (s_red[2] + s_red[3]);
-    for (int k = 1; k < groups; ++k)
-        y += s_y[k * quads + tid];
-    const int p = attend_position(a, b, s);
-    const float inv = 1.0f / sum;
+    for (uint32_t k = 1; k < groups && (int)k < d.y; ++k)
+        add(s_m[k], s_l[k], s_y[k * quads + tid]);
+    const float inv = 1.0f / l;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        y[i] = p < 0 ? 0.0f : p >= a.cap || sum == 0.0f ? __uint_as_float(0x7fc00000u) : y[i] * inv;
+        y[i] = p < 0 ? 0.0f : p >= a.cap || l == 0.0f ? __uint_as_float(0x7fc00000u) : y[i] * inv;
     uint2 w;
     w.x = OP::pack(y[0], y[1]);
     w.y = OP::pack(y[2], y[3]);
-    *(uint2 *)((char *)a.out + 2 * ((token * Hq + head) * D + c)) = w;
+    *(uint2 *)((char *)a.out + 2 * ((int64_t)blockIdx.x * D + c)) = w;
 }
 
 struct Plan {
@@ -89,7 +82,8 @@ struct Plan {
 constexpr size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 // Segments of few tiles go to a workgroup each; else all tiles are shared
-// evenly among `workers` and the pieces joined.
+// evenly among `workers` and the pieces joined (where 32 bits count all
+// tiles that the table could hold).
 Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c)
 {
     Plan p{};
@@ -98,8 +92,8 @@ Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c)
     const int rm = 16 * p.mt;
     p.segments = tok.B * ((rows + rm - 1) / rm) * c.heads;
     const int64_t tiles = (tok.width << c.page_shift) / kAttTile;
-    if (tiles > 2 * kAttWaves) {
-        p.workers = 256 * 3;
+    if (tiles > 2 * kAttWaves && p.segments < 0x40000000 && tiles + kAttPiece < 0xffff0000u / p.segments) {
+        p.workers = 256 * attend_occupancy(c.D <= 64 ? 4 : c.D <= 128 ? 8 : 16, p.mt);
         const size_t slots = (size_t)2 * p.workers * (rows < rm ? rows : rm);
         p.desc = up16(p.segments * sizeof(int2));
         p.ml = up16(slots * sizeof(float2));
@@ -144,7 +138,7 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
     a.G = q->heads / c.heads;
     a.rows = (int)rows;
     a.blocks = (int)((rows + rm - 1) / rm);
-    a.units = tok.B * a.blocks;
+    a.units = (uint32_t)(tok.B * a.blocks);
     a.workers = p.workers;
     a.slot_rows = (int)(rows < rm ? rows : rm);
     a.desc = (int2 *)ws;

@@ -40,6 +40,7 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kAttTile = 32;             // positions a wave takes at a time
 constexpr int kAttWaves = 4;             // waves of a workgroup: they take tiles in turn
+constexpr int kAttPiece = 6;             // tiles' time that beginning and ending a piece takes
 constexpr int kAttOut = 0x40000000;      // an offset past every descriptor below: reads zeros
 
 struct AttendArgs {
@@ -53,13 +54,21 @@ struct AttendArgs {
     void *out;
     int G, rows;             // query heads a cache head; rows of a sequence on one cache head (S G)
     int blocks;              // units of a sequence
-    int64_t units;
+    uint32_t units;
     int workers;             // workgroups that share all tiles evenly; 0: one workgroup a segment
     int slot_rows;           // rows kept of a piece: min(rows, 16 MT)
     int2 *desc;              // [segments]: first slot, pieces
     float2 *part_ml;         // [2 workers][slot_rows]: maximum, sum
     float *part_o;           // [2 workers][slot_rows][D]
 };
+
+// v, computed anew where it is used: what follows from it is not kept in
+// registers across the loops.
+EP_DEV int opaque(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 EP_DEV int dpp_row_max(int v)
 {
@@ -81,21 +90,28 @@ EP_DEV int attend_position(const AttendArgs &a, int64_t b, int s)
 EP_DEV int first_seen(const AttendArgs &a, int p) { return p >= a.window ? p - a.window + 1 : 0; }
 
 // Tiles that the rows of unit u reach (one at least: its outputs are written
-// with that tile).
+// with that tile), and the first of them.
 template <int RM>
-EP_DEV uint32_t unit_tiles(const AttendArgs &a, int64_t u)
+EP_DEV uint32_t unit_tiles(const AttendArgs &a, uint32_t u, uint32_t &first)
 {
-    const int64_t b = u / a.blocks;
+    const uint32_t b = u / (uint32_t)a.blocks;
     const int r0 = (int)(u - b * a.blocks) * RM, r1 = min(r0 + RM, a.rows);
+    const int s0 = (uint32_t)r0 / (uint32_t)a.G, s1 = (uint32_t)(r1 - 1) / (uint32_t)a.G;
     int lo = a.cap, hi = -1;
-    for (int s = r0 / a.G; s <= (r1 - 1) / a.G; ++s) {
-        const int p = attend_position(a, b, s);
-        if (p >= 0 && p < a.cap) {
-            hi = max(hi, p);
-            lo = min(lo, first_seen(a, p));
-        }
+    for (int s = s0; s <= s1; s += 4) {
+        int p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)      // four loads in flight; the last token again past the end
+            p[i] = attend_position(a, b, min(s + i, s1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (p[i] >= 0 && p[i] < a.cap) {
+                hi = max(hi, p[i]);
+                lo = min(lo, first_seen(a, p[i]));
+            }
     }
-    return hi < 0 ? 1u : (uint32_t)(hi / kAttTile - lo / kAttTile + 1);
+    first = hi < 0 ? 0u : (uint32_t)(lo / kAttTile);
+    return hi < 0 ? 1u : (uint32_t)(hi / kAttTile) - first + 1;
 }
 
 // 16-bit arithmetic of a product's operands.
@@ -190,11 +206,14 @@ EP_DEV __amdgpu_buffer_rsrc_t tile_rsrc(const void *base, int64_t byte, bool ok,
     return buffer_rsrc((const char *)base + (ok ? byte : 0), ok ? (uint32_t)bytes : 0u);
 }
 
+// Workgroups of a kernel that a compute unit holds (waves of a SIMD).
+constexpr int attend_occupancy(int CW, int MT) { return CW == 4 ? (MT == 1 ? 3 : 2) : CW == 8 ? 2 : 1; }
+
 // QOP: type of the queries; CODE: EP_I8, EP_E4M3, or QOP's type.  KS: steps of
 // 32 values of a head, CW: output columns a lane (16 CW >= D), MT: 16-row
 // tiles of query rows.
 template <typename QOP, int CODE, int KS, int CW, int MT>
-__global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
+__global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) attend_kernel(AttendArgs a)
 {
     constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
     constexpr int ES = k8 ? 1 : 2, KL = k8 ? KS / 2 : KS, RM = 16 * MT, DP = 16 * CW, VW = CW * ES / 4;
@@ -221,19 +240,48 @@ __global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
     for (int i = 0; i < 4; ++i)
         voff[i] = CW * n < D ? ((4 * g + i) * D + CW * n) * ES : kAttOut;
 
-    // ---- one piece: tiles [t0, t1) of a segment, counted from its first;
-    // t1 < 0: all of them.  slot < 0: the outputs are written.
-    auto piece = [&](int64_t u, int h, int t0, int t1, int slot) {
-        const int64_t b = u / a.blocks;
-        const int r0 = (int)(u - b * a.blocks) * RM;
-        int first[MT], last[MT];
+    // ---- one piece: tiles [t0, t1) of the positions; t0 < 0: all that the
+    // unit's rows reach.  slot < 0: the outputs are written.
+    auto piece = [&](uint32_t u, int h, int t0, int t1, int slot) {
+        const uint32_t ub = u / (uint32_t)a.blocks;
+        const int r0 = (int)(u - ub * a.blocks) * RM;
+        const int64_t b = ub;
+        const int lx = opaque(lane), ln = lx & 15, lg = lx >> 4;
+        const int32_t *table = a.tok.table + b * a.tok.table_stride;
+        auto load_ids = [&](int j) {
+            const int64_t at = (int64_t)(j * kAttTile + 16 * (lane & 1)) >> a.c.page_shift;
+            return a.tok.width > 0 ? table[at < a.tok.width ? at : a.tok.width - 1] : -1;
+        };
+        // Pages, positions and queries load together where the first tile is
+        // known: a share's piece, or no window.
+        const bool known = t0 >= 0 || a.window >= a.cap;
+        int j = max(t0, 0) + wave, ids = 0;
+        if (known)
+            ids = load_ids(j);
+        int pos[MT], first[MT], last[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const int row = r0 + 16 * mt + ln;
+            pos[mt] = row < a.rows ? attend_position(a, b, (uint32_t)row / (uint32_t)a.G) : -1;
+        }
+        __builtin_amdgcn_sched_barrier(0);       // loads return in order: the positions' wait must not cover the queries
         u32x4_t q[MT][KS];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const int row = min(r0 + 16 * mt + ln, a.rows - 1);
+            const int s = (uint32_t)row / (uint32_t)a.G, gq = row - s * a.G;
+            const char *src = (const char *)a.q + 2 * (b * a.q_sb + s * a.q_ss + (int64_t)(h * a.G + gq) * a.q_sh);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const int d = k8 ? 64 * (k / 2) + 16 * lg + 8 * (k & 1) : 32 * k + 8 * lg;
+                q[mt][k] = *(const u32x4_t *)(src + 2 * (d < D ? d : 0));
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
         int lo = -a.cap, hi = -1, in_lo = 0, in_hi = -a.cap;     // over the rows: seen by any (lo negated), by all
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            const int row = r0 + 16 * mt + n;
-            const int s = min(row, a.rows - 1) / a.G, gq = row - s * a.G;
-            const int p = row < a.rows ? attend_position(a, b, s) : -1;
+            const int p = pos[mt];
             const bool some = p >= 0 && p < a.cap;
             first[mt] = some ? first_seen(a, p) : a.cap;
             last[mt] = some ? p : -1;
@@ -241,29 +289,21 @@ __global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
             hi = max(hi, last[mt]);
             in_lo = max(in_lo, some ? first[mt] : 0);
             in_hi = max(in_hi, some ? -p : -a.cap);
-            const char *src = (const char *)a.q + 2 * (b * a.q_sb + s * a.q_ss + (int64_t)(h * a.G + gq) * a.q_sh);
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const int d = k8 ? 64 * (k / 2) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g;
-                q[mt][k] = row < a.rows && d < D ? *(const u32x4_t *)(src + 2 * d) : (u32x4_t){0, 0, 0, 0};
-            }
-            if (wave == 0 && g == 0)
-                s_p[16 * mt + n] = p;
+            if (wave == 0 && lg == 0)
+                s_p[16 * mt + ln] = p;
         }
         lo = -dpp_row_max(lo);
         hi = dpp_row_max(hi);
         in_lo = dpp_row_max(in_lo);
         in_hi = -dpp_row_max(in_hi);
         const bool ragged = lo != in_lo || hi != in_hi;     // rows differ in what they see
-        const int tile0 = hi < 0 ? 0 : lo / kAttTile;
-        const int end = t1 < 0 ? (hi < 0 ? 1 : hi / kAttTile + 1) : tile0 + t1;
+        const int end = t0 >= 0 ? t1 : hi < 0 ? 1 : hi / kAttTile + 1;
+        if (!known) {
+            j = (hi < 0 ? 0 : lo / kAttTile) + wave;
+            ids = load_ids(j);
+        }
 
         // ---- loads
-        const int32_t *table = a.tok.table + b * a.tok.table_stride;
-        auto load_ids = [&](int j) {
-            const int64_t at = (int64_t)(j * kAttTile + 16 * (lane & 1)) >> a.c.page_shift;
-            return a.tok.width > 0 ? table[at < a.tok.width ? at : a.tok.width - 1] : -1;
-        };
         u32x4_t kr[2][KL];
         uint32_t vr[8][VW];
         float ks[8], vs[8];
@@ -336,12 +376,22 @@ __global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
             for (int t = 0; t < CW; ++t)
                 o[mt][t] = (f32x4_t){0, 0, 0, 0};
         }
-        int j = tile0 + t0 + wave;
-        int ids = load_ids(j);
         locate(ids, j);
         ids = load_ids(j + kAttWaves);
+        __builtin_amdgcn_sched_barrier(0);
         load_k();
+        __builtin_amdgcn_sched_barrier(0);       // loads return in order: the keys' wait must not cover the values
         load_v();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const int d = k8 ? 64 * (k / 2) + 16 * lg + 8 * (k & 1) : 32 * k + 8 * lg;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    q[mt][k][i] = d < D ? q[mt][k][i] : 0u;
+            }
         for (; j < end; j += kAttWaves) {
             const int j0 = j * kAttTile;
             const bool bad0 = !good[0], bad1 = !good[1];
@@ -371,9 +421,11 @@ __global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
                 for (int e = 0; e < 8; ++e)
                     x[mt][e] = sc[mt][e / 4][e % 4] * (k8 ? ks[e] * a.scale : a.scale);
             // the next tile's keys (none past the end: empty descriptors)
+            __builtin_amdgcn_sched_barrier(0);
             locate(ids, j + kAttWaves);
             ids = load_ids(j + 2 * kAttWaves);
             load_k();
+            __builtin_amdgcn_sched_barrier(0);
 
             // A tile that some row sees in part (or that names a page the pool
             // lacks: its scores are NaN) masks its scores one by one.
@@ -428,16 +480,9 @@ __global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
             // Values: what no row sees becomes zero (its weights are zero, and
             // zero times a NaN is NaN); what some rows see and others not is
             // taken out if it is not finite, and added where it is seen.
-            uint32_t keep[4];
-            if (edge)
+            u32x4_t f[CW];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int p = j0 + 16 * (e / 2) + 4 * g + 2 * (e % 2);
-                    keep[e] = (p >= lo && p <= hi ? 0xffffu : 0u) | (p + 1 >= lo && p + 1 <= hi ? 0xffff0000u : 0u);
-                }
-#pragma unroll
-            for (int t = 0; t < CW; ++t) {
-                u32x4_t f;
+            for (int t = 0; t < CW; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (k8) {
@@ -449,75 +494,89 @@ __global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
                             codes2<CODE, false>(vr[2 * e][t / 4], v0[0], v0[1]);
                             codes2<CODE, false>(vr[2 * e + 1][t / 4], v1[0], v1[1]);
                         }
-                        f[e] = high_halves(v0[t & 1], v1[t & 1]);
+                        f[t][e] = high_halves(v0[t & 1], v1[t & 1]);
                     } else {
-                        f[e] = __builtin_amdgcn_perm(vr[2 * e + 1][t / 2], vr[2 * e][t / 2],
-                                                     t & 1 ? 0x07060302u : 0x05040100u);
+                        f[t][e] = __builtin_amdgcn_perm(vr[2 * e + 1][t / 2], vr[2 * e][t / 2],
+                                                        t & 1 ? 0x07060302u : 0x05040100u);
                     }
                 }
-                if (edge) {
+            if (edge) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        f[e] &= keep[e];
-                    if (CODE != EP_I8 && ragged) {
+                for (int e = 0; e < 4; ++e) {
+                    const int p = j0 + 16 * (e / 2) + 4 * g + 2 * (e % 2);
+                    const uint32_t keep = (p >= lo && p <= hi ? 0xffffu : 0u) |
+                                          (p + 1 >= lo && p + 1 <= hi ? 0xffff0000u : 0u);
+#pragma unroll
+                    for (int t = 0; t < CW; ++t)
+                        f[t][e] &= keep;
+                }
+                if (CODE != EP_I8 && ragged) {
+                    u32x4_t one[MT];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            one[mt][e] = (seen[mt] >> (2 * e) & 1 ? VOP::kOne : 0u) |
+                                         (seen[mt] >> (2 * e + 1) & 1 ? VOP::kOne << 16 : 0u);
+#pragma unroll
+                    for (int t = 0; t < CW; ++t) {
                         u32x4_t odd;
                         uint32_t some = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint32_t z = ((f[e] & VOP::kExp) == VOP::kExp ? 0xffffu : 0u) |
-                                               ((f[e] >> 16 & VOP::kExp) == VOP::kExp ? 0xffff0000u : 0u);
+                            const uint32_t z = ((f[t][e] & VOP::kExp) == VOP::kExp ? 0xffffu : 0u) |
+                                               ((f[t][e] >> 16 & VOP::kExp) == VOP::kExp ? 0xffff0000u : 0u);
                             odd[e] = z & (VOP::kOne | VOP::kOne << 16);
-                            f[e] &= ~z;
+                            f[t][e] &= ~z;
                             some |= z;
                         }
                         if (__any(some != 0))
 #pragma unroll
                             for (int mt = 0; mt < MT; ++mt) {
-                                u32x4_t one;
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    one[e] = (seen[mt] >> (2 * e) & 1 ? VOP::kOne : 0u) |
-                                             (seen[mt] >> (2 * e + 1) & 1 ? VOP::kOne << 16 : 0u);
-                                const f32x4_t hits = VOP::mfma(odd, one, (f32x4_t){0, 0, 0, 0});
+                                const f32x4_t hits = VOP::mfma(odd, one[mt], (f32x4_t){0, 0, 0, 0});
 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
                                     o[mt][t][i] = hits[i] > 0.0f ? nan : o[mt][t][i];
                             }
                     }
                 }
+            }
+#pragma unroll
+            for (int t = 0; t < CW; ++t)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
-                    o[mt][t] = VOP::mfma(f, pl[mt], VOP::mfma(f, ph[mt], o[mt][t]));
-            }
+                    o[mt][t] = VOP::mfma(f[t], pl[mt], VOP::mfma(f[t], ph[mt], o[mt][t]));
+            __builtin_amdgcn_sched_barrier(0);
             load_v();
         }
 
         // ---- the waves' parts of the piece
+        const int ex = opaque(lane), en = ex & 15, eg = ex >> 4, tid = opaque(threadIdx.x);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             l[mt] = xor32_sum(xor16_sum(l[mt]));
-            if (g == 0) {
-                s_m[wave][16 * mt + n] = m[mt];
-                s_l[wave][16 * mt + n] = l[mt];
+            if (eg == 0) {
+                s_m[wave][16 * mt + en] = m[mt];
+                s_l[wave][16 * mt + en] = l[mt];
             }
         }
         __syncthreads();
         const int rows = min(RM, a.rows - r0);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            float top = s_m[0][16 * mt + n];
+            float top = s_m[0][16 * mt + en];
 #pragma unroll
             for (int w = 1; w < kAttWaves; ++w)
-                top = fmaxf(top, s_m[w][16 * mt + n]);
+                top = fmaxf(top, s_m[w][16 * mt + en]);
             const float f = __builtin_amdgcn_exp2f(m[mt] - (top == -INFINITY ? 0.0f : top));
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int t = 0; t < CW; t += 4)
-                    *(f32x4_t *)&s_o[wave][n][CW * (4 * g + i) + t] =
+                    *(f32x4_t *)&s_o[wave][en][CW * (4 * eg + i) + t] =
                         (f32x4_t){o[mt][t][i] * f, o[mt][t + 1][i] * f, o[mt][t + 2][i] * f, o[mt][t + 3][i] * f};
             __syncthreads();
-            for (int e = threadIdx.x; e < 16 * DP / 4; e += 64 * kAttWaves) {
+            for (int e = tid; e < 16 * DP / 4; e += 64 * kAttWaves) {
                 const int row = e / (DP / 4), d = 4 * (e % (DP / 4)), r = 16 * mt + row;
                 if (r >= rows || d >= D)
                     continue;
@@ -539,7 +598,7 @@ __global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
                         a.part_ml[at] = make_float2(mx, sum);
                     continue;
                 }
-                const int p = s_p[r], s = (r0 + r) / a.G, gq = r0 + r - s * a.G;
+                const int p = s_p[r], s = (uint32_t)(r0 + r) / (uint32_t)a.G, gq = r0 + r - s * a.G;
                 const float inv = 1.0f / sum;      // no weight at all (every score -inf) gives NaN
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -553,61 +612,77 @@ __global__ void __launch_bounds__(64 * kAttWaves) attend_kernel(AttendArgs a)
         }
     };
 
-    // ---- an even share of all tiles, in the order unit, cache head, tile.
-    // Every wave counts the units' tiles by itself, 64 units at a time.
-    uint32_t tiles = 0, upto = 0;        // of the lane's unit; of all units up to it in this block of 64
-    int64_t u0 = -1;
-    auto load_units = [&](int64_t from) {
-        u0 = from;
-        tiles = from + lane < a.units ? unit_tiles<RM>(a, from + lane) : 0u;
-        upto = tiles;
+    // ---- one segment a workgroup (workers == 0), or an even share of all tiles
+    // in the order unit, cache head, tile.  Every wave counts the units' tiles by
+    // itself, 64 units at a time; the host bounds all counts to 32 bits.
+    const uint32_t units = a.units;
+    auto at_lane = [](uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); };
+    uint32_t u = blockIdx.x / (uint32_t)H;
+    int h = (int)(blockIdx.x - u * H), t0 = -1, t1 = 0, slot = -1;
+    uint32_t f = 0, begin = 0, stop = 1, per = 1, total = 0;
+    uint32_t first = 0, cost = 0, upto = 0;        // of the lane's unit; of all units up to it in this block of 64
+    uint32_t u0 = 0, before = 0;         // the block's first unit; tiles ahead of it
+    bool counting = a.workers > 0, load = counting;
+    for (;;) {
+        if (load) {
+            cost = u0 + lane < units ? unit_tiles<RM>(a, u0 + lane, first) + kAttPiece : 0u;
+            upto = cost;
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t v = __shfl_up(upto, d, 64);
-            upto += lane >= d ? v : 0u;
+            for (int d = 1; d < 64; d *= 2) {
+                const uint32_t v = __shfl_up(upto, d, 64);
+                upto += lane >= d ? v : 0u;
+            }
+            load = false;
         }
-    };
-    int64_t total = 0;
-    if (a.workers)
-        for (int64_t from = 0; from < a.units; from += 64) {
-            load_units(from);
-            total += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * H;
+        if (counting) {
+            total += at_lane(upto, 63) * H;
+            u0 += 64;
+            load = u0 < units;
+            if (load)
+                continue;
+            counting = false;
+            per = max((total + a.workers - 1) / (uint32_t)a.workers, (uint32_t)kAttWaves);
+            f = begin = min(blockIdx.x * per, total);
+            stop = min(begin + per, total);
+            u0 = 0;
+            load = units > 64;
+            if (load && f < stop)
+                continue;
         }
-    else
-        total = 1;                       // a piece: the whole segment
-    const int64_t per = a.workers ? max((total + a.workers - 1) / a.workers, (int64_t)kAttWaves) : 1;
-    const int64_t begin = a.workers ? blockIdx.x * per : 0, stop = min(begin + per, total);
-    int64_t before = 0;                  // tiles ahead of this block of units
-    if (begin < stop && u0 > 0)
-        load_units(0);
-    for (int64_t f = begin; f < stop;) {
-        int64_t u = blockIdx.x / (unsigned)H, next = stop;
-        int h = (int)(blockIdx.x - u * H), t0 = 0, t1 = -1, slot = -1;
+        if (f >= stop)
+            return;
         if (a.workers) {
-            uint64_t hit;
-            while (!(hit = __ballot(before + (int64_t)upto * H > f))) {
-                before += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63) * H;
-                if (u0 + 64 >= a.units)      // not reached while positions stay as they are
+            const uint64_t hit = __ballot(before + upto * H > f);
+            if (!hit) {
+                before += at_lane(upto, 63) * H;
+                u0 += 64;
+                load = true;
+                if (u0 >= units)           // not reached while positions stay as they are
                     return;
-                load_units(u0 + 64);
+                continue;
             }
             const int i = __builtin_ctzll(hit);
-            const uint32_t nt = (uint32_t)__builtin_amdgcn_readlane((int)tiles, i);
-            const int64_t seg0 = before + (int64_t)((uint32_t)__builtin_amdgcn_readlane((int)upto, i) - nt) * H;
+            const uint32_t n1 = at_lane(cost, i), seg0 = before + (at_lane(upto, i) - n1) * H;
             u = u0 + i;
-            h = (int)((f - seg0) / nt);
-            const int64_t head0 = seg0 + (int64_t)h * nt;              // the segment's first tile
-            t0 = (int)(f - head0);
-            t1 = (int)min((int64_t)nt, stop - head0);
-            const int64_t w0 = head0 / per, w1 = min((head0 + nt - 1) / per, (int64_t)a.workers - 1);
-            if (t0 == 0 && threadIdx.x == 0)
-                a.desc[u * H + h] = make_int2((int)(2 * w0 + (head0 % per != 0)), (int)(w1 - w0 + 1));
-            // a worker's piece is kept in its first slot if it begins the worker's share, else in its second
-            slot = t0 == 0 && t1 == (int)nt ? -1 : 2 * (int)blockIdx.x + (f != begin);
-            next = head0 + t1;
-        }
+            h = (int)((f - seg0) / n1);
+            const uint32_t next = seg0 + (h + 1) * n1, head0 = next - n1 + kAttPiece;     // the segment's tiles: [head0, next)
+            const uint32_t f0 = max(f, head0), f1 = min(next, stop);
+            f = f1;
+            if (f0 >= f1)
+                continue;                  // a share that ends within what a segment's beginning takes
+            const int base = (int)at_lane(first, i) - (int)head0;
+            t0 = base + (int)f0;
+            t1 = base + (int)f1;
+            if (f0 == head0 && threadIdx.x == 0) {
+                const uint32_t w1 = min((next - 1) / per, (uint32_t)a.workers - 1);
+                a.desc[u * H + h] = make_int2(2 * (int)blockIdx.x + (head0 - kAttPiece >= begin), (int)(w1 - blockIdx.x + 1));
+            }
+            // A piece that begins before its worker's share does is kept in the
+            // worker's first slot, else in its second.
+            slot = f0 == head0 && f1 == next ? -1 : 2 * (int)blockIdx.x + (head0 - kAttPiece >= begin);
+        } else
+            f = stop;
         piece(u, h, t0, t1, slot);
-        f = next;
     }
 }
 
