@@ -4,10 +4,21 @@
 //
 // One kernel shape serves all three: a row is one head's D values of one
 // token, a lane holds 16 of them as two 16-byte chunks, and D / 16 lanes
-// (rounded up to a power of two) hold a row.  With pairs (i, i + dim / 2) a
-// lane's two chunks are the two halves of its pairs, so a turn needs nothing
-// from another lane, and a row's largest magnitude is a few lane exchanges
-// within 16 lanes.  All of it is bound by the bytes of the rows.
+// (rounded up to a power of two) hold a row.  The chunks lie dim / 2 apart
+// (D / 2 without a turn): with pairs (i, i + dim / 2) a turn needs nothing
+// from another lane, in either layout neighbouring lanes load and store
+// neighbouring chunks, and a row's largest magnitude is a few lane exchanges
+// within 16 lanes.
+//
+// All of it is bound by the bytes of the rows.  Inputs are read once, and
+// large outputs leave the caches before they are read again, so both go past
+// them as non-temporal accesses: 16384 tokens of 32 + 8 heads of 128 turn in
+// 59 us (5.7 TB/s; 70 with plain accesses), 8 x 4096 rows of 8 heads are read
+// out of an int8 cache in 35 us (50), two prompts of 4096 tokens enter an
+// e4m3 cache and are read back in 50 us (60).  Four rows of one token a group
+// of lanes, with one look-up of position, page and angles, were slower: lanes
+// of a wave then hold queries, keys and values at once and take every path
+// (those prompts 124 us), and one token's call grows with the code it fetches.
 #include "ep_common.h"
 #include "ep_internal.h"
 #include "ep_paged.h"
@@ -35,13 +46,12 @@ struct Chunks {
     EP_DEV int at(int e) const { return e < 8 ? a + e : b + e - 8; }
 };
 
-// Lane u's chunks where whole chunks can be loaded: the two halves of the
-// pairs (i, i + dim / 2), else 16 adjacent values.
-EP_DEV Chunks chunks_of(int u, const Turn &t, bool turned)
+// Lane u's chunks where whole chunks can be loaded: half of the turned values
+// apart (dim 0: no turn), or half of the others.
+EP_DEV Chunks chunks_of(int u, int dim, int D)
 {
-    if (turned && !t.interleaved && u < t.dim / 16)
-        return {8 * u, 8 * u + t.dim / 2};
-    return {16 * u, 16 * u + 8};
+    const int w = u - dim / 16;
+    return w < 0 ? Chunks{8 * u, 8 * u + dim / 2} : Chunks{dim + 8 * w, dim + 8 * w + (D - dim) / 2};
 }
 
 template <typename T>
@@ -62,24 +72,37 @@ EP_DEV f16_t from_f32<f16_t>(float v) { return (f16_t)v; }
 template <>
 EP_DEV uint16_t from_f32<uint16_t>(float v) { return f32_to_bf16(v); }
 
-// 8 values from or to 16-byte aligned (32 for f32) memory.
+// 8 values from or to 16-byte aligned memory; loads of what is read once.
 template <typename T>
 EP_DEV void load8(const T *p, float *v)
 {
     T r[8];
-    __builtin_memcpy(r, __builtin_assume_aligned(p, 16), sizeof r);
+    u32x4_t w[sizeof r / 16];
+#pragma unroll
+    for (unsigned i = 0; i < sizeof r / 16; ++i)
+        w[i] = __builtin_nontemporal_load((const u32x4_t *)p + i);
+    __builtin_memcpy(r, w, sizeof r);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         v[i] = to_f32<T>(r[i]);
 }
-template <typename T>
+// STREAM: past the caches (a parameter of the kernels: a branch's two stores
+// would be merged into one plain store).
+template <bool STREAM, typename T>
 EP_DEV void store8(T *p, const float *v)
 {
     T r[8];
+    u32x4_t w[sizeof r / 16];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         r[i] = from_f32<T>(v[i]);
-    __builtin_memcpy(__builtin_assume_aligned(p, 16), r, sizeof r);
+    __builtin_memcpy(w, r, sizeof r);
+#pragma unroll
+    for (unsigned i = 0; i < sizeof r / 16; ++i)
+        if constexpr (STREAM)
+            __builtin_nontemporal_store(w[i], (u32x4_t *)p + i);
+        else
+            ((u32x4_t *)p)[i] = w[i];
 }
 
 // (a cos - b sin, b cos + a sin), each product rounded before the sum: the
@@ -100,14 +123,18 @@ template <typename T, bool VEC>
 EP_DEV Chunks load_row(const T *x, int D, int u, const Turn &t, bool turned, int64_t p, float *v)
 {
     if constexpr (VEC) {
-        const Chunks ch = chunks_of(u, t, turned);
+        const Chunks ch = chunks_of(u, t.dim, D);
         load8(x + ch.a, v);
         load8(x + ch.b, v + 8);
         if (turned && 16 * u < t.dim) {
-            const float *cs = t.cos_t + p * (t.dim / 2) + 8 * u, *sn = t.sin_t + p * (t.dim / 2) + 8 * u;
+            // cosines and sines of the pairs of both chunks
+            const float *cs = t.cos_t + p * (t.dim / 2), *sn = t.sin_t + p * (t.dim / 2);
+            const int i0 = t.interleaved ? ch.a / 2 : ch.a, i1 = t.interleaved ? ch.b / 2 : ch.a + 4;
             float c[8], s[8];
-            load8(cs, c);
-            load8(sn, s);
+            __builtin_memcpy(c, __builtin_assume_aligned(cs + i0, 16), 16);
+            __builtin_memcpy(c + 4, __builtin_assume_aligned(cs + i1, 16), 16);
+            __builtin_memcpy(s, __builtin_assume_aligned(sn + i0, 16), 16);
+            __builtin_memcpy(s + 4, __builtin_assume_aligned(sn + i1, 16), 16);
             if (t.interleaved) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -142,12 +169,12 @@ EP_DEV Chunks load_row(const T *x, int D, int u, const Turn &t, bool turned, int
     }
 }
 
-template <typename T, bool VEC>
+template <bool VEC, bool STREAM, typename T>
 EP_DEV void store_row(T *y, int D, const Chunks &ch, const float *v)
 {
     if constexpr (VEC) {
-        store8(y + ch.a, v);
-        store8(y + ch.b, v + 8);
+        store8<STREAM>(y + ch.a, v);
+        store8<STREAM>(y + ch.b, v + 8);
     } else {
         for (int e = 0; e < 16; ++e)
             if (ch.at(e) < D)
@@ -216,24 +243,25 @@ struct Token {
     int64_t b, s, p;
 };
 
-EP_DEV Token token_at(const PagedTokens &t, int64_t i)
+EP_DEV Token token_at(const PagedTokens &t, uint32_t i)
 {
     Token k;
-    k.b = i / t.S;
-    k.s = i - k.b * t.S;
+    const uint32_t b = i / (uint32_t)t.S;
+    k.b = b;
+    k.s = i - b * (uint32_t)t.S;
     k.p = t.pos[k.b * t.pos_sb + k.s * t.pos_ss];
     return k;
 }
 
 // Which row a lane group of `lanes` works on: (token, head) of 256 / lanes
 // rows a workgroup.
-EP_DEV bool row_at(int64_t rows, int heads, int lanes, int64_t &token, int &head, int &u)
+EP_DEV bool row_at(uint32_t rows, int heads, int lanes, uint32_t &token, int &head, int &u)
 {
-    const int64_t r = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    const uint32_t r = blockIdx.x * (256u / lanes) + threadIdx.x / (uint32_t)lanes;
     u = threadIdx.x & (lanes - 1);
     if (r >= rows)
         return false;
-    token = r / heads;
+    token = r / (uint32_t)heads;
     head = (int)(r - token * heads);
     return true;
 }
@@ -243,14 +271,14 @@ struct RotateArgs {
     Turn turn;
     PagedTokens tok;
     void *q_out, *k_out;
-    int64_t rows;
+    uint32_t rows;
     int D, lanes;
 };
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool STREAM>
 __global__ void __launch_bounds__(256) rotate_kernel(RotateArgs a)
 {
-    int64_t token;
+    uint32_t token;
     int head, u;
     if (!row_at(a.rows, a.q.heads + a.k.heads, a.lanes, token, head, u) || 16 * u >= a.D)
         return;
@@ -258,7 +286,7 @@ __global__ void __launch_bounds__(256) rotate_kernel(RotateArgs a)
     const bool is_q = head < a.q.heads;
     const Rows &x = is_q ? a.q : a.k;
     const int h = is_q ? head : head - a.q.heads;
-    T *y = (T *)(is_q ? a.q_out : a.k_out) + (token * x.heads + h) * a.D;
+    T *y = (T *)(is_q ? a.q_out : a.k_out) + ((int64_t)token * x.heads + h) * a.D;
     float v[16];
     const bool ok = t.p >= 0 && t.p < a.turn.max_pos;
     const Chunks ch = load_row<T, VEC>((const T *)x.ptr + t.b * x.sb + t.s * x.ss + h * x.sh, a.D, u, a.turn, ok, t.p, v);
@@ -268,7 +296,7 @@ __global__ void __launch_bounds__(256) rotate_kernel(RotateArgs a)
         for (int e = 0; e < 16; ++e)
             v[e] = fill;
     }
-    store_row<T, VEC>(y, a.D, ch, v);
+    store_row<VEC, STREAM>(y, a.D, ch, v);
 }
 
 struct AppendArgs {
@@ -277,25 +305,28 @@ struct AppendArgs {
     PagedTokens tok;
     PagedCache c;
     void *q_out;
-    int64_t rows;
+    uint32_t rows;
     int lanes;
 };
 
-// The slot (row of [n_pages][page], times heads later) of position p, or
-// false: padding, past the table, or not a page.
+// Position p's page and row in it; false (and the pool's first row, which can
+// be read) for padding, past the table, or where the table names no page.
 EP_DEV bool slot_of(const PagedTokens &t, const PagedCache &c, int64_t b, int64_t p, int64_t &page, int &row)
 {
-    if (p < 0 || (p >> c.page_shift) >= t.width)
-        return false;
-    page = t.table[b * t.table_stride + (p >> c.page_shift)];
-    row = (int)(p & (c.page - 1));
-    return page >= 0 && page < c.n_pages;
+    const int64_t i = p >> c.page_shift;
+    int32_t id = -1;
+    if (p >= 0 && i < t.width)
+        id = t.table[b * t.table_stride + i];
+    const bool ok = id >= 0 && id < c.n_pages;
+    page = ok ? id : 0;
+    row = ok ? (int)(p & (c.page - 1)) : 0;
+    return ok;
 }
 
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool STREAM>
 __global__ void __launch_bounds__(256) append_kernel(AppendArgs a)
 {
-    int64_t token;
+    uint32_t token;
     int head, u;
     const int D = a.c.D, Hq = a.q.heads, Hk = a.c.heads;
     if (!row_at(a.rows, Hq + 2 * Hk, a.lanes, token, head, u))
@@ -319,7 +350,7 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a)
     }
     if (is_q) {
         if (mine)
-            store_row<T, VEC>((T *)a.q_out + (token * Hq + h) * D, D, ch, v);
+            store_row<VEC, STREAM>((T *)a.q_out + ((int64_t)token * Hq + h) * D, D, ch, v);
         return;
     }
     int64_t page = 0;
@@ -331,9 +362,9 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a)
     if (a.c.dtype == EP_F16 || a.c.dtype == EP_BF16) {
         if (mine) {
             if (a.c.dtype == EP_F16)
-                store_row<f16_t, true>((f16_t *)dst + at * D, D, ch, v);
+                store_row<true, false>((f16_t *)dst + at * D, D, ch, v);
             else
-                store_row<uint16_t, true>((uint16_t *)dst + at * D, D, ch, v);
+                store_row<true, false>((uint16_t *)dst + at * D, D, ch, v);
         }
         return;
     }
@@ -359,14 +390,14 @@ struct ReadArgs {
     PagedTokens tok;
     PagedCache c;
     void *k_out, *v_out;
-    int64_t rows;
+    uint32_t rows;
     int lanes;
 };
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ void __launch_bounds__(256) read_kernel(ReadArgs a)
 {
-    int64_t token;
+    uint32_t token;
     int head, u;
     const int D = a.c.D, Hk = a.c.heads;
     if (!row_at(a.rows, 2 * Hk, a.lanes, token, head, u) || 16 * u >= D)
@@ -374,37 +405,38 @@ __global__ void __launch_bounds__(256) read_kernel(ReadArgs a)
     const Token t = token_at(a.tok, token);
     const bool is_v = head >= Hk;
     const int h = is_v ? head - Hk : head;
-    float v[16];
+    const Chunks ch = chunks_of(u, 0, D);
     int64_t page;
     int row;
-    if (slot_of(a.tok, a.c, t.b, t.p, page, row)) {
-        const int64_t at = (page * Hk + h) * a.c.page + row;
-        const void *src = is_v ? a.c.v : a.c.k;
-        if (a.c.dtype == EP_F16 || a.c.dtype == EP_BF16) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (a.c.dtype == EP_F16)
-                    load8((const f16_t *)src + at * D + 16 * u + 8 * i, v + 8 * i);
-                else
-                    load8((const uint16_t *)src + at * D + 16 * u + 8 * i, v + 8 * i);
-            }
-        } else {
-            const float s = (is_v ? a.c.v_scale : a.c.k_scale)[at];
-            const u32x4_t w = *(const u32x4_t *)((const uint8_t *)src + at * D + 16 * u);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                decode4(w[i], a.c.dtype, v + 4 * i);
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                v[e] *= s;
-        }
+    const bool ok = slot_of(a.tok, a.c, t.b, t.p, page, row);
+    // Loaded either way, with no branch on ok: this compiler lost the value of
+    // D that the output's address needs, in the lanes that skipped such a branch.
+    const int64_t at = (page * Hk + h) * a.c.page + row;
+    const void *src = is_v ? a.c.v : a.c.k;
+    float v[16];
+    if (a.c.dtype == EP_F16) {
+        load8((const f16_t *)src + at * D + ch.a, v);
+        load8((const f16_t *)src + at * D + ch.b, v + 8);
+    } else if (a.c.dtype == EP_BF16) {
+        load8((const uint16_t *)src + at * D + ch.a, v);
+        load8((const uint16_t *)src + at * D + ch.b, v + 8);
     } else {
-        const float fill = t.p < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
+        const float s = (is_v ? a.c.v_scale : a.c.k_scale)[at];
+        uint32_t w[4];
+        __builtin_memcpy(w, __builtin_assume_aligned((const uint8_t *)src + at * D + ch.a, 8), 8);
+        __builtin_memcpy(w + 2, __builtin_assume_aligned((const uint8_t *)src + at * D + ch.b, 8), 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            decode4(w[i], a.c.dtype, v + 4 * i);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-            v[e] = fill;
+            v[e] *= s;
     }
-    store_row<T, true>((T *)(is_v ? a.v_out : a.k_out) + (token * Hk + h) * D, D, {16 * u, 16 * u + 8}, v);
+    const float fill = t.p < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        v[e] = ok ? v[e] : fill;
+    store_row<true, STREAM>((T *)(is_v ? a.v_out : a.k_out) + ((int64_t)token * Hk + h) * D, D, ch, v);
 }
 
 bool aligned(const void *p, int64_t n) { return ((uintptr_t)p % n) == 0; }
@@ -444,35 +476,51 @@ Turn turn_of(const ep_rotation *rot, int inverse)
     return Turn{rot->cos_t, rot->sin_t, rot->max_pos, rot->dim, rot->interleaved, inverse ? -1.0f : 1.0f};
 }
 
-int grid_of(int64_t rows, int lanes, unsigned &grid)
+// More than half of what the L2 caches hold together: their inputs pass there too.
+bool streams(int64_t values, int dtype) { return values * (dtype == EP_F32 ? 4 : 2) > (int64_t)16 << 20; }
+
+// Rows of a call (counted in 32 bits) and its grid.
+int grid_of(const PagedTokens &tok, int heads, int lanes, uint32_t &rows, unsigned &grid)
 {
-    const int64_t per = 256 / lanes, n = (rows + per - 1) / per;
-    if (n > 0x7fffffff)
-        return set_error(EP_DECLINE_SHAPE, "%lld rows are more than one launch takes", (long long)rows);
-    grid = (unsigned)n;
+    const int64_t n = tok.B * tok.S * heads, per = 256 / lanes;
+    if (n > 0xffffff00)
+        return set_error(EP_DECLINE_SHAPE, "%lld rows are more than one launch takes", (long long)n);
+    rows = (uint32_t)n;
+    grid = (unsigned)((n + per - 1) / per);
     return EP_OK;
 }
 
-template <bool VEC>
+template <bool VEC, bool STREAM>
 void rotate_typed(int dtype, unsigned grid, const RotateArgs &a, hipStream_t st)
 {
     if (dtype == EP_F32)
-        rotate_kernel<float, VEC><<<grid, 256, 0, st>>>(a);
+        rotate_kernel<float, VEC, STREAM><<<grid, 256, 0, st>>>(a);
     else if (dtype == EP_F16)
-        rotate_kernel<f16_t, VEC><<<grid, 256, 0, st>>>(a);
+        rotate_kernel<f16_t, VEC, STREAM><<<grid, 256, 0, st>>>(a);
     else
-        rotate_kernel<uint16_t, VEC><<<grid, 256, 0, st>>>(a);
+        rotate_kernel<uint16_t, VEC, STREAM><<<grid, 256, 0, st>>>(a);
 }
 
-template <bool VEC>
+template <bool VEC, bool STREAM>
 void append_typed(int dtype, unsigned grid, const AppendArgs &a, hipStream_t st)
 {
     if (dtype == EP_F32)
-        append_kernel<float, VEC><<<grid, 256, 0, st>>>(a);
+        append_kernel<float, VEC, STREAM><<<grid, 256, 0, st>>>(a);
     else if (dtype == EP_F16)
-        append_kernel<f16_t, VEC><<<grid, 256, 0, st>>>(a);
+        append_kernel<f16_t, VEC, STREAM><<<grid, 256, 0, st>>>(a);
     else
-        append_kernel<uint16_t, VEC><<<grid, 256, 0, st>>>(a);
+        append_kernel<uint16_t, VEC, STREAM><<<grid, 256, 0, st>>>(a);
+}
+
+template <bool STREAM>
+void read_typed(int dtype, unsigned grid, const ReadArgs &a, hipStream_t st)
+{
+    if (dtype == EP_F32)
+        read_kernel<float, STREAM><<<grid, 256, 0, st>>>(a);
+    else if (dtype == EP_F16)
+        read_kernel<f16_t, STREAM><<<grid, 256, 0, st>>>(a);
+    else
+        read_kernel<uint16_t, STREAM><<<grid, 256, 0, st>>>(a);
 }
 
 }  // namespace
@@ -481,17 +529,18 @@ int launch_rotate(const ep_heads *q, const ep_heads *k, const ep_rotation *rot, 
                   int inverse, void *q_out, void *k_out, hipStream_t stream)
 {
     RotateArgs a{rows_of(q), rows_of(k), turn_of(rot, inverse), tok, q_out, k_out, 0, (int)D, lanes_of(D)};
-    a.rows = tok.B * tok.S * (a.q.heads + a.k.heads);
     unsigned grid;
-    const int rc = grid_of(a.rows, a.lanes, grid);
+    const int rc = grid_of(tok, a.q.heads + a.k.heads, a.lanes, a.rows, grid);
     if (rc != EP_OK || a.rows == 0)
         return rc;
     const bool vec = whole_rows(D, rot) && whole_chunks(q, tok.B, tok.S) && aligned(q_out, 16) &&
                      (!a.k.ptr || (whole_chunks(k, tok.B, tok.S) && aligned(k_out, 16)));
-    if (vec)
-        rotate_typed<true>(q->dtype, grid, a, stream);
+    if (vec && streams((int64_t)a.rows * D, q->dtype))
+        rotate_typed<true, true>(q->dtype, grid, a, stream);
+    else if (vec)
+        rotate_typed<true, false>(q->dtype, grid, a, stream);
     else
-        rotate_typed<false>(q->dtype, grid, a, stream);
+        rotate_typed<false, false>(q->dtype, grid, a, stream);
     EP_HIP_CHECK(hipGetLastError());
     return EP_OK;
 }
@@ -500,17 +549,18 @@ int launch_kv_append(const ep_heads *q, const ep_heads *k, const ep_heads *v, co
                      const PagedTokens &tok, const PagedCache &c, void *q_out, hipStream_t stream)
 {
     AppendArgs a{rows_of(q), rows_of(k), rows_of(v), turn_of(rot, 0), tok, c, q_out, 0, lanes_of(c.D)};
-    a.rows = tok.B * tok.S * (a.q.heads + 2 * c.heads);
     unsigned grid;
-    const int rc = grid_of(a.rows, a.lanes, grid);
+    const int rc = grid_of(tok, a.q.heads + 2 * c.heads, a.lanes, a.rows, grid);
     if (rc != EP_OK || a.rows == 0)
         return rc;
     const bool vec = whole_rows(c.D, rot) && whole_chunks(k, tok.B, tok.S) && whole_chunks(v, tok.B, tok.S) &&
                      (!a.q.ptr || (whole_chunks(q, tok.B, tok.S) && aligned(q_out, 16)));
-    if (vec)
-        append_typed<true>(k->dtype, grid, a, stream);
+    if (vec && streams(tok.B * tok.S * a.q.heads * c.D, k->dtype))
+        append_typed<true, true>(k->dtype, grid, a, stream);
+    else if (vec)
+        append_typed<true, false>(k->dtype, grid, a, stream);
     else
-        append_typed<false>(k->dtype, grid, a, stream);
+        append_typed<false, false>(k->dtype, grid, a, stream);
     EP_HIP_CHECK(hipGetLastError());
     return EP_OK;
 }
@@ -518,19 +568,17 @@ int launch_kv_append(const ep_heads *q, const ep_heads *k, const ep_heads *v, co
 int launch_kv_read(const PagedTokens &tok, const PagedCache &c, void *k_out, void *v_out, int out_dtype,
                    hipStream_t stream)
 {
-    ReadArgs a{tok, c, k_out, v_out, tok.B * tok.S * 2 * c.heads, lanes_of(c.D)};
+    ReadArgs a{tok, c, k_out, v_out, 0, lanes_of(c.D)};
     unsigned grid;
-    const int rc = grid_of(a.rows, a.lanes, grid);
+    const int rc = grid_of(tok, 2 * c.heads, a.lanes, a.rows, grid);
     if (rc != EP_OK || a.rows == 0)
         return rc;
     if (!aligned(k_out, 16) || !aligned(v_out, 16))
         return set_error(EP_DECLINE_SHAPE, "cache read: outputs must be 16-byte aligned");
-    if (out_dtype == EP_F32)
-        read_kernel<float><<<grid, 256, 0, stream>>>(a);
-    else if (out_dtype == EP_F16)
-        read_kernel<f16_t><<<grid, 256, 0, stream>>>(a);
+    if (streams((int64_t)a.rows * c.D, out_dtype))
+        read_typed<true>(out_dtype, grid, a, stream);
     else
-        read_kernel<uint16_t><<<grid, 256, 0, stream>>>(a);
+        read_typed<false>(out_dtype, grid, a, stream);
     EP_HIP_CHECK(hipGetLastError());
     return EP_OK;
 }
