@@ -10,40 +10,12 @@
 //
 // Host code only (no HIP header): the current stream's handle comes from
 // torch, the entry points' addresses from the loaded library.
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <ATen/ATen.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <c10/core/GradMode.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
+#include "torch_call.h"
 
-#include <stdint.h>
+namespace epure_torch {
 
-#include "epure_hip.h"
-
-namespace {
-
-decltype(&ep_dequant_matmul_workspace) fn_ws;
-decltype(&ep_dequant_matmul) fn_matmul;
-decltype(&ep_dequant_matmul_bwd_workspace) fn_bwd_ws;
-decltype(&ep_dequant_matmul_bwd) fn_backward;
 decltype(&ep_last_error) fn_error;
-PyObject *fn_stream;  // torch._C._cuda_getCurrentRawStream
-
-// EP_F32 / EP_F16 / EP_BF16, or -1.
-int dtype_code(const at::Tensor &t)
-{
-    switch (t.scalar_type()) {
-    case at::kFloat:
-        return EP_F32;
-    case at::kHalf:
-        return EP_F16;
-    case at::kBFloat16:
-        return EP_BF16;
-    default:
-        return -1;
-    }
-}
+PyObject *fn_stream;
 
 // A call that a torch mode, a functorch transform or a tensor wrapper wants
 // to see: those take the path through torch's operators.
@@ -68,6 +40,50 @@ bool plain_tensor(PyObject *o)
     return t.defined() && t.layout() == at::kStrided && t.unsafeGetTensorImpl()->has_storage() &&
            !t.key_set().has_any(wrapped);
 }
+
+// The current stream of the tensor's device (nullptr and *ok false: a Python
+// error is set).  A host tensor is refused here: its device index, -1, names
+// the current device's stream to torch, and the kernels would read host memory.
+void *stream_of(const at::Tensor &t, bool *ok)
+{
+    TORCH_CHECK_VALUE(t.is_cuda(), "expected a GPU tensor, but got one on ", t.device());
+    PyObject *idx = PyLong_FromLong(t.get_device());
+    PyObject *r = idx ? PyObject_CallOneArg(fn_stream, idx) : nullptr;
+    Py_XDECREF(idx);
+    void *s = r ? PyLong_AsVoidPtr(r) : nullptr;
+    Py_XDECREF(r);
+    *ok = !PyErr_Occurred();
+    return s;
+}
+
+at::Tensor bytes_like(const at::Tensor &t, size_t n)
+{
+    return n ? at::empty({(int64_t)n}, t.options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
+}
+
+PyObject *failed(const char *what, int rc)
+{
+    return PyErr_Format(PyExc_RuntimeError, "%s failed (%d): %s", what, rc, fn_error());
+}
+
+bool args_are(Py_ssize_t n, Py_ssize_t want)
+{
+    if (n == want)
+        return true;
+    PyErr_Format(PyExc_TypeError, "%zd arguments wanted, %zd given", want, n);
+    return false;
+}
+
+}  // namespace epure_torch
+
+using namespace epure_torch;
+
+namespace {
+
+decltype(&ep_dequant_matmul_workspace) fn_ws;
+decltype(&ep_dequant_matmul) fn_matmul;
+decltype(&ep_dequant_matmul_bwd_workspace) fn_bwd_ws;
+decltype(&ep_dequant_matmul_bwd) fn_backward;
 
 struct Weight {
     const uint8_t *packed;
@@ -98,31 +114,6 @@ bool weight(const at::Tensor &packed, const at::Tensor &scale, const at::Tensor 
     return true;
 }
 
-// The current stream of the tensor's device (nullptr and *ok false: a Python
-// error is set).  A host tensor is refused here: its device index, -1, names
-// the current device's stream to torch, and the kernels would read host memory.
-void *stream_of(const at::Tensor &t, bool *ok)
-{
-    TORCH_CHECK_VALUE(t.is_cuda(), "expected a GPU tensor, but got one on ", t.device());
-    PyObject *idx = PyLong_FromLong(t.get_device());
-    PyObject *r = idx ? PyObject_CallOneArg(fn_stream, idx) : nullptr;
-    Py_XDECREF(idx);
-    void *s = r ? PyLong_AsVoidPtr(r) : nullptr;
-    Py_XDECREF(r);
-    *ok = !PyErr_Occurred();
-    return s;
-}
-
-at::Tensor bytes_like(const at::Tensor &t, size_t n)
-{
-    return n ? at::empty({(int64_t)n}, t.options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
-}
-
-PyObject *failed(const char *what, int rc)
-{
-    return PyErr_Format(PyExc_RuntimeError, "%s failed (%d): %s", what, rc, fn_error());
-}
-
 // y = x2 . W^T, `out` given or of x2's type.  A new reference to y, None
 // where the library declines, nullptr with an error set.
 PyObject *run_matmul(const at::Tensor &x2, const Weight &w, at::Tensor out, const at::Tensor &shown, bool accumulate)
@@ -146,14 +137,6 @@ PyObject *run_matmul(const at::Tensor &x2, const Weight &w, at::Tensor out, cons
     if (rc > 0)
         Py_RETURN_NONE;
     return THPVariable_Wrap(shown);
-}
-
-bool args_are(Py_ssize_t n, Py_ssize_t want)
-{
-    if (n == want)
-        return true;
-    PyErr_Format(PyExc_TypeError, "%zd arguments wanted, %zd given", want, n);
-    return false;
 }
 
 bool tensors(PyObject *const *args, int n)
@@ -329,4 +312,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "epure_torch", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_epure_torch(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_epure_torch(void)
+{
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddFunctions(m, paged_methods) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

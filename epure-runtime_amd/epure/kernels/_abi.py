@@ -149,7 +149,7 @@ TORCH_PATH = os.path.join(os.path.dirname(LIB_PATH), "epure_torch.so")
 
 
 def _load_call(handle):
-    """The extension that calls ``handle``'s matmul entry points on tensors."""
+    """The extension that calls ``handle``'s matmul and paged-cache entry points on tensors."""
     loader = importlib.machinery.ExtensionFileLoader("epure_torch", TORCH_PATH)
     ext = importlib.util.module_from_spec(
         importlib.util.spec_from_file_location("epure_torch", TORCH_PATH, loader=loader))
@@ -157,6 +157,8 @@ def _load_call(handle):
     ext.bind(addr("ep_dequant_matmul_workspace"), addr("ep_dequant_matmul"),
              addr("ep_dequant_matmul_bwd_workspace"), addr("ep_dequant_matmul_bwd"),
              addr("ep_last_error"), getattr(torch._C, "_cuda_getCurrentRawStream", None))
+    ext.bind_paged(addr("ep_rotate"), addr("ep_kv_append"), addr("ep_kv_read"),
+                   addr("ep_paged_attention_workspace"), addr("ep_paged_attention"))
     return ext
 
 

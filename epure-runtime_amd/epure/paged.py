@@ -40,6 +40,13 @@ def _no_grad(*tensors):
         raise RuntimeError("the paged cache has no backward: call under torch.no_grad()")
 
 
+def _native():
+    """The native call path, or None.  Its calls return NotImplemented for all
+    that is not an ordinary call on plain GPU tensors: those go on below, where
+    arguments are checked and refused."""
+    return _abi.call if cuda_kernel.available() else None
+
+
 def _run(what, rc):
     if not _abi.check(rc, what):
         raise ValueError(f"{what} declined: {_abi.last_error()}")
@@ -176,6 +183,11 @@ class Rotary:
     def rotate(self, q, k, positions):
         """q and k ([B, S, heads, D], one type) turned by their tokens'
         positions (broadcast to [B, S]).  Differentiable in both."""
+        call = _native()
+        if call is not None:
+            r = call.rotate(q, k, positions, self.cos, self.sin, self.layout == "interleaved")
+            if r is not NotImplemented:
+                return r
         self._check(q, k, positions)
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
             return _Rotate.apply(q, k, positions, self, False)
@@ -183,6 +195,11 @@ class Rotary:
 
     def __call__(self, x, positions):
         """One tensor [B, S, heads, D] turned."""
+        call = _native()
+        if call is not None:
+            r = call.rotate(x, None, positions, self.cos, self.sin, self.layout == "interleaved")
+            if r is not NotImplemented:
+                return r
         self._check(x, None, positions)
         if torch.is_grad_enabled() and x.requires_grad:
             return _Rotate.apply(x, None, positions, self, False)[0]
@@ -277,6 +294,13 @@ class PagedKVCache:
         With ``rotary``, k is turned on its way into the cache and q (if
         given, [B, S, q heads, D]) on its way out; returns q turned, or None
         without q.  A turned key is rounded once, to the cache's type."""
+        call = _native()
+        if call is not None:
+            cos, sin, inter = (None, None, False) if rotary is None else \
+                (rotary.cos, rotary.sin, rotary.layout == "interleaved")
+            r = call.append(k, v, positions, table, q, cos, sin, inter, self.k, self.v, self.k_scale, self.v_scale)
+            if r is not NotImplemented:
+                return r
         _no_grad(q, k, v)
         _require(self.k, k, v, positions, table, *(() if q is None else (q,)),
                  *(() if rotary is None else (rotary.cos,)))
@@ -304,6 +328,11 @@ class PagedKVCache:
 
     def read(self, positions, table, dtype=torch.bfloat16):
         """(k, v) [B, S, heads, D] in ``dtype``: the rows at positions [B, S]."""
+        call = _native()
+        if call is not None:
+            r = call.read(positions, table, dtype, self.k, self.v, self.k_scale, self.v_scale)
+            if r is not NotImplemented:
+                return r
         _require(self.k, positions, table)
         if _abi.dtype_code(dtype) is None:
             raise TypeError(f"the cache is read as float32, float16 or bfloat16, not {dtype}")
@@ -324,6 +353,11 @@ class PagedKVCache:
         their own position (append them first); [B, S, q heads, D] in q's
         type.  ``scale`` defaults to D ** -0.5, ``window`` to all.  A 16-bit
         cache must have q's type.  Meant for one new token, or a few."""
+        call = _native()
+        if call is not None:
+            r = call.attend(q, positions, table, scale, window, self.k, self.v, self.k_scale, self.v_scale)
+            if r is not NotImplemented:
+                return r
         _no_grad(q)
         _require(self.k, q, positions, table)
         q = _heads4("q", q)
