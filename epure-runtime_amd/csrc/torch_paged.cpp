@@ -118,14 +118,32 @@ bool needs_grad(std::initializer_list<const at::Tensor *> ts)
 at::Tensor like(const at::Tensor &t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }
 
 // ------------------------------------------------------------------ rotation
+// What a rotation's gradient needs of it.  The engine runs a node's backward
+// pass on the stream of its forward pass (from a thread that does not hold the
+// interpreter's lock), so that stream is kept rather than asked for.
 struct Turn {
     at::Tensor positions, cos, sin;
-    bool interleaved;
+    bool interleaved, inverse;
+    void *stream;
+
+    void save(torch::autograd::AutogradContext *ctx) const
+    {
+        ctx->save_for_backward({positions, cos, sin});
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["inverse"] = inverse;
+        ctx->saved_data["stream"] = (int64_t)stream;
+    }
+    // The way back of a saved turn.
+    static Turn back(torch::autograd::AutogradContext *ctx)
+    {
+        const auto s = ctx->get_saved_variables();
+        return Turn{s[0], s[1], s[2], ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool(),
+                    (void *)ctx->saved_data["stream"].toInt()};
+    }
 };
 
-// q and k (undefined: none) turned.  From any thread: the engine's run the
-// backward pass without the interpreter's lock.
-int turn(const at::Tensor &q, const at::Tensor &k, const Turn &t, bool inverse, at::Tensor &qo, at::Tensor &ko)
+// q and k (undefined: none) turned.
+int turn(const at::Tensor &q, const at::Tensor &k, const Turn &t, at::Tensor &qo, at::Tensor &ko)
 {
     ep_rotation r;
     ep_tokens tok;
@@ -136,22 +154,9 @@ int turn(const at::Tensor &q, const at::Tensor &k, const Turn &t, bool inverse, 
     qo = like(q);
     if (k.defined())
         ko = like(k);
-    const PyGILState_STATE gil = PyGILState_Ensure();
-    bool ok = false;
-    void *stream = nullptr;
-    try {
-        stream = stream_of(qs, &ok);
-    } catch (...) {
-        PyGILState_Release(gil);
-        throw;
-    }
-    if (!ok)
-        PyErr_Clear();
-    PyGILState_Release(gil);
-    TORCH_CHECK(ok, "rotation: no stream");
     const ep_heads qh = heads_of(qs), kh = k.defined() ? heads_of(ks) : ep_heads{};
-    return fn_rotate(&qh, k.defined() ? &kh : nullptr, &r, &tok, q.size(3), inverse, qo.data_ptr(),
-                     k.defined() ? ko.data_ptr() : nullptr, stream);
+    return fn_rotate(&qh, k.defined() ? &kh : nullptr, &r, &tok, q.size(3), t.inverse, qo.data_ptr(),
+                     k.defined() ? ko.data_ptr() : nullptr, t.stream);
 }
 
 void turned(int rc)
@@ -163,54 +168,43 @@ void turned(int rc)
 // One tensor, or two of a call, turned; the gradient of a turn is the turn
 // the other way, and differentiable likewise.
 struct RotateOne : torch::autograd::Function<RotateOne> {
-    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &positions,
-                              const at::Tensor &cos, const at::Tensor &sin, bool interleaved, bool inverse)
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const Turn &t)
     {
-        ctx->save_for_backward({positions, cos, sin});
-        ctx->saved_data["interleaved"] = interleaved;
-        ctx->saved_data["inverse"] = inverse;
+        t.save(ctx);
         at::Tensor y, none;
-        turned(turn(x, none, Turn{positions, cos, sin, interleaved}, inverse, y, none));
+        turned(turn(x, none, t, y, none));
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                    torch::autograd::variable_list g)
     {
-        const auto s = ctx->get_saved_variables();
-        return {RotateOne::apply(g[0], s[0], s[1], s[2], ctx->saved_data["interleaved"].toBool(),
-                                 !ctx->saved_data["inverse"].toBool()),
-                at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        return {RotateOne::apply(g[0], Turn::back(ctx)), at::Tensor()};
     }
 };
 
 struct RotateTwo : torch::autograd::Function<RotateTwo> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &q,
-                                                  const at::Tensor &k, const at::Tensor &positions,
-                                                  const at::Tensor &cos, const at::Tensor &sin, bool interleaved,
-                                                  bool inverse)
+                                                  const at::Tensor &k, const Turn &t)
     {
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({positions, cos, sin});
-        ctx->saved_data["interleaved"] = interleaved;
-        ctx->saved_data["inverse"] = inverse;
+        t.save(ctx);
         at::Tensor qo, ko;
-        turned(turn(q, k, Turn{positions, cos, sin, interleaved}, inverse, qo, ko));
+        turned(turn(q, k, t, qo, ko));
         return {qo, ko};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
                                                    torch::autograd::variable_list g)
     {
-        const auto s = ctx->get_saved_variables();
-        const bool interleaved = ctx->saved_data["interleaved"].toBool(), back = !ctx->saved_data["inverse"].toBool();
-        torch::autograd::variable_list r(7);
+        const Turn t = Turn::back(ctx);
+        torch::autograd::variable_list r(3);
         if (g[0].defined() && g[1].defined()) {
-            const auto two = RotateTwo::apply(g[0], g[1], s[0], s[1], s[2], interleaved, back);
+            const auto two = RotateTwo::apply(g[0], g[1], t);
             r[0] = two[0];
             r[1] = two[1];
         } else
             for (int i = 0; i < 2; ++i)
                 if (g[i].defined())
-                    r[i] = RotateOne::apply(g[i], s[0], s[1], s[2], interleaved, back);
+                    r[i] = RotateOne::apply(g[i], t);
         return r;
     }
 };
@@ -240,33 +234,36 @@ PyObject *rotate(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     if (two && (!k || !heads_ok(*k) || k->scalar_type() != q->scalar_type() || k->size(0) != q->size(0) ||
                 k->size(1) != q->size(1) || k->size(3) != q->size(3)))
         Py_RETURN_NOTIMPLEMENTED;
+    bool ok;
+    void *stream = stream_of(*q, &ok);
+    if (!ok)
+        return nullptr;
+    const Turn t{*pos, *cos, *sin, (bool)interleaved, false, stream};
     at::Tensor qo, ko;
-    if (needs_grad({q, k})) {
-        if (two) {
-            const auto y = RotateTwo::apply(*q, *k, *pos, *cos, *sin, (bool)interleaved, false);
-            qo = y[0];
-            ko = y[1];
-        } else
-            qo = RotateOne::apply(*q, *pos, *cos, *sin, (bool)interleaved, false);
-    } else {
-        const int rc = turn(*q, two ? *k : at::Tensor(), Turn{*pos, *cos, *sin, (bool)interleaved}, false, qo, ko);
+    if (!needs_grad({q, k})) {
+        const int rc = turn(*q, two ? *k : at::Tensor(), t, qo, ko);
         if (rc > 0)
             Py_RETURN_NOTIMPLEMENTED;
         if (rc < 0)
             return failed("ep_rotate", rc);
-    }
+    } else if (two) {
+        const auto y = RotateTwo::apply(*q, *k, t);
+        qo = y[0];
+        ko = y[1];
+    } else
+        qo = RotateOne::apply(*q, t);
     PyObject *a = THPVariable_Wrap(qo);
     if (!two || !a)
         return a;
-    PyObject *b = THPVariable_Wrap(ko), *t = b ? PyTuple_New(2) : nullptr;
-    if (!t) {
+    PyObject *b = THPVariable_Wrap(ko), *pair = b ? PyTuple_New(2) : nullptr;
+    if (!pair) {
         Py_DECREF(a);
         Py_XDECREF(b);
         return nullptr;
     }
-    PyTuple_SET_ITEM(t, 0, a);
-    PyTuple_SET_ITEM(t, 1, b);
-    return t;
+    PyTuple_SET_ITEM(pair, 0, a);
+    PyTuple_SET_ITEM(pair, 1, b);
+    return pair;
     END_HANDLE_TH_ERRORS
 }
 
