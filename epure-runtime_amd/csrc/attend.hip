@@ -3,6 +3,8 @@
 // The kernel and its layout: attend_kernel.h.
 #include <math.h>
 
+#include <algorithm>
+
 #include "attend_kernel.h"
 
 namespace ep {
@@ -24,7 +26,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int RM)
     const int p = attend_position(a, b, s);
     if (d.y <= 1)       // one worker wrote the output
         return;
-    const uint32_t quads = D / 4, groups = 256 / quads, grp = tid / quads, c = 4 * (tid - grp * quads);
+    const uint32_t quads = D / 4, groups = blockDim.x / quads, grp = tid / quads, c = 4 * (tid - grp * quads);
     float m = -INFINITY, l = 0.0f;
     f32x4_t y = {0, 0, 0, 0};
     auto add = [&](float m2, float l2, f32x4_t y2) {
@@ -84,7 +86,7 @@ constexpr size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 // Segments of few tiles go to a workgroup each; else all tiles are shared
 // evenly among `workers` and the pieces joined (where 32 bits count all
 // tiles that the table could hold).
-Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c)
+Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t window)
 {
     Plan p{};
     const int64_t rows = tok.S * (q->heads / c.heads);
@@ -92,7 +94,8 @@ Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c)
     const int rm = 16 * p.mt;
     p.segments = tok.B * ((rows + rm - 1) / rm) * c.heads;
     const int64_t tiles = (tok.width << c.page_shift) / kAttTile;
-    if (tiles > 2 * kAttWaves && p.segments < 0x40000000 && tiles + kAttPiece < 0xffff0000u / p.segments) {
+    const int64_t most = window > 0 ? std::min(tiles, (window + tok.S) / kAttTile + 2) : tiles;
+    if (most > (p.segments >= 256 ? 32 : 16) && p.segments < 0x40000000 && tiles + kAttPiece < 0xffff0000u / p.segments) {
         p.workers = 256 * attend_occupancy(c.D <= 64 ? 4 : c.D <= 128 ? 8 : 16, p.mt);
         const size_t slots = (size_t)2 * p.workers * (rows < rm ? rows : rm);
         p.desc = up16(p.segments * sizeof(int2));
@@ -108,14 +111,14 @@ size_t attend_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCa
 {
     if (tok.B == 0 || tok.S == 0)
         return 0;
-    const Plan p = plan(q, tok, c);
+    const Plan p = plan(q, tok, c, 0);
     return p.desc + p.ml + p.o;
 }
 
 int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, float scale, int64_t window,
                   void *out, void *ws, size_t ws_bytes, hipStream_t stream)
 {
-    const Plan p = plan(q, tok, c);
+    const Plan p = plan(q, tok, c, window);
     const int64_t cap = tok.width << c.page_shift, rows = tok.S * (q->heads / c.heads), rm = 16 * p.mt;
     const int64_t out_rows = tok.B * tok.S * q->heads;
     if (cap > 0x3fffffff || rows > 0x3fffffff || p.segments > 0x7fffffff || out_rows > 0x7fffffff)
@@ -156,9 +159,9 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
     EP_HIP_CHECK(hipGetLastError());
     if (p.workers) {
         if (q->dtype == EP_BF16)
-            join_kernel<OpBf16><<<(unsigned)out_rows, 256, 0, stream>>>(a, (int)rm);
+            join_kernel<OpBf16><<<(unsigned)out_rows, p.segments * 8 >= p.workers ? 128 : 256, 0, stream>>>(a, (int)rm);
         else
-            join_kernel<OpF16><<<(unsigned)out_rows, 256, 0, stream>>>(a, (int)rm);
+            join_kernel<OpF16><<<(unsigned)out_rows, p.segments * 8 >= p.workers ? 128 : 256, 0, stream>>>(a, (int)rm);
         EP_HIP_CHECK(hipGetLastError());
     }
     return EP_OK;

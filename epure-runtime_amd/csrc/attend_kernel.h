@@ -207,7 +207,10 @@ EP_DEV __amdgpu_buffer_rsrc_t tile_rsrc(const void *base, int64_t byte, bool ok,
 }
 
 // Workgroups of a kernel that a compute unit holds (waves of a SIMD).
-constexpr int attend_occupancy(int CW, int MT) { return CW == 4 ? (MT == 1 ? 3 : 2) : CW == 8 ? 2 : 1; }
+#ifndef OCC2
+#define OCC2 2
+#endif
+constexpr int attend_occupancy(int CW, int MT) { return CW == 4 ? (MT == 1 ? 3 : 2) : CW == 8 ? (MT == 1 ? 2 : OCC2) : 1; }
 
 // QOP: type of the queries; CODE: EP_I8, EP_E4M3, or QOP's type.  KS: steps of
 // 32 values of a head, CW: output columns a lane (16 CW >= D), MT: 16-row
@@ -222,6 +225,10 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
     __shared__ float s_o[kAttWaves][16][DP + 4];
     __shared__ float s_m[kAttWaves][RM], s_l[kAttWaves][RM];
     __shared__ int s_p[RM];
+    // Queries of more than one row tile stay in LDS: their registers are what
+    // a second wave on the SIMD needs.
+    constexpr bool kQueriesInLds = MT > 1;
+    __shared__ u32x4_t s_q[kQueriesInLds ? MT * KS * 64 : 1];
 
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -265,17 +272,27 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
             pos[mt] = row < a.rows ? attend_position(a, b, (uint32_t)row / (uint32_t)a.G) : -1;
         }
         __builtin_amdgcn_sched_barrier(0);       // loads return in order: the positions' wait must not cover the queries
-        u32x4_t q[MT][KS];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        // (mt, k): values of step k of row n, zero past D
+        auto query = [&](int mt, int k) {
             const int row = min(r0 + 16 * mt + ln, a.rows - 1);
             const int s = (uint32_t)row / (uint32_t)a.G, gq = row - s * a.G;
-            const char *src = (const char *)a.q + 2 * (b * a.q_sb + s * a.q_ss + (int64_t)(h * a.G + gq) * a.q_sh);
+            const int d = k8 ? 64 * (k / 2) + 16 * lg + 8 * (k & 1) : 32 * k + 8 * lg;
+            const int64_t at = b * a.q_sb + s * a.q_ss + (int64_t)(h * a.G + gq) * a.q_sh + (d < D ? d : 0);
+            return *(const u32x4_t *)((const char *)a.q + 2 * at);
+        };
+        auto in_head = [&](int k, u32x4_t w) {
+            const int d = k8 ? 64 * (k / 2) + 16 * lg + 8 * (k & 1) : 32 * k + 8 * lg;
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const int d = k8 ? 64 * (k / 2) + 16 * lg + 8 * (k & 1) : 32 * k + 8 * lg;
-                q[mt][k] = *(const u32x4_t *)(src + 2 * (d < D ? d : 0));
-            }
+            for (int i = 0; i < 4; ++i)
+                w[i] = d < D ? w[i] : 0u;
+            return w;
+        };
+        constexpr int QN = kQueriesInLds ? (MT * KS + kAttWaves - 1) / kAttWaves : MT * KS;
+        u32x4_t q[QN];
+#pragma unroll
+        for (int i = 0; i < QN; ++i) {
+            const int f = kQueriesInLds ? min(kAttWaves * i + wave, MT * KS - 1) : i;
+            q[i] = query(f / KS, f % KS);
         }
         __builtin_amdgcn_sched_barrier(0);
         int lo = -a.cap, hi = -1, in_lo = 0, in_hi = -a.cap;     // over the rows: seen by any (lo negated), by all
@@ -384,15 +401,17 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
         load_v();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const int d = k8 ? 64 * (k / 2) + 16 * lg + 8 * (k & 1) : 32 * k + 8 * lg;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    q[mt][k][i] = d < D ? q[mt][k][i] : 0u;
-            }
+        for (int i = 0; i < QN; ++i) {
+            const int f = kQueriesInLds ? min(kAttWaves * i + wave, MT * KS - 1) : i;
+            q[i] = in_head(f % KS, q[i]);
+            if constexpr (kQueriesInLds)
+                s_q[64 * f + lx] = q[i];
+        }
+        if constexpr (kQueriesInLds)
+            lds_barrier();
         for (; j < end; j += kAttWaves) {
+            if constexpr (kQueriesInLds)
+                asm volatile("" ::: "memory");      // the queries are read again for each tile
             const int j0 = j * kAttTile;
             const bool bad0 = !good[0], bad1 = !good[1];
             f32x4_t sc[MT][2];
@@ -412,7 +431,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
                         f = kr[t][k];
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
-                        sc[mt][t] = QOP::mfma(f, q[mt][k], sc[mt][t]);
+                        sc[mt][t] = QOP::mfma(f, kQueriesInLds ? s_q[64 * (mt * KS + k) + lane] : q[mt * KS + k], sc[mt][t]);
                 }
             float x[MT][8];
 #pragma unroll
@@ -569,6 +588,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
             for (int w = 1; w < kAttWaves; ++w)
                 top = fmaxf(top, s_m[w][16 * mt + en]);
             const float f = __builtin_amdgcn_exp2f(m[mt] - (top == -INFINITY ? 0.0f : top));
+            if (16 * mt + en < rows)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -576,9 +596,9 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
                     *(f32x4_t *)&s_o[wave][en][CW * (4 * eg + i) + t] =
                         (f32x4_t){o[mt][t][i] * f, o[mt][t + 1][i] * f, o[mt][t + 2][i] * f, o[mt][t + 3][i] * f};
             __syncthreads();
-            for (int e = tid; e < 16 * DP / 4; e += 64 * kAttWaves) {
+            for (int e = tid; e < min(16, rows - 16 * mt) * (DP / 4); e += 64 * kAttWaves) {
                 const int row = e / (DP / 4), d = 4 * (e % (DP / 4)), r = 16 * mt + row;
-                if (r >= rows || d >= D)
+                if (d >= D)
                     continue;
                 float mx = s_m[0][r], sum = 0.0f;
 #pragma unroll
