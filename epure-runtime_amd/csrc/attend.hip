@@ -81,6 +81,18 @@ struct Plan {
     size_t desc, ml, o;     // bytes of the workspace's parts
 };
 
+// A piece takes some 6 us beyond its tiles, and a tile as long as a worker's
+// part of the bandwidth needs for its bytes: 6 tiles' time for 128 16-bit
+// values and 512 workers.  Short sequences of a ragged batch cost that much
+// more than their lengths say (a worker that got a dozen of them took 97 us
+// where the rest took 46).
+constexpr int kMostPiece = 786432 / (16 * 256);
+int piece_tiles(const PagedCache &c, int workers)
+{
+    const int row = c.D * (c.dtype == EP_F16 || c.dtype == EP_BF16 ? 2 : 1);
+    return 786432 / (row * std::max(workers, 256));
+}
+
 constexpr size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 // Segments of few tiles go to a workgroup each; else all tiles are shared
@@ -95,7 +107,7 @@ Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_
     p.segments = tok.B * ((rows + rm - 1) / rm) * c.heads;
     const int64_t tiles = (tok.width << c.page_shift) / kAttTile;
     const int64_t most = window > 0 ? std::min(tiles, (window + tok.S) / kAttTile + 2) : tiles;
-    if (most > (p.segments >= 256 ? 32 : 16) && p.segments < 0x40000000 && tiles + kAttPiece < 0xffff0000u / p.segments) {
+    if (most > (p.segments >= 256 ? 32 : 16) && p.segments < 0x40000000 && tiles + kMostPiece < 0xffff0000u / p.segments) {
         p.workers = 256 * attend_occupancy(c.D <= 64 ? 4 : c.D <= 128 ? 8 : 16, p.mt);
         const size_t slots = (size_t)2 * p.workers * (rows < rm ? rows : rm);
         p.desc = up16(p.segments * sizeof(int2));
@@ -143,6 +155,7 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
     a.blocks = (int)((rows + rm - 1) / rm);
     a.units = (uint32_t)(tok.B * a.blocks);
     a.workers = p.workers;
+    a.piece = piece_tiles(c, p.workers);
     a.slot_rows = (int)(rows < rm ? rows : rm);
     a.desc = (int2 *)ws;
     a.part_ml = (float2 *)((char *)ws + p.desc);

@@ -40,7 +40,6 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kAttTile = 32;             // positions a wave takes at a time
 constexpr int kAttWaves = 4;             // waves of a workgroup: they take tiles in turn
-constexpr int kAttPiece = 6;             // tiles' time that beginning and ending a piece takes
 constexpr int kAttOut = 0x40000000;      // an offset past every descriptor below: reads zeros
 
 struct AttendArgs {
@@ -56,6 +55,7 @@ struct AttendArgs {
     int blocks;              // units of a sequence
     uint32_t units;
     int workers;             // workgroups that share all tiles evenly; 0: one workgroup a segment
+    int piece;               // tiles' time that beginning and ending a piece takes
     int slot_rows;           // rows kept of a piece: min(rows, 16 MT)
     int2 *desc;              // [segments]: first slot, pieces
     float2 *part_ml;         // [2 workers][slot_rows]: maximum, sum
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
     bool counting = a.workers > 0, load = counting;
     for (;;) {
         if (load) {
-            cost = u0 + lane < units ? unit_tiles<RM>(a, u0 + lane, first) + kAttPiece : 0u;
+            cost = u0 + lane < units ? unit_tiles<RM>(a, u0 + lane, first) + a.piece : 0u;
             upto = cost;
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) {
@@ -661,7 +661,10 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
             if (load)
                 continue;
             counting = false;
-            per = max((total + a.workers - 1) / (uint32_t)a.workers, (uint32_t)kAttWaves);
+            // At least a tile a wave, and up to two while that leaves a share to
+            // every compute unit: one workgroup on each before a second.
+            per = max((total + a.workers - 1) / (uint32_t)a.workers,
+                      min(max((total + 255) / 256, (uint32_t)kAttWaves), 2u * kAttWaves));
             f = begin = min(blockIdx.x * per, total);
             stop = min(begin + per, total);
             u0 = 0;
@@ -685,7 +688,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
             const uint32_t n1 = at_lane(cost, i), seg0 = before + (at_lane(upto, i) - n1) * H;
             u = u0 + i;
             h = (int)((f - seg0) / n1);
-            const uint32_t next = seg0 + (h + 1) * n1, head0 = next - n1 + kAttPiece;     // the segment's tiles: [head0, next)
+            const uint32_t next = seg0 + (h + 1) * n1, head0 = next - n1 + a.piece;     // the segment's tiles: [head0, next)
             const uint32_t f0 = max(f, head0), f1 = min(next, stop);
             f = f1;
             if (f0 >= f1)
@@ -695,11 +698,11 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
             t1 = base + (int)f1;
             if (f0 == head0 && threadIdx.x == 0) {
                 const uint32_t w1 = min((next - 1) / per, (uint32_t)a.workers - 1);
-                a.desc[u * H + h] = make_int2(2 * (int)blockIdx.x + (head0 - kAttPiece >= begin), (int)(w1 - blockIdx.x + 1));
+                a.desc[u * H + h] = make_int2(2 * (int)blockIdx.x + (head0 - a.piece >= begin), (int)(w1 - blockIdx.x + 1));
             }
             // A piece that begins before its worker's share does is kept in the
             // worker's first slot, else in its second.
-            slot = f0 == head0 && f1 == next ? -1 : 2 * (int)blockIdx.x + (head0 - kAttPiece >= begin);
+            slot = f0 == head0 && f1 == next ? -1 : 2 * (int)blockIdx.x + (head0 - a.piece >= begin);
         } else
             f = stop;
         piece(u, h, t0, t1, slot);
