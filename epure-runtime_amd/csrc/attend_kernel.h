@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
     constexpr int ES = k8 ? 1 : 2, KL = k8 ? KS / 2 : KS, RM = 16 * MT, DP = 16 * CW, VW = CW * ES / 4;
     static_assert(!k8 || KS % 2 == 0, "8-bit keys are read in chunks of two steps");
     using VOP = typename std::conditional<k8, OpBf16, QOP>::type;
-    __shared__ float s_o[kAttWaves][16][DP + 4];
+    __shared__ float s_o[kAttWaves][RM][DP + 4];
     __shared__ float s_m[kAttWaves][RM], s_l[kAttWaves][RM];
     __shared__ int s_p[RM];
     // Queries of more than one row tile stay in LDS: their registers are what
@@ -569,8 +569,11 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
             load_v();
         }
 
-        // ---- the waves' parts of the piece
+        // ---- the waves' parts of the piece: each leaves its rows as they are,
+        // and what is read is weighed.  The barriers order LDS only, so that no
+        // store to memory is waited for.
         const int ex = opaque(lane), en = ex & 15, eg = ex >> 4, tid = opaque(threadIdx.x);
+        const int rows = min(RM, a.rows - r0);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             l[mt] = xor32_sum(xor16_sum(l[mt]));
@@ -578,58 +581,52 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
                 s_m[wave][16 * mt + en] = m[mt];
                 s_l[wave][16 * mt + en] = l[mt];
             }
-        }
-        __syncthreads();
-        const int rows = min(RM, a.rows - r0);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            float top = s_m[0][16 * mt + en];
-#pragma unroll
-            for (int w = 1; w < kAttWaves; ++w)
-                top = fmaxf(top, s_m[w][16 * mt + en]);
-            const float f = __builtin_amdgcn_exp2f(m[mt] - (top == -INFINITY ? 0.0f : top));
             if (16 * mt + en < rows)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int t = 0; t < CW; t += 4)
-                    *(f32x4_t *)&s_o[wave][en][CW * (4 * eg + i) + t] =
-                        (f32x4_t){o[mt][t][i] * f, o[mt][t + 1][i] * f, o[mt][t + 2][i] * f, o[mt][t + 3][i] * f};
-            __syncthreads();
-            for (int e = tid; e < min(16, rows - 16 * mt) * (DP / 4); e += 64 * kAttWaves) {
-                const int row = e / (DP / 4), d = 4 * (e % (DP / 4)), r = 16 * mt + row;
-                if (d >= D)
-                    continue;
-                float mx = s_m[0][r], sum = 0.0f;
+                    for (int t = 0; t < CW; t += 4)
+                        *(f32x4_t *)&s_o[wave][16 * mt + en][CW * (4 * eg + i) + t] =
+                            (f32x4_t){o[mt][t][i], o[mt][t + 1][i], o[mt][t + 2][i], o[mt][t + 3][i]};
+        }
+        lds_barrier();
+        for (int e = tid; e < rows * (DP / 4); e += 64 * kAttWaves) {
+            const int r = e / (DP / 4), d = 4 * (e % (DP / 4));
+            if (d >= D)
+                continue;
+            float mx = s_m[0][r], sum = 0.0f;
 #pragma unroll
-                for (int w = 1; w < kAttWaves; ++w)
-                    mx = fmaxf(mx, s_m[w][r]);
-                const float mu = mx == -INFINITY ? 0.0f : mx;
-                f32x4_t y = {0, 0, 0, 0};
+            for (int w = 1; w < kAttWaves; ++w)
+                mx = fmaxf(mx, s_m[w][r]);
+            const float mu = mx == -INFINITY ? 0.0f : mx;
+            f32x4_t y = {0, 0, 0, 0};
 #pragma unroll
-                for (int w = 0; w < kAttWaves; ++w) {
-                    sum += s_l[w][r] * __builtin_amdgcn_exp2f(s_m[w][r] - mu);
-                    y += *(const f32x4_t *)&s_o[w][row][d];
-                }
-                if (slot >= 0) {
-                    const int64_t at = (int64_t)slot * a.slot_rows + r;
-                    *(f32x4_t *)(a.part_o + at * D + d) = y;
-                    if (d == 0)
-                        a.part_ml[at] = make_float2(mx, sum);
-                    continue;
-                }
-                const int p = s_p[r], s = (uint32_t)(r0 + r) / (uint32_t)a.G, gq = r0 + r - s * a.G;
-                const float inv = 1.0f / sum;      // no weight at all (every score -inf) gives NaN
+            for (int w = 0; w < kAttWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(s_m[w][r] - mu);
+                const f32x4_t v = *(const f32x4_t *)&s_o[w][r][d];
+                sum = fmaf(s_l[w][r], f, sum);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    y[i] = p < 0 ? 0.0f : p >= a.cap || sum == 0.0f ? nan : y[i] * inv;
-                uint2 w;
-                w.x = QOP::pack(y[0], y[1]);
-                w.y = QOP::pack(y[2], y[3]);
-                *(uint2 *)((char *)a.out + 2 * (((b * a.tok.S + s) * H * a.G + h * a.G + gq) * D + d)) = w;
+                    y[i] = fmaf(v[i], f, y[i]);
             }
-            __syncthreads();
+            if (slot >= 0) {
+                const int64_t at = (int64_t)slot * a.slot_rows + r;
+                *(f32x4_t *)(a.part_o + at * D + d) = y;
+                if (d == 0)
+                    a.part_ml[at] = make_float2(mx, sum);
+                continue;
+            }
+            const int p = s_p[r], s = (uint32_t)(r0 + r) / (uint32_t)a.G, gq = r0 + r - s * a.G;
+            const float inv = 1.0f / sum;      // no weight at all (every score -inf) gives NaN
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                y[i] = p < 0 ? 0.0f : p >= a.cap || sum == 0.0f ? nan : y[i] * inv;
+            uint2 w;
+            w.x = QOP::pack(y[0], y[1]);
+            w.y = QOP::pack(y[2], y[3]);
+            *(uint2 *)((char *)a.out + 2 * (((b * a.tok.S + s) * H * a.G + h * a.G + gq) * D + d)) = w;
         }
+        lds_barrier();
     };
 
     // ---- one segment a workgroup (workers == 0), or an even share of all tiles
