@@ -106,8 +106,10 @@ Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_
     const int rm = 16 * p.mt;
     p.segments = tok.B * ((rows + rm - 1) / rm) * c.heads;
     const int64_t tiles = (tok.width << c.page_shift) / kAttTile;
-    const int64_t most = window > 0 ? std::min(tiles, (window + tok.S) / kAttTile + 2) : tiles;
-    if (most > (p.segments >= 256 ? 32 : 16) && p.segments < 0x40000000 && tiles + kMostPiece < 0xffff0000u / p.segments) {
+    // a window's tiles, if the call's tokens follow one another
+    const int64_t most = window > 0 && window <= tiles * kAttTile
+                             ? std::min(tiles, (window + tok.S) / kAttTile + 2) : tiles;
+    if (most > (p.segments >= 256 ? 32 : 16) && p.segments < 0x40000000 && tiles + kMostPiece < 0x7fff0000 / p.segments) {
         p.workers = 256 * attend_occupancy(c.D <= 64 ? 4 : c.D <= 128 ? 8 : 16, p.mt);
         const size_t slots = (size_t)2 * p.workers * (rows < rm ? rows : rm);
         p.desc = up16(p.segments * sizeof(int2));
@@ -156,6 +158,13 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
     a.units = (uint32_t)(tok.B * a.blocks);
     a.workers = p.workers;
     a.piece = piece_tiles(c, p.workers);
+    // Values pass the caches on their way (4 x 131072 positions in 313 us, 348
+    // with plain loads).  Keys do too (308) unless they are read again soon: by
+    // a sequence's next unit in this call (64 rows a key head: 85 us, 79 with
+    // plain key loads), or by the next call where the 256 MB behind the L2
+    // caches hold a few such pools (16 x 2-4 thousand int8 positions: 28.7, 26.9).
+    a.keys_once = a.blocks == 1 && c.n_pages * c.heads * c.page * c.D * (c.dtype == EP_F16 || c.dtype == EP_BF16 ? 2 : 1)
+                                       > (int64_t)80 << 20;
     a.slot_rows = (int)(rows < rm ? rows : rm);
     a.desc = (int2 *)ws;
     a.part_ml = (float2 *)((char *)ws + p.desc);

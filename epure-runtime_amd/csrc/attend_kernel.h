@@ -40,6 +40,7 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kAttTile = 32;             // positions a wave takes at a time
 constexpr int kAttWaves = 4;             // waves of a workgroup: they take tiles in turn
+constexpr int kAttOnce = 2;              // a load's non-temporal bit: rows that are read once
 constexpr int kAttOut = 0x40000000;      // an offset past every descriptor below: reads zeros
 
 struct AttendArgs {
@@ -56,6 +57,7 @@ struct AttendArgs {
     uint32_t units;
     int workers;             // workgroups that share all tiles evenly; 0: one workgroup a segment
     int piece;               // tiles' time that beginning and ending a piece takes
+    int keys_once;           // keys are loaded past the caches, as values are
     int slot_rows;           // rows kept of a piece: min(rows, 16 MT)
     int2 *desc;              // [segments]: first slot, pieces
     float2 *part_ml;         // [2 workers][slot_rows]: maximum, sum
@@ -347,10 +349,16 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const auto r = tile_rsrc(a.c.k, at[t] * D * ES, good[t], 16 * D * ES);
+                if (a.keys_once)
 #pragma unroll
-                for (int k = 0; k < KL; ++k)
-                    kr[t][k] = __builtin_amdgcn_raw_buffer_load_b128(
-                        r, k >= KL - 2 ? koff[k - (KL - 2)] : kbase + 64 * k, 0, 0);
+                    for (int k = 0; k < KL; ++k)
+                        kr[t][k] = __builtin_amdgcn_raw_buffer_load_b128(
+                            r, k >= KL - 2 ? koff[k - (KL - 2)] : kbase + 64 * k, 0, kAttOnce);
+                else
+#pragma unroll
+                    for (int k = 0; k < KL; ++k)
+                        kr[t][k] = __builtin_amdgcn_raw_buffer_load_b128(
+                            r, k >= KL - 2 ? koff[k - (KL - 2)] : kbase + 64 * k, 0, 0);
             }
             if constexpr (k8)
                 load_scales(a.c.k_scale, ks);
@@ -363,15 +371,15 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
                 for (int i = 0; i < 4; ++i) {
                     uint32_t *dst = vr[4 * t + i];
                     if constexpr (VW == 1)
-                        dst[0] = __builtin_amdgcn_raw_buffer_load_b32(r, voff[i], 0, 0);
+                        dst[0] = __builtin_amdgcn_raw_buffer_load_b32(r, voff[i], 0, kAttOnce);
                     else if constexpr (VW == 2) {
-                        const auto w = __builtin_amdgcn_raw_buffer_load_b64(r, voff[i], 0, 0);
+                        const auto w = __builtin_amdgcn_raw_buffer_load_b64(r, voff[i], 0, kAttOnce);
                         dst[0] = w[0];
                         dst[1] = w[1];
                     } else
 #pragma unroll
                         for (int c = 0; c < VW; c += 4) {
-                            const auto w = __builtin_amdgcn_raw_buffer_load_b128(r, voff[i] + 4 * c, 0, 0);
+                            const auto w = __builtin_amdgcn_raw_buffer_load_b128(r, voff[i] + 4 * c, 0, kAttOnce);
 #pragma unroll
                             for (int x = 0; x < 4; ++x)
                                 dst[c + x] = w[x];
