@@ -81,6 +81,9 @@ int check_attend(const ep_heads *q, const ep_tokens *t, const ep_kv_cache *cache
         rc = check_cache(cache, c);
     if (rc != EP_OK)
         return rc;
+    if (t->width > 0x3fffffff >> c.page_shift)
+        return set_error(EP_DECLINE_SHAPE, "a table of %lld pages of %d rows: up to 2^30 positions are served",
+                         (long long)t->width, c.page);
     if (q->dtype == EP_F32)
         return set_error(EP_DECLINE_DTYPE, "attention: q must be f16 or bf16");
     if ((c.dtype == EP_F16 || c.dtype == EP_BF16) && c.dtype != q->dtype)

@@ -110,15 +110,21 @@ int ep_kv_read(const ep_tokens *tokens, const ep_kv_cache *cache, void *k_out, v
                void *stream);
 
 /*
- * out [B, S, q heads, D] (dense, q's type): each token's attention over the
- * cache positions max(0, p - window + 1) .. p of its sequence (window <= 0:
- * from 0), p its own position, softmax of scale * q . k; q heads a multiple
- * of the cache's, head h reads cache head h / (q heads / heads).  q: EP_F16
- * or EP_BF16, 16-byte aligned with strides of whole 8 values; a 16-bit cache
- * has q's type.  Scores, softmax and sums are f32.  NaN and infinities of
- * positions that a token does not attend to do not reach it.
+ * out [B, S, q heads, D] (dense, q's type, 16-byte aligned): each token's
+ * attention over the cache positions max(0, p - window + 1) .. p of its
+ * sequence (window <= 0: from 0), p its own position, softmax of scale *
+ * q . k; q heads a multiple of the cache's, head h reads cache head h / (q
+ * heads / heads).  Tokens of a call may stand anywhere, in any order.  q:
+ * EP_F16 or EP_BF16, 16-byte aligned with strides of whole 8 values; a 16-bit
+ * cache has q's type; a table of at most 2^30 positions.  Scores, softmax and
+ * sums are f32, the weights enter their product with 16 bits or more.  NaN
+ * and infinities of positions that a token does not attend to do not reach
+ * it; an infinite value that it attends to gives an infinity or NaN.  Any
+ * number of new tokens is served; more than 32 query rows (tokens times heads
+ * a cache head) read the cache once per 32.
  * Workspace: ep_paged_attention_workspace() bytes (0 if the shape is
- * declined), read and written by this call alone.
+ * declined, or none is needed), 16-byte aligned, read and written by this call
+ * alone.
  */
 size_t ep_paged_attention_workspace(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache);
 int ep_paged_attention(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache, float scale,
