@@ -36,7 +36,7 @@
 // 441 MB, 81 us, four waves a workgroup and two workgroups a compute unit, 16
 // KiB (bf16) in flight a wave.  Short calls are a chain of loads: arguments,
 // positions with pages and queries, keys and values, 7 us in all for 129
-// positions; the code is kept small (13 KB) because it is fetched cold.
+// positions; the code is kept small (10 KB) because it is fetched cold.
 #pragma once
 
 #include "ep_common.h"
@@ -129,7 +129,7 @@ EP_DEV uint32_t unit_tiles(const AttendArgs &a, uint32_t u, uint32_t &first)
 struct OpBf16 {
     static constexpr int kDtype = EP_BF16;
     static constexpr float kShift = 0.0f;
-    static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u;
+    static constexpr uint32_t kOne = 0x3f80u;
     static EP_DEV f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c)
     {
         bf16x8_t x, y;
@@ -152,7 +152,7 @@ struct OpBf16 {
 struct OpF16 {
     static constexpr int kDtype = EP_F16;
     static constexpr float kShift = 15.0f;
-    static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u;
+    static constexpr uint32_t kOne = 0x3c00u;
     static EP_DEV f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c)
     {
         f16x8_t x, y;
@@ -183,6 +183,20 @@ EP_DEV void codes2(uint32_t w, float &x, float &y)
         const f32x2_t v = __builtin_amdgcn_cvt_pk_f32_fp8(w, HI);
         x = v[0];
         y = v[1];
+    }
+}
+
+// All bits set in each value of w that is infinite or NaN.
+template <int CODE>
+EP_DEV uint32_t not_finite(uint32_t w)
+{
+    if constexpr (CODE == EP_E4M3) {     // NaN: 0x7f; one more sets the sign bit
+        const uint32_t h = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        return (h >> 7) * 0xffu;
+    } else {                             // all exponent bits; one more of them sets the sign bit
+        constexpr uint32_t e = CODE == EP_BF16 ? 0x7f807f80u : 0x7c007c00u, one = CODE == EP_BF16 ? 0x00800080u : 0x04000400u;
+        const uint32_t h = ((w & e) + one) & 0x80008000u;
+        return (h >> 15) * 0xffffu;
     }
 }
 
@@ -217,16 +231,14 @@ EP_DEV __amdgpu_buffer_rsrc_t tile_rsrc(const void *base, int64_t byte, bool ok,
     return buffer_rsrc((const char *)base + (ok ? byte : 0), ok ? (uint32_t)bytes : 0u);
 }
 
-// Workgroups of a kernel that a compute unit holds (waves of a SIMD).
-#ifndef OCC2
-#define OCC2 2
-#endif
-constexpr int attend_occupancy(int CW, int MT) { return CW == 4 ? (MT == 1 ? 3 : 2) : CW == 8 ? (MT == 1 ? 2 : OCC2) : 1; }
+// Workgroups of a kernel that a compute unit holds (waves of a SIMD).  Three of
+// the one-token kernels would fit at 128 values, and gain nothing.
+constexpr int attend_occupancy(int CW, int MT) { return CW == 4 ? (MT == 1 ? 3 : 2) : CW == 8 ? 2 : 1; }
 
 // QOP: type of the queries; CODE: EP_I8, EP_E4M3, or QOP's type.  KS: steps of
 // 32 values of a head, CW: output columns a lane (16 CW >= D), MT: 16-row
 // tiles of query rows.
-template <typename QOP, int CODE, int KS, int CW, int MT>
+template <typename QOP, int CODE, int KS, int CW, int MT, bool RAGGED>
 __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) attend_kernel(AttendArgs a)
 {
     constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
@@ -333,7 +345,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
 
         // ---- loads
         u32x4_t kr[2][KL];
-        uint32_t vr[8][VW];
+        uint32_t vr[VW][8];      // [dword of the columns][row]
         float ks[8], vs[8];
         bool good[2];
         int64_t at[2];       // row of each half's first position
@@ -378,20 +390,20 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
                 const auto r = tile_rsrc(a.c.v, at[t] * D * ES, good[t], 16 * D * ES);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    uint32_t *dst = vr[4 * t + i];
+                    const int row = 4 * t + i;
                     if constexpr (VW == 1)
-                        dst[0] = __builtin_amdgcn_raw_buffer_load_b32(r, voff[i], 0, kAttOnce);
+                        vr[0][row] = __builtin_amdgcn_raw_buffer_load_b32(r, voff[i], 0, kAttOnce);
                     else if constexpr (VW == 2) {
                         const auto w = __builtin_amdgcn_raw_buffer_load_b64(r, voff[i], 0, kAttOnce);
-                        dst[0] = w[0];
-                        dst[1] = w[1];
+                        vr[0][row] = w[0];
+                        vr[1][row] = w[1];
                     } else
 #pragma unroll
                         for (int c = 0; c < VW; c += 4) {
                             const auto w = __builtin_amdgcn_raw_buffer_load_b128(r, voff[i] + 4 * c, 0, kAttOnce);
 #pragma unroll
                             for (int x = 0; x < 4; ++x)
-                                dst[c + x] = w[x];
+                                vr[c + x][row] = w[x];
                         }
                 }
             }
@@ -516,37 +528,37 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
             // Values: what no row sees becomes zero (its weights are zero, and
             // zero times a NaN is NaN); what some rows see and others not is
             // taken out if it is not finite, and added where it is seen.
-            u32x4_t f[CW];
-#pragma unroll
-            for (int t = 0; t < CW; ++t)
+            // Operand of column t: eight rows' values side by side.
+            auto column = [&](const uint32_t (&rows)[8], int t) {
+                u32x4_t f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if constexpr (k8) {
                         float v0[2], v1[2];
                         if (t & 2) {
-                            codes2<CODE, true>(vr[2 * e][t / 4], v0[0], v0[1]);
-                            codes2<CODE, true>(vr[2 * e + 1][t / 4], v1[0], v1[1]);
+                            codes2<CODE, true>(rows[2 * e], v0[0], v0[1]);
+                            codes2<CODE, true>(rows[2 * e + 1], v1[0], v1[1]);
                         } else {
-                            codes2<CODE, false>(vr[2 * e][t / 4], v0[0], v0[1]);
-                            codes2<CODE, false>(vr[2 * e + 1][t / 4], v1[0], v1[1]);
+                            codes2<CODE, false>(rows[2 * e], v0[0], v0[1]);
+                            codes2<CODE, false>(rows[2 * e + 1], v1[0], v1[1]);
                         }
-                        f[t][e] = high_halves(v0[t & 1], v1[t & 1]);
+                        f[e] = high_halves(v0[t & 1], v1[t & 1]);
                     } else {
-                        f[t][e] = __builtin_amdgcn_perm(vr[2 * e + 1][t / 2], vr[2 * e][t / 2],
-                                                        t & 1 ? 0x07060302u : 0x05040100u);
+                        f[e] = __builtin_amdgcn_perm(rows[2 * e + 1], rows[2 * e], t & 1 ? 0x07060302u : 0x05040100u);
                     }
                 }
+                return f;
+            };
             if (edge) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int p = j0 + 16 * (e / 2) + 4 * g + 2 * (e % 2);
-                    const uint32_t keep = (p >= lo && p <= hi ? 0xffffu : 0u) |
-                                          (p + 1 >= lo && p + 1 <= hi ? 0xffff0000u : 0u);
+                for (int r = 0; r < 8; ++r) {
+                    const int p = j0 + 16 * (r / 4) + 4 * g + r % 4;
+                    const uint32_t keep = p >= lo && p <= hi ? ~0u : 0u;
 #pragma unroll
-                    for (int t = 0; t < CW; ++t)
-                        f[t][e] &= keep;
+                    for (int c = 0; c < VW; ++c)
+                        vr[c][r] &= keep;
                 }
-                if (CODE != EP_I8 && ragged) {
+                if (RAGGED && CODE != EP_I8 && ragged) {
                     u32x4_t one[MT];
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
@@ -555,33 +567,35 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
                             one[mt][e] = (seen[mt] >> (2 * e) & 1 ? VOP::kOne : 0u) |
                                          (seen[mt] >> (2 * e + 1) & 1 ? VOP::kOne << 16 : 0u);
 #pragma unroll
-                    for (int t = 0; t < CW; ++t) {
-                        u32x4_t odd;
-                        uint32_t some = 0;
+                    for (int c = 0; c < VW; ++c) {
+                        uint32_t odd[8], some = 0;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t z = ((f[t][e] & VOP::kExp) == VOP::kExp ? 0xffffu : 0u) |
-                                               ((f[t][e] >> 16 & VOP::kExp) == VOP::kExp ? 0xffff0000u : 0u);
-                            odd[e] = z & (VOP::kOne | VOP::kOne << 16);
-                            f[t][e] &= ~z;
-                            some |= z;
+                        for (int r = 0; r < 8; ++r) {
+                            odd[r] = not_finite<CODE>(vr[c][r]);
+                            some |= odd[r];
+                            vr[c][r] &= ~odd[r];
+                            odd[r] &= k8 ? 0x38383838u : VOP::kOne | VOP::kOne << 16;     // ones of the type
                         }
                         if (__any(some != 0))
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) {
-                                const f32x4_t hits = VOP::mfma(odd, one[mt], (f32x4_t){0, 0, 0, 0});
+                            for (int t = c * (4 / ES); t < (c + 1) * (4 / ES); ++t)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    o[mt][t][i] = hits[i] > 0.0f ? nan : o[mt][t][i];
-                            }
+                                for (int mt = 0; mt < MT; ++mt) {
+                                    const f32x4_t hits = VOP::mfma(column(odd, t), one[mt], (f32x4_t){0, 0, 0, 0});
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        o[mt][t][i] = hits[i] > 0.0f ? nan : o[mt][t][i];
+                                }
                     }
                 }
             }
 #pragma unroll
-            for (int t = 0; t < CW; ++t)
+            for (int t = 0; t < CW; ++t) {
+                const u32x4_t f = column(vr[t * ES / 4], t);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
-                    o[mt][t] = VOP::mfma(f[t], pl[mt], VOP::mfma(f[t], ph[mt], o[mt][t]));
+                    o[mt][t] = VOP::mfma(f, pl[mt], VOP::mfma(f, ph[mt], o[mt][t]));
+            }
             __builtin_amdgcn_sched_barrier(0);
             load_v();
         }
@@ -724,30 +738,32 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
 }
 
 // Instantiations of one pair of types, by D and rows (attend_gen_*.hip).
-template <typename QOP, int CODE, int MT>
+template <typename QOP, int CODE, int MT, bool RAGGED>
 void attend_by_size(const AttendArgs &a, unsigned grid, hipStream_t st)
 {
     constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
     const int D = a.c.D;
     if (D <= 64)
-        attend_kernel<QOP, CODE, 2, 4, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+        attend_kernel<QOP, CODE, 2, 4, MT, RAGGED><<<grid, 64 * kAttWaves, 0, st>>>(a);
     else if (!k8 && D <= 96)
-        attend_kernel<QOP, CODE, k8 ? 4 : 3, 8, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+        attend_kernel<QOP, CODE, k8 ? 4 : 3, 8, MT, RAGGED><<<grid, 64 * kAttWaves, 0, st>>>(a);
     else if (D <= 128)
-        attend_kernel<QOP, CODE, 4, 8, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+        attend_kernel<QOP, CODE, 4, 8, MT, RAGGED><<<grid, 64 * kAttWaves, 0, st>>>(a);
     else if (D <= 192)
-        attend_kernel<QOP, CODE, 6, 16, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+        attend_kernel<QOP, CODE, 6, 16, MT, RAGGED><<<grid, 64 * kAttWaves, 0, st>>>(a);
     else
-        attend_kernel<QOP, CODE, 8, 16, MT><<<grid, 64 * kAttWaves, 0, st>>>(a);
+        attend_kernel<QOP, CODE, 8, 16, MT, RAGGED><<<grid, 64 * kAttWaves, 0, st>>>(a);
 }
 
 template <typename QOP, int CODE>
 void attend_by_rows(const AttendArgs &a, int mt, unsigned grid, hipStream_t st)
 {
-    if (mt == 1)
-        attend_by_size<QOP, CODE, 1>(a, grid, st);
+    if (mt == 1 && a.tok.S == 1)
+        attend_by_size<QOP, CODE, 1, false>(a, grid, st);
+    else if (mt == 1)
+        attend_by_size<QOP, CODE, 1, true>(a, grid, st);
     else
-        attend_by_size<QOP, CODE, 2>(a, grid, st);
+        attend_by_size<QOP, CODE, 2, true>(a, grid, st);
 }
 
 void attend_bf16(const AttendArgs &a, int mt, unsigned grid, hipStream_t st);
