@@ -13,12 +13,14 @@
 // All of it is bound by the bytes of the rows.  Inputs are read once, and
 // large outputs leave the caches before they are read again, so both go past
 // them as non-temporal accesses: 16384 tokens of 32 + 8 heads of 128 turn in
-// 59 us (5.7 TB/s; 70 with plain accesses), 8 x 4096 rows of 8 heads are read
+// 58 us (5.8 TB/s; 70 with plain accesses), 8 x 4096 rows of 8 heads are read
 // out of an int8 cache in 35 us (50), two prompts of 4096 tokens enter an
-// e4m3 cache and are read back in 50 us (60).  Four rows of one token a group
+// e4m3 cache and are read back in 46 us (60).  Four rows of one token a group
 // of lanes, with one look-up of position, page and angles, were slower: lanes
 // of a wave then hold queries, keys and values at once and take every path
 // (those prompts 124 us), and one token's call grows with the code it fetches.
+// Position and row load side by side, page and angles after them: with the row
+// behind the position those prompts took 49.5 us, 8 tokens 3.4 instead of 3.2.
 #include "ep_common.h"
 #include "ep_internal.h"
 #include "ep_paged.h"
@@ -39,6 +41,14 @@ struct Rows {
     int64_t sb, ss, sh;
     int heads;
 };
+
+// a or b, field by field: a choice between two of the kernel's arguments by
+// address would load them from memory once more.
+EP_DEV Rows pick(bool first, const Rows &a, const Rows &b)
+{
+    return {first ? a.ptr : b.ptr, first ? a.sb : b.sb, first ? a.ss : b.ss, first ? a.sh : b.sh,
+            first ? a.heads : b.heads};
+}
 
 // Element index (within its row) of value e of a lane: chunk a, then chunk b.
 struct Chunks {
@@ -72,19 +82,33 @@ EP_DEV f16_t from_f32<f16_t>(float v) { return (f16_t)v; }
 template <>
 EP_DEV uint16_t from_f32<uint16_t>(float v) { return f32_to_bf16(v); }
 
-// 8 values from or to 16-byte aligned memory; loads of what is read once.
+// 8 values in 16-byte aligned memory, as they lie there.  Loads of what is
+// read once.
+template <typename T>
+struct Raw8 {
+    u32x4_t w[sizeof(T) / 2];
+    EP_DEV void load(const T *p)
+    {
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(T) / 2; ++i)
+            w[i] = __builtin_nontemporal_load((const u32x4_t *)p + i);
+    }
+    EP_DEV void widen(float *v) const
+    {
+        T r[8];
+        __builtin_memcpy(r, w, sizeof r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = to_f32<T>(r[i]);
+    }
+};
+
 template <typename T>
 EP_DEV void load8(const T *p, float *v)
 {
-    T r[8];
-    u32x4_t w[sizeof r / 16];
-#pragma unroll
-    for (unsigned i = 0; i < sizeof r / 16; ++i)
-        w[i] = __builtin_nontemporal_load((const u32x4_t *)p + i);
-    __builtin_memcpy(r, w, sizeof r);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        v[i] = to_f32<T>(r[i]);
+    Raw8<T> r;
+    r.load(p);
+    r.widen(v);
 }
 // STREAM: past the caches (a parameter of the kernels: a branch's two stores
 // would be merged into one plain store).
@@ -116,25 +140,48 @@ EP_DEV void turn_pair(float a, float b, float c, float s, float &ta, float &tb)
     tb = bc + as;
 }
 
-// The 16 values of lane u of the row at x, turned by position p (in the
-// tables) where `turned`.  VEC: chunks are loaded whole (D and, with a turn,
-// dim / 2 in whole chunks, everything 16-byte aligned); else value by value.
+// The 16 values of lane u of the row at x.  VEC: chunks are loaded whole (D
+// and, with a turn, dim / 2 in whole chunks, everything 16-byte aligned); else
+// value by value.  load() needs no position and goes ahead of what waits for
+// one; values() then turns by position p (in the tables) where `turned`.
 template <typename T, bool VEC>
-EP_DEV Chunks load_row(const T *x, int D, int u, const Turn &t, bool turned, int64_t p, float *v)
-{
-    if constexpr (VEC) {
-        const Chunks ch = chunks_of(u, t.dim, D);
-        load8(x + ch.a, v);
-        load8(x + ch.b, v + 8);
-        if (turned && 16 * u < t.dim) {
-            // cosines and sines of the pairs of both chunks
-            const float *cs = t.cos_t + p * (t.dim / 2), *sn = t.sin_t + p * (t.dim / 2);
-            const int i0 = t.interleaved ? ch.a / 2 : ch.a, i1 = t.interleaved ? ch.b / 2 : ch.a + 4;
+struct LaneRow {
+    const T *x;
+    int D, u;
+    Chunks ch;
+    Raw8<T> a, b;
+
+    EP_DEV void load(const T *src, int D_, int u_, const Turn &t)
+    {
+        x = src;
+        D = D_;
+        u = u_;
+        ch = VEC ? chunks_of(u, t.dim, D) : Chunks{16 * u, 16 * u + 8};
+        if constexpr (VEC) {
+            a.load(x + ch.a);
+            b.load(x + ch.b);
+        }
+    }
+    EP_DEV void values(const Turn &t, bool turned, int64_t p, float *v) const
+    {
+        const int half = t.dim / 2;
+        if constexpr (VEC) {
+            // cosines and sines of the pairs of both chunks (of some row, not
+            // used, where nothing turns: a branch would part the loads)
             float c[8], s[8];
-            __builtin_memcpy(c, __builtin_assume_aligned(cs + i0, 16), 16);
-            __builtin_memcpy(c + 4, __builtin_assume_aligned(cs + i1, 16), 16);
-            __builtin_memcpy(s, __builtin_assume_aligned(sn + i0, 16), 16);
-            __builtin_memcpy(s + 4, __builtin_assume_aligned(sn + i1, 16), 16);
+            const bool turns = turned && 16 * u < t.dim;
+            if (t.max_pos > 0) {
+                const int64_t at = turns ? p * half + (t.interleaved ? ch.a / 2 : ch.a) : 0;
+                const int64_t next = turns ? p * half + (t.interleaved ? ch.b / 2 : ch.a + 4) : 0;
+                __builtin_memcpy(c, __builtin_assume_aligned(t.cos_t + at, 16), 16);
+                __builtin_memcpy(c + 4, __builtin_assume_aligned(t.cos_t + next, 16), 16);
+                __builtin_memcpy(s, __builtin_assume_aligned(t.sin_t + at, 16), 16);
+                __builtin_memcpy(s + 4, __builtin_assume_aligned(t.sin_t + next, 16), 16);
+            }
+            a.widen(v);
+            b.widen(v + 8);
+            if (!turns)
+                return;
             if (t.interleaved) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -144,30 +191,26 @@ EP_DEV Chunks load_row(const T *x, int D, int u, const Turn &t, bool turned, int
                 for (int i = 0; i < 8; ++i)
                     turn_pair(v[i], v[i + 8], c[i], t.sign * s[i], v[i], v[i + 8]);
             }
-        }
-        return ch;
-    } else {
-        const Chunks ch{16 * u, 16 * u + 8};
-        const int half = t.dim / 2;
-        for (int e = 0; e < 16; ++e) {
-            const int d = 16 * u + e;
-            v[e] = d < D ? to_f32<T>(x[d]) : 0.0f;
-            if (turned && d < t.dim) {
-                const bool second = t.interleaved ? (d & 1) : d >= half;
-                const int i = t.interleaved ? d >> 1 : (second ? d - half : d);
-                const int other = t.interleaved ? d ^ 1 : (second ? d - half : d + half);
-                const float y = to_f32<T>(x[other]), c = t.cos_t[p * half + i], s = t.sign * t.sin_t[p * half + i];
-                float ta, tb;
-                if (second)
-                    turn_pair(y, v[e], c, s, ta, tb);
-                else
-                    turn_pair(v[e], y, c, s, ta, tb);
-                v[e] = second ? tb : ta;
+        } else {
+            for (int e = 0; e < 16; ++e) {
+                const int d = 16 * u + e;
+                v[e] = d < D ? to_f32<T>(x[d]) : 0.0f;
+                if (turned && d < t.dim) {
+                    const bool second = t.interleaved ? (d & 1) : d >= half;
+                    const int i = t.interleaved ? d >> 1 : (second ? d - half : d);
+                    const int other = t.interleaved ? d ^ 1 : (second ? d - half : d + half);
+                    const float y = to_f32<T>(x[other]), c = t.cos_t[p * half + i], s = t.sign * t.sin_t[p * half + i];
+                    float ta, tb;
+                    if (second)
+                        turn_pair(y, v[e], c, s, ta, tb);
+                    else
+                        turn_pair(v[e], y, c, s, ta, tb);
+                    v[e] = second ? tb : ta;
+                }
             }
         }
-        return ch;
     }
-}
+};
 
 template <bool VEC, bool STREAM, typename T>
 EP_DEV void store_row(T *y, int D, const Chunks &ch, const float *v)
@@ -250,6 +293,7 @@ EP_DEV Token token_at(const PagedTokens &t, uint32_t i)
     k.b = b;
     k.s = i - b * (uint32_t)t.S;
     k.p = t.pos[k.b * t.pos_sb + k.s * t.pos_ss];
+    __builtin_amdgcn_sched_barrier(0);      // ahead of the rows: what follows waits for it first
     return k;
 }
 
@@ -284,19 +328,19 @@ __global__ void __launch_bounds__(256) rotate_kernel(RotateArgs a)
         return;
     const Token t = token_at(a.tok, token);
     const bool is_q = head < a.q.heads;
-    const Rows &x = is_q ? a.q : a.k;
+    const Rows x = pick(is_q, a.q, a.k);
     const int h = is_q ? head : head - a.q.heads;
     T *y = (T *)(is_q ? a.q_out : a.k_out) + ((int64_t)token * x.heads + h) * a.D;
     float v[16];
+    LaneRow<T, VEC> row;
+    row.load((const T *)x.ptr + t.b * x.sb + t.s * x.ss + h * x.sh, a.D, u, a.turn);
     const bool ok = t.p >= 0 && t.p < a.turn.max_pos;
-    const Chunks ch = load_row<T, VEC>((const T *)x.ptr + t.b * x.sb + t.s * x.ss + h * x.sh, a.D, u, a.turn, ok, t.p, v);
-    if (!ok) {
-        const float fill = t.p < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
+    row.values(a.turn, ok, t.p, v);
+    const float fill = t.p < 0 ? 0.0f : __uint_as_float(0x7fc00000u);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            v[e] = fill;
-    }
-    store_row<VEC, STREAM>(y, a.D, ch, v);
+    for (int e = 0; e < 16; ++e)
+        v[e] = ok ? v[e] : fill;
+    store_row<VEC, STREAM>(y, a.D, row.ch, v);
 }
 
 struct AppendArgs {
@@ -334,28 +378,28 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a)
     const Token t = token_at(a.tok, token);
     const bool mine = 16 * u < D;   // lanes past the row only take part in its maximum
     const bool is_q = head < Hq, is_v = head >= Hq + Hk;
-    const Rows &x = is_q ? a.q : is_v ? a.v : a.k;
+    const Rows x = pick(is_q, a.q, pick(is_v, a.v, a.k));
     const int h = is_q ? head : is_v ? head - Hq - Hk : head - Hq;
+    LaneRow<T, VEC> lane_row;       // lanes past the row take its start
+    lane_row.load((const T *)x.ptr + t.b * x.sb + t.s * x.ss + h * x.sh, D, mine ? u : 0, a.turn);
+    const Chunks ch = lane_row.ch;
     const bool turns = !is_v && a.turn.dim > 0;
     const bool known = t.p >= 0 && (!turns || t.p < a.turn.max_pos);
+    int64_t page;
+    int row;
+    const bool stored = slot_of(a.tok, a.c, t.b, t.p, page, row);   // one answer for all lanes of a row
     float v[16];
-    Chunks ch{0, 0};
-    if (mine)
-        ch = load_row<T, VEC>((const T *)x.ptr + t.b * x.sb + t.s * x.ss + h * x.sh, D, u, a.turn, turns && known, t.p, v);
-    if (!mine || !known) {
-        const float fill = t.p < 0 || !mine ? 0.0f : __uint_as_float(0x7fc00000u);
+    lane_row.values(a.turn, turns && known, t.p, v);
+    const float fill = t.p < 0 || !mine ? 0.0f : __uint_as_float(0x7fc00000u);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            v[e] = fill;
-    }
+    for (int e = 0; e < 16; ++e)
+        v[e] = mine && known ? v[e] : fill;
     if (is_q) {
         if (mine)
             store_row<VEC, STREAM>((T *)a.q_out + ((int64_t)token * Hq + h) * D, D, ch, v);
         return;
     }
-    int64_t page = 0;
-    int row = 0;
-    if (!known || !slot_of(a.tok, a.c, t.b, t.p, page, row))   // one answer for all lanes of a row
+    if (!known || !stored)
         return;
     const int64_t at = (page * Hk + h) * a.c.page + row;
     void *dst = is_v ? a.c.v : a.c.k;

@@ -174,3 +174,17 @@ def test_a_workspace_that_is_too_small_is_refused():
     for p, n in ((ws.data_ptr(), need - 1), (None, need), (None, 0)):
         assert _abi.lib.ep_paged_attention(*args(p, n)) == -3 and _abi.last_error()
     assert _abi.lib.ep_paged_attention(*args(ws.data_ptr() + 8, need)) == 2
+
+
+@pytest.mark.parametrize("dim", [64, 40])
+def test_a_rotation_without_positions_has_no_tables(dim):
+    """max_pos 0: the tables may be null, and every position lies past them."""
+    g = gen(8)
+    x, out = normal(g, 1, 3, 2, 64), torch.zeros(1, 3, 2, 64, dtype=BF16, device=DEV)
+    pos = torch.tensor([[0, -1, 5]], device=DEV)
+    heads = _abi.Heads(x.data_ptr(), _abi.BF16, 2, 384, 128, 64)
+    tok = _abi.Tokens(1, 3, pos.data_ptr(), 3, 1, None, 0, 0)
+    stream = _abi.stream_handle(DEV)
+    assert _abi.lib.ep_rotate(heads, None, _abi.Rotation(None, None, 0, dim, 0), tok, 64, 0, out.data_ptr(), None,
+                              stream) == 0
+    assert out[0, [0, 2]].isnan().all() and (out[0, 1] == 0).all()
