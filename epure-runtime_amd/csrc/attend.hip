@@ -95,12 +95,13 @@ int piece_tiles(const PagedCache &c, int workers)
 
 constexpr size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
-// Segments of few tiles go to a workgroup each: up to 16 tiles (22 tiles of 8
-// segments take 11.4 us so, 10.2 shared), or 32 where the segments alone fill
-// the compute units (512 segments of 16 tiles: 17 us, 22 shared; 256 of 1 to
-// 128 tiles: 64 us, 59 shared).  Else all tiles are shared evenly among
-// `workers`, as many workgroups as are resident at once, and the pieces joined (where 32 bits count all
-// tiles that the table could hold).
+// Segments of few tiles go to a workgroup each: up to 16 tiles, or up to 32
+// the more segments there are to fill the compute units (8 segments of 22 tiles
+// take 11.4 us so, 10.2 shared; 64 of 19, 12.0 and 13.1; 128 of 19, 12.5 and
+// 17.2; 512 of 16, 17 and 22; 256 of 1 to 128, 64 and 59).  Else all tiles are
+// shared evenly among `workers`, as many workgroups as are resident at once,
+// and the pieces joined (where 32 bits count all tiles that the table could
+// hold).
 Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t window)
 {
     Plan p{};
@@ -112,7 +113,7 @@ Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_
     // a window's tiles, if the call's tokens follow one another
     const int64_t most = window > 0 && window <= tiles * kAttTile
                              ? std::min(tiles, (window + tok.S) / kAttTile + 2) : tiles;
-    if (most > (p.segments >= 256 ? 32 : 16) && p.segments < 0x40000000 && tiles + kMostPiece < 0x7fff0000 / p.segments) {
+    if (most > std::min<int64_t>(16 + p.segments / 8, 32) && p.segments < 0x40000000 && tiles + kMostPiece < 0x7fff0000 / p.segments) {
         p.workers = 256 * attend_occupancy(c.D <= 64 ? 4 : c.D <= 128 ? 8 : 16, p.mt);
         const size_t slots = (size_t)2 * p.workers * (rows < rm ? rows : rm);
         p.desc = up16(p.segments * sizeof(int2));
