@@ -81,6 +81,8 @@ struct Plan {
     size_t desc, ml, o;     // bytes of the workspace's parts
 };
 
+int row_bytes(const PagedCache &c) { return c.D * (c.dtype == EP_F16 || c.dtype == EP_BF16 ? 2 : 1); }
+
 // A piece takes some 6 us beyond its tiles, and a tile as long as a worker's
 // part of the bandwidth needs for its bytes: 6 tiles' time for 128 16-bit
 // values and 512 workers.  Short sequences of a ragged batch cost that much
@@ -89,8 +91,7 @@ struct Plan {
 constexpr int kMostPiece = 786432 / (16 * 256);
 int piece_tiles(const PagedCache &c, int workers)
 {
-    const int row = c.D * (c.dtype == EP_F16 || c.dtype == EP_BF16 ? 2 : 1);
-    return 786432 / (row * std::max(workers, 256));
+    return 786432 / (row_bytes(c) * std::max(workers, 256));
 }
 
 constexpr size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
@@ -102,6 +103,14 @@ constexpr size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 // shared evenly among `workers`, as many workgroups as are resident at once,
 // and the pieces joined (where 32 bits count all tiles that the table could
 // hold).
+//
+// A long call goes to one workgroup a compute unit where its four waves' tiles
+// are 16 KiB each: what is in flight is enough, and there are half as many
+// pieces (4 x 131072 bf16 positions of 128 values 301 us, 307 with two; one
+// head of 131072 27 and 33; 32 rows a key head 48 and 51).  Smaller tiles need
+// the second one (48 x 8192 in int8: 107 us with one, 86 with two; of 80 bf16
+// values 31.5 and 29.3), and short calls both (one sequence of 8000: 15.9 and
+// 15.2).
 Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t window)
 {
     Plan p{};
@@ -160,14 +169,14 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
     a.blocks = (int)((rows + rm - 1) / rm);
     a.units = (uint32_t)(tok.B * a.blocks);
     a.workers = p.workers;
+    a.few = row_bytes(c) >= 256 ? 256 : p.workers;
     a.piece = piece_tiles(c, p.workers);
     // Values pass the caches on their way (4 x 131072 positions in 313 us, 348
     // with plain loads).  Keys do too (308) unless they are read again soon: by
     // a sequence's next unit in this call (64 rows a key head: 85 us, 79 with
     // plain key loads), or by the next call where the 256 MB behind the L2
     // caches hold a few such pools (16 x 2-4 thousand int8 positions: 28.7, 26.9).
-    a.keys_once = a.blocks == 1 && c.n_pages * c.heads * c.page * c.D * (c.dtype == EP_F16 || c.dtype == EP_BF16 ? 2 : 1)
-                                       > (int64_t)80 << 20;
+    a.keys_once = a.blocks == 1 && c.n_pages * c.heads * c.page * row_bytes(c) > (int64_t)80 << 20;
     a.slot_rows = (int)(rows < rm ? rows : rm);
     a.desc = (int2 *)ws;
     a.part_ml = (float2 *)((char *)ws + p.desc);

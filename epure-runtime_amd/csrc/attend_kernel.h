@@ -32,9 +32,9 @@
 // or a NaN (it meets both terms).
 //
 // Bound by the bytes of keys and values: 4 x 131072 positions of 8 heads of
-// 128 in bf16, 2.06 GB, take 304 us (6.8 TB/s) and 48 of up to 8192 in int8,
-// 441 MB, 81 us, four waves a workgroup and two workgroups a compute unit, 16
-// KiB (bf16) in flight a wave.  Short calls are a chain of loads: arguments,
+// 128 in bf16, 2.06 GB, take 297 us (6.9 TB/s) and 48 of up to 8192 in int8,
+// 441 MB, 81 us, four waves a workgroup with a tile of 16 KiB (bf16) in flight
+// each, one or two workgroups a compute unit.  Short calls are a chain of loads: arguments,
 // positions with pages and queries, keys and values, 7 us in all for 129
 // positions; the code is kept small (10 KB) because it is fetched cold.
 #pragma once
@@ -65,6 +65,7 @@ struct AttendArgs {
     int blocks;              // units of a sequence
     uint32_t units;
     int workers;             // workgroups that share all tiles evenly; 0: one workgroup a segment
+    int few;                 // shares of a large call, of more than 16 tiles each
     int piece;               // tiles' time that beginning and ending a piece takes
     int keys_once;           // keys are loaded past the caches, as values are
     int slot_rows;           // rows kept of a piece: min(rows, 16 MT)
@@ -691,7 +692,8 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
             counting = false;
             // At least a tile a wave, and up to two while that leaves a share to
             // every compute unit: one workgroup on each before a second.
-            per = max((total + a.workers - 1) / (uint32_t)a.workers,
+            const uint32_t shares = total > 16u * a.few ? a.few : a.workers;
+            per = max((total + shares - 1) / shares,
                       min(max((total + 255) / 256, (uint32_t)kAttWaves), 2u * kAttWaves));
             f = begin = min(blockIdx.x * per, total);
             stop = min(begin + per, total);
