@@ -51,17 +51,21 @@ class BatchDecoder:
         self.owned[i], self.lengths[i] = [], 0
         self.table[i].fill_(-1)
 
-    def _grow(self, i, n):
-        """Pages for n more positions of sequence i."""
-        have, need = len(self.owned[i]), -(-(self.lengths[i] + n) // self.page)
+    def _more(self, i, n):
+        """How many pages n more positions of sequence i take."""
         if self.lengths[i] + n > self.max_len:
             raise ValueError(f"sequence {i}: {self.lengths[i] + n} positions, at most {self.max_len}")
-        if need - have > len(self.free):
-            raise RuntimeError(f"out of pages: sequence {i} needs {need - have}, {len(self.free)} are free")
-        if need > have:
-            new = [self.free.pop() for _ in range(need - have)]
+        return -(-(self.lengths[i] + n) // self.page) - len(self.owned[i])
+
+    def _grow(self, i, n):
+        """Pages for n more positions of sequence i."""
+        have, more = len(self.owned[i]), self._more(i, n)
+        if more > len(self.free):
+            raise RuntimeError(f"out of pages: sequence {i} needs {more}, {len(self.free)} are free")
+        if more > 0:
+            new = [self.free.pop() for _ in range(more)]
             self.owned[i] += new
-            self.table[i, have:need] = torch.tensor(new, dtype=torch.int32, device=self.table.device)
+            self.table[i, have:have + more] = torch.tensor(new, dtype=torch.int32, device=self.table.device)
         self.lengths[i] += n
 
     @torch.no_grad()
@@ -72,6 +76,11 @@ class BatchDecoder:
         dev, cfg = self.table.device, self.cfg
         if len(tokens) > self.table.shape[0]:
             raise ValueError(f"{len(tokens)} sequences in a batch of {self.table.shape[0]}")
+        if any(not 0 <= t < cfg.vocab for new in tokens for t in new):
+            raise ValueError(f"token ids must lie in [0, {cfg.vocab})")
+        need = sum(self._more(i, len(t)) for i, t in enumerate(tokens))
+        if need > len(self.free):       # before any sequence grows
+            raise RuntimeError(f"out of pages: the call needs {need}, {len(self.free)} are free")
         for i, t in enumerate(tokens):
             if len(t) > 0:
                 self._grow(i, len(t))

@@ -293,7 +293,9 @@ class PagedKVCache:
 
         With ``rotary``, k is turned on its way into the cache and q (if
         given, [B, S, q heads, D]) on its way out; returns q turned, or None
-        without q.  A turned key is rounded once, to the cache's type."""
+        without q.  A turned key is rounded once, to the cache's type.  Tokens
+        of one call at the same place of a page race: what it holds then is
+        neither's for certain."""
         call = _native()
         if call is not None:
             cos, sin, inter = (None, None, False) if rotary is None else \

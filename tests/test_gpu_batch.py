@@ -80,3 +80,16 @@ def test_a_sequence_does_not_depend_on_the_pages_it_gets():
     d.free = keep[::-1]
     assert again == first
     assert all(len(o) == 8 for o in first)
+
+
+def test_a_call_that_does_not_fit_changes_nothing():
+    w = random_weights(DecoderConfig(256, 256, 1, 2, 1, 64, 50, 1e4), device="cpu")
+    d = BatchDecoder(w, 3, 64, page=16, n_pages=5)
+    d._grow(1, 16)
+    table = d.table.clone()
+    for bad, error in (([[1] * 33, [], [1] * 33], RuntimeError),     # 6 pages of 4
+                       ([[1], [1] * 49], ValueError),                # past max_len
+                       ([[1], [50]], ValueError), ([[1], [3, -1]], ValueError)):
+        with pytest.raises(error):
+            d.forward(bad)
+        assert d.lengths == [0, 16, 0] and len(d.free) == 4 and (d.table == table).all()
