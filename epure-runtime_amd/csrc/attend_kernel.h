@@ -415,6 +415,14 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
         // ---- the running softmax
         float m[MT], l[MT];
         f32x4_t o[MT][CW];
+        // Outputs that a value which is not finite has reached.  Written into the
+        // sums where they happen, they hold some 80 registers more in the loop,
+        // which with 16 columns a lane and two row tiles does not fit: 36 of them
+        // went through memory, in the queue of the rows' loads (16 x 2-4 thousand
+        // positions of 256 bf16 values, 32 rows a key head: 73 us, 57 with a bit
+        // each, looked at in the end).  With 8 columns the bits cost some 25 more.
+        constexpr bool kHitsApart = RAGGED && CODE != EP_I8 && CW == 16;
+        uint32_t hit[MT][2] = {};
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             m[mt] = -INFINITY;
@@ -585,7 +593,10 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
                                     const f32x4_t hits = VOP::mfma(column(odd, t), one[mt], (f32x4_t){0, 0, 0, 0});
 #pragma unroll
                                     for (int i = 0; i < 4; ++i)
-                                        o[mt][t][i] = hits[i] > 0.0f ? nan : o[mt][t][i];
+                                        if constexpr (kHitsApart)
+                                            hit[mt][t / 8] |= (hits[i] > 0.0f ? 1u : 0u) << (4 * (t % 8) + i);
+                                        else
+                                            o[mt][t][i] = hits[i] > 0.0f ? nan : o[mt][t][i];
                                 }
                     }
                 }
@@ -608,6 +619,12 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
         const int rows = min(RM, a.rows - r0);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
+            if constexpr (kHitsApart)
+#pragma unroll
+                for (int t = 0; t < CW; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[mt][t][i] = hit[mt][t / 8] >> (4 * (t % 8) + i) & 1 ? nan : o[mt][t][i];
             l[mt] = xor32_sum(xor16_sum(l[mt]));
             if (eg == 0) {
                 s_m[wave][16 * mt + en] = m[mt];

@@ -188,3 +188,35 @@ def test_a_rotation_without_positions_has_no_tables(dim):
     assert _abi.lib.ep_rotate(heads, None, _abi.Rotation(None, None, 0, dim, 0), tok, 64, 0, out.data_ptr(), None,
                               stream) == 0
     assert out[0, [0, 2]].isnan().all() and (out[0, 1] == 0).all()
+
+
+@pytest.mark.parametrize("length", [90, 3000])
+@pytest.mark.parametrize("group", [2, 4])
+@pytest.mark.parametrize("dim,dtype", [(64, F16), (96, BF16), (128, BF16), (192, F16), (256, BF16), (256, F16),
+                                       (192, E4M3), (256, E4M3)])
+def test_values_that_are_not_finite_reach_the_rows_and_columns_that_see_them(dim, dtype, group, length):
+    """Eight tokens, 16 or 32 rows a key head; windows that begin and end
+    around positions with an infinity or a NaN in a column of every four."""
+    g = gen(9)
+    qdt = dtype if dtype.itemsize == 2 else BF16
+    pages = -(-length // 16)
+    cache = epure.PagedKVCache(pages, 16, 2, dim, dtype, DEV)
+    table = torch.randperm(pages, generator=g, device=DEV).to(torch.int32)[None]
+    pos = torch.arange(length, device=DEV)[None]
+    k, v = normal(g, 1, length, 2, dim, dtype=F32), normal(g, 1, length, 2, dim, dtype=F32)
+    v[0, length - 5, 0, 0::4] = float("inf")
+    v[0, length - 3, 1, 3::4] = float("nan")
+    v[0, length - 3, 0, dim - 1] = float("-inf")
+    v[0, 22, :, 1::4] = float("nan")
+    cache.append(k, v, pos, table)
+    kc, vc = op.stands_for(k, dtype), op.stands_for(v, dtype)
+    q = normal(g, 1, 8, 2 * group, dim, dtype=qdt)
+    rows = torch.arange(length - 8, length, device=DEV)[None]
+    window = length - 26                 # from 19 .. 26: the first four rows see 22
+    out = cache.attend(q, rows, table, window=window).cpu()
+    want, mag, big = op.attend(q, kc, vc, rows.cpu(), dim ** -0.5, window)
+    clean = torch.isfinite(want)
+    assert clean.any() and not clean.all()
+    assert torch.equal(torch.isfinite(out), clean)
+    tol = op.attend_tolerance(want, mag, big, qdt, dim)
+    assert ((out.double() - want).abs() <= tol)[clean].all()
