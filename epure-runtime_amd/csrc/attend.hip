@@ -105,12 +105,13 @@ constexpr size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 // hold).
 //
 // A long call goes to one workgroup a compute unit where its four waves' tiles
-// are 16 KiB each: what is in flight is enough, and there are half as many
+// are 12 KiB each: what is in flight is enough, and there are half as many
 // pieces (4 x 131072 bf16 positions of 128 values 301 us, 307 with two; one
-// head of 131072 27 and 33; 32 rows a key head 48 and 51).  Smaller tiles need
-// the second one (48 x 8192 in int8: 107 us with one, 86 with two; of 80 bf16
-// values 31.5 and 29.3), and short calls both (one sequence of 8000: 15.9 and
-// 15.2).
+// head of 131072 27 and 33; 32 rows a key head 48 and 51; 192 int8 values, 4 x
+// 131072 positions 280 and 283, one head 31 and 41, 16 x 2-8 thousand 34.4 and
+// 33.3).  Smaller tiles need the second one (48 x 8192 in int8: 107 us with
+// one, 86 with two; of 80 bf16 values 31.5 and 29.3), and short calls both (one
+// sequence of 8000: 15.9 and 15.2).
 Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t window)
 {
     Plan p{};
@@ -123,7 +124,7 @@ Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_
     const int64_t most = window > 0 && window <= tiles * kAttTile
                              ? std::min(tiles, (window + tok.S) / kAttTile + 2) : tiles;
     if (most > std::min<int64_t>(16 + p.segments / 8, 32) && p.segments < 0x40000000 && tiles + kMostPiece < 0x7fff0000 / p.segments) {
-        p.workers = 256 * attend_occupancy(c.D <= 64 ? 4 : c.D <= 128 ? 8 : 16, p.mt);
+        p.workers = 256 * attend_occupancy(attend_columns(c.D), p.mt, tok.S > 1 && c.dtype != EP_I8);
         const size_t slots = (size_t)2 * p.workers * (rows < rm ? rows : rm);
         p.desc = up16(p.segments * sizeof(int2));
         p.ml = up16(slots * sizeof(float2));
@@ -169,7 +170,7 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
     a.blocks = (int)((rows + rm - 1) / rm);
     a.units = (uint32_t)(tok.B * a.blocks);
     a.workers = p.workers;
-    a.few = row_bytes(c) >= 256 ? 256 : p.workers;
+    a.few = row_bytes(c) >= 192 ? 256 : p.workers;
     a.piece = piece_tiles(c, p.workers);
     // Values pass the caches on their way (4 x 131072 positions in 313 us, 348
     // with plain loads).  Keys do too (308) unless they are read again soon: by

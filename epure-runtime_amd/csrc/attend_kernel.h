@@ -34,9 +34,9 @@
 // Bound by the bytes of keys and values: 4 x 131072 positions of 8 heads of
 // 128 in bf16, 2.06 GB, take 297 us (6.9 TB/s) and 48 of up to 8192 in int8,
 // 441 MB, 81 us, four waves a workgroup with a tile of 16 KiB (bf16) in flight
-// each, one or two workgroups a compute unit.  Short calls are a chain of loads: arguments,
-// positions with pages and queries, keys and values, 7 us in all for 129
-// positions; the code is kept small (10 KB) because it is fetched cold.
+// each, one or two workgroups a compute unit.  Short calls are a chain of loads:
+// arguments, positions with pages and queries, keys and values, 7 us in all for
+// 129 positions; the code is kept small (10 KB) because it is fetched cold.
 #pragma once
 
 #include "ep_common.h"
@@ -233,14 +233,27 @@ EP_DEV __amdgpu_buffer_rsrc_t tile_rsrc(const void *base, int64_t byte, bool ok,
 }
 
 // Workgroups of a kernel that a compute unit holds (waves of a SIMD).  Three of
-// the one-token kernels would fit at 128 values, and gain nothing.
-constexpr int attend_occupancy(int CW, int MT) { return CW == 4 ? (MT == 1 ? 3 : 2) : CW == 8 ? 2 : 1; }
+// the one-token kernels would fit at 128 values, and gain nothing.  `lookout`:
+// several tokens over values that may each be infinite or a NaN; what looks
+// for them takes some 40 registers, too many for two waves with 12 columns
+// (33 would go through memory).
+constexpr int attend_occupancy(int CW, int MT, bool lookout)
+{
+    return CW == 4 ? (MT == 1 ? 3 : 2) : CW == 8 || (CW == 12 && MT == 1 && !lookout) ? 2 : 1;
+}
+
+// Output columns a lane for heads of D values: 16 lanes read a row, and a
+// lane's columns end where the row does.  Against 16, 12 columns leave room for
+// a second wave on the SIMD with one new token, and a quarter of the second
+// product out (16 x 2-4 thousand positions: 144 int8 values 23.3 us, 27.0 with
+// 16 columns; 192 bf16 values 36.8 and 37.8, 32 rows a key head 45.8 and 48.7).
+constexpr int attend_columns(int D) { return D <= 64 ? 4 : D <= 128 ? 8 : D <= 192 && D % 12 == 0 ? 12 : 16; }
 
 // QOP: type of the queries; CODE: EP_I8, EP_E4M3, or QOP's type.  KS: steps of
 // 32 values of a head, CW: output columns a lane (16 CW >= D), MT: 16-row
 // tiles of query rows.
 template <typename QOP, int CODE, int KS, int CW, int MT, bool RAGGED>
-__global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) attend_kernel(AttendArgs a)
+__global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGED && CODE != EP_I8)) attend_kernel(AttendArgs a)
 {
     constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
     constexpr int ES = k8 ? 1 : 2, KL = k8 ? KS / 2 : KS, RM = 16 * MT, DP = 16 * CW, VW = CW * ES / 4;
@@ -401,10 +414,21 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
                     } else
 #pragma unroll
                         for (int c = 0; c < VW; c += 4) {
-                            const auto w = __builtin_amdgcn_raw_buffer_load_b128(r, voff[i] + 4 * c, 0, kAttOnce);
+                            if (c + 4 <= VW) {
+                                const auto w = __builtin_amdgcn_raw_buffer_load_b128(r, voff[i] + 4 * c, 0, kAttOnce);
 #pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                vr[c + x][row] = w[x];
+                                for (int x = 0; x < 4; ++x)
+                                    vr[c + x][row] = w[x];
+                            } else if (c + 3 == VW) {
+                                const auto w = __builtin_amdgcn_raw_buffer_load_b96(r, voff[i] + 4 * c, 0, kAttOnce);
+#pragma unroll
+                                for (int x = 0; x < 3; ++x)
+                                    vr[c + x][row] = w[x];
+                            } else {
+                                const auto w = __builtin_amdgcn_raw_buffer_load_b64(r, voff[i] + 4 * c, 0, kAttOnce);
+                                vr[c][row] = w[0];
+                                vr[c + 1][row] = w[1];
+                            }
                         }
                 }
             }
@@ -421,7 +445,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT)) atte
         // went through memory, in the queue of the rows' loads (16 x 2-4 thousand
         // positions of 256 bf16 values, 32 rows a key head: 73 us, 57 with a bit
         // each, looked at in the end).  With 8 columns the bits cost some 25 more.
-        constexpr bool kHitsApart = RAGGED && CODE != EP_I8 && CW == 16;
+        constexpr bool kHitsApart = RAGGED && CODE != EP_I8 && CW >= 12;
         uint32_t hit[MT][2] = {};
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -768,6 +792,8 @@ void attend_by_size(const AttendArgs &a, unsigned grid, hipStream_t st)
         attend_kernel<QOP, CODE, k8 ? 4 : 3, 8, MT, RAGGED><<<grid, 64 * kAttWaves, 0, st>>>(a);
     else if (D <= 128)
         attend_kernel<QOP, CODE, 4, 8, MT, RAGGED><<<grid, 64 * kAttWaves, 0, st>>>(a);
+    else if (D <= 192 && attend_columns(D) == 12)
+        attend_kernel<QOP, CODE, 6, 12, MT, RAGGED><<<grid, 64 * kAttWaves, 0, st>>>(a);
     else if (D <= 192)
         attend_kernel<QOP, CODE, 6, 16, MT, RAGGED><<<grid, 64 * kAttWaves, 0, st>>>(a);
     else

@@ -220,3 +220,17 @@ def test_values_that_are_not_finite_reach_the_rows_and_columns_that_see_them(dim
     assert torch.equal(torch.isfinite(out), clean)
     tol = op.attend_tolerance(want, mag, big, qdt, dim)
     assert ((out.double() - want).abs() <= tol)[clean].all()
+
+
+@pytest.mark.parametrize("dtype,qdt", [(BF16, BF16), (F16, F16), (I8, F16), (E4M3, BF16)])
+@pytest.mark.parametrize("S,group", [(1, 5), (2, 6), (3, 7)])
+@pytest.mark.parametrize("D", [32, 112, 144, 160, 176, 208])
+def test_head_sizes_between_powers_of_two(D, S, group, dtype, qdt):
+    """What 16 lanes with 4, 8, 12 or 16 columns each cover, in part and whole."""
+    g = gen(10)
+    lengths = [1 + S, 200, 1700]
+    cache, table, kc, vc = filled(g, lengths, 32, 2, D, dtype)
+    pos = (torch.tensor(lengths, device=DEV)[:, None] - S + torch.arange(S, device=DEV))
+    q = normal(g, 3, S, 2 * group, D, dtype=qdt)
+    check(cache, table, q, pos, kc, vc)
+    check(cache, table, q, pos, kc, vc, window=37)
