@@ -88,6 +88,13 @@ def _tokens(x, positions, table=None):
     return t, (positions, table)
 
 
+# Keys of a scaling that some kind reads, or that say nothing about the
+# frequencies of ``dim`` rotated values (dim is the rotated part already).
+_SCALING_KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "factor",
+                 "original_max_position_embeddings", "low_freq_factor", "high_freq_factor", "beta_fast", "beta_slow",
+                 "attention_factor", "mscale", "mscale_all_dim", "truncate"}
+
+
 def rope_frequencies(dim, theta=10000.0, scaling=None):
     """Angle per position of the dim / 2 pairs (float64) and the attention factor.
 
@@ -97,9 +104,17 @@ def rope_frequencies(dim, theta=10000.0, scaling=None):
     ``original_max_position_embeddings``: frequencies of fewer turns within
     the original context than ``low`` are divided by the factor, those of
     more than ``high`` kept, those between blended) or "yarn" (``factor``,
-    ``original_max_position_embeddings``, ``beta_fast`` 32, ``beta_slow`` 1,
-    ``attention_factor``: the blend is linear in the pair's index between the
-    pairs that make ``beta_fast`` and ``beta_slow`` turns)."""
+    ``original_max_position_embeddings``, ``beta_fast`` 32, ``beta_slow`` 1:
+    the blend is linear in the pair's index between the pairs that make
+    ``beta_fast`` and ``beta_slow`` turns, widened to whole indices unless
+    ``truncate`` is false; the attention factor is ``attention_factor``, or
+    M(mscale) / M(mscale_all_dim) with both given, or M(1), where M(s) = 0.1 s
+    ln(factor) + 1, and 1 for factors up to 1).  A key that none of them knows
+    raises ValueError."""
+    if scaling is not None:
+        unknown = sorted(k for k, v in scaling.items() if v is not None and k not in _SCALING_KEYS)
+        if unknown:
+            raise ValueError(f"rope scaling: {', '.join(map(str, unknown))} not served")
     f = float(theta) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
     kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
     if kind == "default":
@@ -119,12 +134,16 @@ def rope_frequencies(dim, theta=10000.0, scaling=None):
         keep = ((old * f / (2 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)
         return keep * f + (1.0 - keep) * f / factor, 1.0
     pair = lambda turns: dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
-    lo = max(math.floor(pair(float(scaling.get("beta_fast") or 32.0))), 0)
-    hi = min(math.ceil(pair(float(scaling.get("beta_slow") or 1.0))), dim - 1)
+    lo, hi = pair(float(scaling.get("beta_fast") or 32.0)), pair(float(scaling.get("beta_slow") or 1.0))
+    if scaling.get("truncate") is None or scaling["truncate"]:
+        lo, hi = math.floor(lo), math.ceil(hi)
+    lo, hi = max(lo, 0), min(hi, dim - 1)
     ramp = ((torch.arange(dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
     m = scaling.get("attention_factor")
     if m is None:
-        m = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+        grow = lambda s: 0.1 * s * math.log(factor) + 1.0 if factor > 1.0 else 1.0  # noqa: E731
+        one, every = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        m = grow(float(one)) / grow(float(every)) if one and every else grow(1.0)
     return f * (1.0 - ramp) + f / factor * ramp, float(m)
 
 
