@@ -384,7 +384,8 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a)
     lane_row.load((const T *)x.ptr + t.b * x.sb + t.s * x.ss + h * x.sh, D, mine ? u : 0, a.turn);
     const Chunks ch = lane_row.ch;
     const bool turns = !is_v && a.turn.dim > 0;
-    const bool known = t.p >= 0 && (!turns || t.p < a.turn.max_pos);
+    // one answer for a token's q, k and v: a value without its key is not stored either
+    const bool known = t.p >= 0 && (a.turn.dim == 0 || t.p < a.turn.max_pos);
     int64_t page;
     int row;
     const bool stored = slot_of(a.tok, a.c, t.b, t.p, page, row);   // one answer for all lanes of a row

@@ -1,0 +1,63 @@
+"""The paged operators where a call is out of the ordinary: tokens past the
+rotation's tables, derivatives that only some tensors want, huge scores."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import epure
+from epure.kernels import _abi, cuda
+from oracle import paged as op
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+BF16, F16, F32, I8, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.int8, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _library():
+    assert cuda.available()
+
+
+@pytest.fixture(params=["native", "python"])
+def path(request, monkeypatch):
+    """Each call path of the operators."""
+    assert _abi.call is not None, _abi.CALL_ERROR
+    if request.param == "python":
+        monkeypatch.setattr(_abi, "call", None)
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def normal(g, *shape, dtype=BF16, std=1.0):
+    return (torch.randn(*shape, generator=g, device=DEV) * std).to(dtype)
+
+
+def raw(cache):
+    """Everything that a cache holds, as bytes."""
+    return [t.view(torch.uint8).clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+
+
+# ------------------------------------------------------------------ past the rotation's tables
+@pytest.mark.parametrize("dtype", [BF16, F16, I8, E4M3])
+@pytest.mark.parametrize("rot", [64, 40])
+def test_a_token_past_the_rotations_tables_stores_neither_key_nor_value(dtype, rot, path):
+    g = gen(1)
+    r = epure.Rotary(rot, 10, device=DEV)
+    q, k, v = (normal(g, 2, 13, h, 64) for h in (4, 2, 2))
+    pos = torch.stack((torch.arange(13), 12 - torch.arange(13))).to(DEV)
+    pos[0, 3] = -1
+    table = torch.tensor([[2], [0]], dtype=torch.int32, device=DEV)
+    caches = [epure.PagedKVCache(3, 16, 2, 64, dtype, DEV) for _ in range(3)]
+    for c in caches:
+        for t in (c.k, c.v):
+            t.view(torch.uint8).fill_(0x5a)
+    caches[0].append(k, v, torch.where(pos < 10, pos, -1), table, rotary=r)     # the rest as padding
+    qo = caches[1].append(k, v, pos, table, q=q, rotary=r)
+    assert caches[2].append(k, v, pos, table, rotary=r) is None
+    past = pos >= 10
+    assert qo[past].isnan().all() and not qo[~past].isnan().any()
+    for c in caches[1:]:
+        for a, b in zip(raw(caches[0]), raw(c)):
+            assert torch.equal(a, b)
