@@ -400,6 +400,7 @@ class PagedKVCache:
         n = _abi.lib.ep_paged_attention_workspace(qh, tok, cache)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         _run("ep_paged_attention", _abi.lib.ep_paged_attention(
-            qh, tok, cache, self.dim ** -0.5 if scale is None else float(scale), int(window or 0), out.data_ptr(),
+            qh, tok, cache, self.dim ** -0.5 if scale is None else float(scale),
+            min(int(window or 0), 2 ** 63 - 1), out.data_ptr(),     # 64 bits there: more would wrap
             ws.data_ptr() if n else None, n, _abi.stream_handle(q.device)))
         return out

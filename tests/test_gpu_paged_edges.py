@@ -61,3 +61,15 @@ def test_a_token_past_the_rotations_tables_stores_neither_key_nor_value(dtype, r
     for c in caches[1:]:
         for a, b in zip(raw(caches[0]), raw(c)):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ windows
+@pytest.mark.parametrize("window", [300, 2 ** 31, 2 ** 63 - 1, 2 ** 63, 2 ** 64 + 5, 2 ** 70])
+def test_a_window_past_the_context_is_no_window(window, path):
+    g = gen(2)
+    cache = epure.PagedKVCache(20, 16, 1, 64, BF16, DEV)
+    table = torch.randperm(20, generator=g, device=DEV).to(torch.int32)[None, :19]
+    x, pos = normal(g, 1, 300, 1, 64), torch.arange(300, device=DEV)[None]
+    cache.append(x, normal(g, 1, 300, 1, 64), pos, table)
+    q = normal(g, 1, 2, 4, 64)
+    assert torch.equal(cache.attend(q, pos[:, -2:], table, window=window), cache.attend(q, pos[:, -2:], table))
