@@ -73,3 +73,17 @@ def test_a_window_past_the_context_is_no_window(window, path):
     cache.append(x, normal(g, 1, 300, 1, 64), pos, table)
     q = normal(g, 1, 2, 4, 64)
     assert torch.equal(cache.attend(q, pos[:, -2:], table, window=window), cache.attend(q, pos[:, -2:], table))
+
+
+# ------------------------------------------------------------------ a call of one and of two
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("rot", [64, 40])
+def test_one_tensor_turns_as_two_do_past_the_tables_too(layout, rot, path):
+    g = gen(9)
+    r = epure.Rotary(rot, 20, layout=layout, device=DEV)
+    q, k = normal(g, 2, 6, 3, 64), normal(g, 2, 6, 1, 64)
+    pos = torch.tensor([[0, 19, 20, -1, 5, 1 << 40]], device=DEV).expand(2, 6)
+    for x, y in zip((q, k), r.rotate(q, k, pos)):
+        one = r(x, pos)
+        assert torch.equal(one.view(torch.int16), y.view(torch.int16))
+        assert torch.equal(one.isnan().all(-1).all(-1), pos >= 20) and torch.equal(one.isnan().any(-1).any(-1), pos >= 20)
