@@ -182,6 +182,7 @@ struct RotateOne : torch::autograd::Function<RotateOne> {
     }
 };
 
+// Two: the output of an input that needs no gradient is a constant.
 struct RotateTwo : torch::autograd::Function<RotateTwo> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &q,
                                                   const at::Tensor &k, const Turn &t)
@@ -190,6 +191,10 @@ struct RotateTwo : torch::autograd::Function<RotateTwo> {
         t.save(ctx);
         at::Tensor qo, ko;
         turned(turn(q, k, t, qo, ko));
+        if (!q.requires_grad())
+            ctx->mark_non_differentiable({qo});
+        if (!k.requires_grad())
+            ctx->mark_non_differentiable({ko});
         return {qo, ko};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,

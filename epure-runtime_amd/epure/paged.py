@@ -164,10 +164,20 @@ class _Rotate(torch.autograd.Function):
         if gq is None and gk is None:
             return None, None, None, None, None
         if gq is None:
-            gk, _ = _Rotate.apply(gk, None, positions, rot, inv)
+            gk, _ = _turned(gk, None, positions, rot, inv)
         else:
-            gq, gk = _Rotate.apply(gq, gk, positions, rot, inv)
+            gq, gk = _turned(gq, gk, positions, rot, inv)
         return gq, gk, None, None, None
+
+
+def _turned(q, k, positions, rotary, inverse):
+    """q and k (or None) turned, each as a function of its input if that needs a gradient, else as a constant."""
+    need = [torch.is_grad_enabled() and t is not None and t.requires_grad for t in (q, k)]
+    if not any(need):
+        return rotary._launch(q, k, positions, inverse)
+    if all(need) or k is None:
+        return _Rotate.apply(q, k, positions, rotary, inverse)
+    return tuple(_turned(t, None, positions, rotary, inverse)[0] for t in (q, k))
 
 
 class Rotary:
@@ -201,16 +211,15 @@ class Rotary:
 
     def rotate(self, q, k, positions):
         """q and k ([B, S, heads, D], one type) turned by their tokens'
-        positions (broadcast to [B, S]).  Differentiable in both."""
+        positions (broadcast to [B, S]).  Differentiable in both; the output
+        of one that needs no gradient needs none either."""
         call = _native()
         if call is not None:
             r = call.rotate(q, k, positions, self.cos, self.sin, self.layout == "interleaved")
             if r is not NotImplemented:
                 return r
         self._check(q, k, positions)
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-            return _Rotate.apply(q, k, positions, self, False)
-        return self._launch(q, k, positions, False)
+        return _turned(q, k, positions, self, False)
 
     def __call__(self, x, positions):
         """One tensor [B, S, heads, D] turned."""
@@ -220,9 +229,7 @@ class Rotary:
             if r is not NotImplemented:
                 return r
         self._check(x, None, positions)
-        if torch.is_grad_enabled() and x.requires_grad:
-            return _Rotate.apply(x, None, positions, self, False)[0]
-        return self._launch(x, None, positions, False)[0]
+        return _turned(x, None, positions, self, False)[0]
 
     def _check(self, q, k, positions):
         _require(q, positions, self.cos, *(() if k is None else (k,)))

@@ -75,6 +75,30 @@ def test_a_window_past_the_context_is_no_window(window, path):
     assert torch.equal(cache.attend(q, pos[:, -2:], table, window=window), cache.attend(q, pos[:, -2:], table))
 
 
+# ------------------------------------------------------------------ gradients of one of two
+@pytest.mark.parametrize("which", [0, 1])
+def test_only_what_wants_a_gradient_gets_one(which, path):
+    """rotate(q, k) with one of them a leaf: the other's output is a constant,
+    and the cache takes it."""
+    g = gen(6)
+    r = epure.Rotary(64, 30, device=DEV)
+    xs = [normal(g, 1, 5, h, 64) for h in (4, 2)]
+    ups = [normal(g, 1, 5, h, 64) for h in (4, 2)]
+    xs[which].requires_grad_()
+    pos = torch.arange(5, device=DEV)[None]
+    y = r.rotate(*xs, pos)
+    assert y[which].requires_grad and not y[1 - which].requires_grad
+    (got,) = torch.autograd.grad(y[which], xs[which], ups[which])
+    both = [x.detach().requires_grad_() for x in xs]
+    want = torch.autograd.grad(r.rotate(*both, pos), both, ups)[which]
+    assert torch.equal(got, want)
+    for a, b in zip(y, r.rotate(*(x.detach() for x in xs), pos)):
+        assert torch.equal(a, b)
+    if which == 0:
+        cache = epure.PagedKVCache(1, 16, 2, 64, BF16, DEV)
+        cache.append(y[1], ups[1], pos, torch.zeros(1, 1, dtype=torch.int32, device=DEV))
+
+
 # ------------------------------------------------------------------ a call of one and of two
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("rot", [64, 40])
