@@ -19,13 +19,14 @@ decltype(&ep_kv_read) fn_read;
 decltype(&ep_paged_attention_workspace) fn_attend_ws;
 decltype(&ep_paged_attention) fn_attend;
 
-// A plain GPU tensor argument on `dev` (any where dev < 0), or nullptr.
+// A plain GPU tensor argument on `dev` (any where dev < 0), or nullptr.  One
+// with a forward-mode tangent is not plain: nothing here would carry it on.
 const at::Tensor *gpu_tensor(PyObject *o, c10::DeviceIndex &dev)
 {
     if (!plain_tensor(o))
         return nullptr;
     const at::Tensor &t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || (dev >= 0 && t.get_device() != dev))
+    if (!t.is_cuda() || (dev >= 0 && t.get_device() != dev) || t._fw_grad(0).defined())
         return nullptr;
     dev = t.get_device();
     return &t;

@@ -20,6 +20,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .kernels import _abi
 from .kernels import cuda as cuda_kernel
@@ -38,6 +39,11 @@ def _require(*tensors):
 def _no_grad(*tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("the paged cache has no backward: call under torch.no_grad()")
+
+
+def _wants(t):
+    """(a gradient, a forward-mode tangent): what is to be derived through t."""
+    return torch.is_grad_enabled() and t.requires_grad, forward_ad.unpack_dual(t).tangent is not None
 
 
 def _native():
@@ -148,12 +154,14 @@ def rope_frequencies(dim, theta=10000.0, scaling=None):
 
 
 class _Rotate(torch.autograd.Function):
-    """q, k turned; the gradient of a turn is the turn the other way."""
+    """q, k turned; the gradient of a turn is the turn the other way, its
+    tangent the tangent turned."""
 
     @staticmethod
     def forward(ctx, q, k, positions, rotary, inverse):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
         ctx.rotary, ctx.inverse = rotary, inverse
         return rotary._launch(q, k, positions, inverse)
 
@@ -169,13 +177,18 @@ class _Rotate(torch.autograd.Function):
             gq, gk = _turned(gq, gk, positions, rot, inv)
         return gq, gk, None, None, None
 
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        return _turned(tq, tk, *ctx.saved_tensors, ctx.rotary, ctx.inverse)
+
 
 def _turned(q, k, positions, rotary, inverse):
-    """q and k (or None) turned, each as a function of its input if that needs a gradient, else as a constant."""
-    need = [torch.is_grad_enabled() and t is not None and t.requires_grad for t in (q, k)]
-    if not any(need):
+    """q and k (or None) turned, each as a function of its input if something
+    is to be derived through that, else as a constant."""
+    want = [_wants(t) for t in (q, k) if t is not None]
+    if not any(map(any, want)):
         return rotary._launch(q, k, positions, inverse)
-    if all(need) or k is None:
+    if want[0] == want[-1]:
         return _Rotate.apply(q, k, positions, rotary, inverse)
     return tuple(_turned(t, None, positions, rotary, inverse)[0] for t in (q, k))
 
@@ -211,8 +224,9 @@ class Rotary:
 
     def rotate(self, q, k, positions):
         """q and k ([B, S, heads, D], one type) turned by their tokens'
-        positions (broadcast to [B, S]).  Differentiable in both; the output
-        of one that needs no gradient needs none either."""
+        positions (broadcast to [B, S]).  Differentiable in both, in reverse
+        and in forward mode; the output of one that needs no gradient needs
+        none either."""
         call = _native()
         if call is not None:
             r = call.rotate(q, k, positions, self.cos, self.sin, self.layout == "interleaved")

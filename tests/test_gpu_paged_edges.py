@@ -75,6 +75,54 @@ def test_a_window_past_the_context_is_no_window(window, path):
     assert torch.equal(cache.attend(q, pos[:, -2:], table, window=window), cache.attend(q, pos[:, -2:], table))
 
 
+# ------------------------------------------------------------------ forward mode
+def test_forward_mode_tangents_turn_with_the_values(path):
+    """The turn is linear: its tangent is the tangent turned."""
+    g = gen(3)
+    r = epure.Rotary(48, 30, layout="interleaved", device=DEV)
+    q, k, tq, tk = (normal(g, 2, 5, h, 64, dtype=F32) for h in (6, 2, 6, 2))
+    pos = torch.tensor([[0, 5, 29, -1, 7]], device=DEV)
+    want, turned = r.rotate(q, k, pos), r.rotate(tq, tk, pos)
+    with forward_ad.dual_level():
+        dq, dk = forward_ad.make_dual(q, tq), forward_ad.make_dual(k, tk)
+        for a, b in ((dq, dk), (dq, k), (q, dk)):
+            out = [forward_ad.unpack_dual(t) for t in r.rotate(a, b, pos)]
+            for o, w, t, x, base in zip(out, want, turned, (a, b), (q, k)):
+                assert torch.equal(o.primal, w)
+                if x is base:
+                    assert o.tangent is None or not o.tangent.any()
+                else:
+                    assert torch.equal(o.tangent, t)
+        one = forward_ad.unpack_dual(r(dq, pos))
+        assert torch.equal(one.primal, want[0]) and torch.equal(one.tangent, turned[0])
+        with torch.no_grad():                       # which forward mode does not heed
+            assert torch.equal(forward_ad.unpack_dual(r(dq, pos)).tangent, turned[0])
+        # the tangent of a gradient: the upstream tangent turned back
+        x = q.clone().requires_grad_()
+        y = r(x, pos)
+        (gt,) = torch.autograd.grad(r(x, pos), x, tq)
+        try:
+            (gx,) = torch.autograd.grad(y, x, forward_ad.make_dual(q, tq))
+        except RuntimeError as e:                   # torch's C++ nodes have no forward mode, and say so
+            assert "jvp" in str(e)
+        else:
+            assert torch.equal(forward_ad.unpack_dual(gx).tangent, gt)
+
+
+def test_reverse_over_forward(path):
+    g = gen(4)
+    r = epure.Rotary(64, 30, device=DEV)
+    q, tq, up = (normal(g, 1, 5, 2, 64, dtype=F32) for _ in range(3))
+    pos = torch.arange(5, device=DEV)
+    tq.requires_grad_()
+    with forward_ad.dual_level():
+        t = forward_ad.unpack_dual(r(forward_ad.make_dual(q, tq), pos)).tangent
+        (got,) = torch.autograd.grad(t, tq, up)
+    x = q.clone().requires_grad_()
+    (want,) = torch.autograd.grad(r(x, pos), x, up)
+    assert torch.equal(got, want)
+
+
 # ------------------------------------------------------------------ gradients of one of two
 @pytest.mark.parametrize("which", [0, 1])
 def test_only_what_wants_a_gradient_gets_one(which, path):
