@@ -72,12 +72,22 @@ bool table_of(const at::Tensor &table, ep_tokens &t)
     return true;
 }
 
+bool needs_grad(std::initializer_list<const at::Tensor *> ts)
+{
+    if (!c10::GradMode::is_enabled())
+        return false;
+    for (const at::Tensor *t : ts)
+        if (t && t->requires_grad())
+            return true;
+    return false;
+}
+
 // The cache of arguments k, v, k_scale, v_scale (None in a 16-bit one).
 bool cache_of(PyObject *const *args, c10::DeviceIndex &dev, ep_kv_cache &c)
 {
     const at::Tensor *k = gpu_tensor(args[0], dev), *v = k ? gpu_tensor(args[1], dev) : nullptr;
     if (!v || k->dim() != 4 || v->sizes() != k->sizes() || v->scalar_type() != k->scalar_type() ||
-        !k->is_contiguous() || !v->is_contiguous())
+        !k->is_contiguous() || !v->is_contiguous() || needs_grad({k, v}))
         return false;
     const auto dt = k->scalar_type();
     const int code = dt == at::kChar ? EP_I8 : dt == at::kFloat8_e4m3fn ? EP_E4M3 : dtype_code(dt);
@@ -87,7 +97,8 @@ bool cache_of(PyObject *const *args, c10::DeviceIndex &dev, ep_kv_cache &c)
     if (code == EP_I8 || code == EP_E4M3)
         for (int i = 0; i < 2; ++i) {
             const at::Tensor *s = gpu_tensor(args[2 + i], dev);
-            if (!s || s->scalar_type() != at::kFloat || !s->is_contiguous() || s->sizes() != k->sizes().slice(0, 3))
+            if (!s || s->scalar_type() != at::kFloat || !s->is_contiguous() || s->sizes() != k->sizes().slice(0, 3) ||
+                needs_grad({s}))
                 return false;
             scale[i] = (float *)s->data_ptr();
         }
@@ -104,16 +115,6 @@ bool rotation_of(const at::Tensor *cos, const at::Tensor *sin, bool interleaved,
     r = ep_rotation{(const float *)cos->const_data_ptr(), (const float *)sin->const_data_ptr(), cos->size(0),
                     (int)(2 * cos->size(1)), interleaved};
     return true;
-}
-
-bool needs_grad(std::initializer_list<const at::Tensor *> ts)
-{
-    if (!c10::GradMode::is_enabled())
-        return false;
-    for (const at::Tensor *t : ts)
-        if (t && t->requires_grad())
-            return true;
-    return false;
 }
 
 at::Tensor like(const at::Tensor &t) { return at::empty(t.sizes(), t.options().requires_grad(false)); }

@@ -37,8 +37,12 @@ def _require(*tensors):
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the paged cache has no backward: call under torch.no_grad()")
+    for t in tensors:
+        gradient, tangent = (False, False) if t is None else _wants(t)
+        if gradient:
+            raise RuntimeError("the paged cache has no backward: call under torch.no_grad()")
+        if tangent:
+            raise RuntimeError("the paged cache has no derivative: call it on tensors without tangents")
 
 
 def _wants(t):
@@ -279,7 +283,8 @@ class PagedKVCache:
     float16, float8_e4m3fn or int8.  An 8-bit row (one head's values of one
     position) stands for code * scale, its scale in ``k_scale`` / ``v_scale``
     ``[n_pages, heads, page]`` (float32).  ``page`` is a power of two from 16
-    to 1024, D a multiple of 16 up to 256."""
+    to 1024, D a multiple of 16 up to 256.  Nothing is derived through a
+    cache: a call that would have to raises."""
 
     def __init__(self, n_pages, page, heads, dim, dtype=torch.bfloat16, device="cuda"):
         if dtype not in _abi.CACHE_DT:
@@ -323,6 +328,9 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.heads, self.page, self.dim, self.dtype = n, h, page, d, k.dtype
 
+    def _held(self):
+        return self.k, self.v, self.k_scale, self.v_scale
+
     def _cache(self):
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         return _abi.KVCache(self.k.data_ptr(), self.v.data_ptr(), ptr(self.k_scale), ptr(self.v_scale),
@@ -343,7 +351,7 @@ class PagedKVCache:
             r = call.append(k, v, positions, table, q, cos, sin, inter, self.k, self.v, self.k_scale, self.v_scale)
             if r is not NotImplemented:
                 return r
-        _no_grad(q, k, v)
+        _no_grad(q, k, v, *self._held())
         _require(self.k, k, v, positions, table, *(() if q is None else (q,)),
                  *(() if rotary is None else (rotary.cos,)))
         k, v = _heads4("k", k), _heads4("v", v)
@@ -375,6 +383,7 @@ class PagedKVCache:
             r = call.read(positions, table, dtype, self.k, self.v, self.k_scale, self.v_scale)
             if r is not NotImplemented:
                 return r
+        _no_grad(*self._held())
         _require(self.k, positions, table)
         if _abi.dtype_code(dtype) is None:
             raise TypeError(f"the cache is read as float32, float16 or bfloat16, not {dtype}")
@@ -400,7 +409,7 @@ class PagedKVCache:
             r = call.attend(q, positions, table, scale, window, self.k, self.v, self.k_scale, self.v_scale)
             if r is not NotImplemented:
                 return r
-        _no_grad(q)
+        _no_grad(q, *self._held())
         _require(self.k, q, positions, table)
         q = _heads4("q", q)
         if q.shape[3] != self.dim or q.shape[2] == 0 or q.shape[2] % self.heads:

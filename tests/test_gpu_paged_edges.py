@@ -123,6 +123,32 @@ def test_reverse_over_forward(path):
     assert torch.equal(got, want)
 
 
+# ------------------------------------------------------------------ cache derivatives
+def test_the_cache_refuses_what_it_has_no_derivative_for(path):
+    g = gen(5)
+    cache = epure.PagedKVCache(2, 16, 2, 64, BF16, DEV)
+    x, pos = normal(g, 1, 3, 2, 64), torch.arange(3, device=DEV)[None]
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    leaf = normal(g, 2, 2, 16, 64).requires_grad_()
+    held = epure.PagedKVCache.of(leaf, leaf.detach())
+    before = raw(cache)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, x)
+        dual = epure.PagedKVCache.of(leaf.detach(), forward_ad.make_dual(leaf.detach(), leaf.detach()))
+        calls = [lambda: cache.append(d, x, pos, table), lambda: cache.append(x, d, pos, table),
+                 lambda: cache.append(x, x, pos, table, q=d), lambda: cache.attend(d, pos, table),
+                 lambda: dual.attend(x, pos, table), lambda: dual.read(pos, table),
+                 lambda: held.attend(x, pos, table), lambda: held.read(pos, table)]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no backward|no derivative"):
+                call()
+    for a, b in zip(before, raw(cache)):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(held.read(pos, table)[0].float(),
+                           leaf.detach()[0, :, :3].transpose(0, 1)[None].float())
+
+
 # ------------------------------------------------------------------ gradients of one of two
 @pytest.mark.parametrize("which", [0, 1])
 def test_only_what_wants_a_gradient_gets_one(which, path):
