@@ -231,6 +231,8 @@ class Rotary:
         positions (broadcast to [B, S]).  Differentiable in both, in reverse
         and in forward mode; the output of one that needs no gradient needs
         none either."""
+        if k is None:
+            raise TypeError("rotate turns two tensors; call the rotation on one")
         call = _native()
         if call is not None:
             r = call.rotate(q, k, positions, self.cos, self.sin, self.layout == "interleaved")
@@ -250,6 +252,9 @@ class Rotary:
         return _turned(x, None, positions, self, False)[0]
 
     def _check(self, q, k, positions):
+        for t in (q, positions) if k is None else (q, k, positions):
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"expected tensors, got {type(t).__name__}")
         _require(q, positions, self.cos, *(() if k is None else (k,)))
         if q.dim() != 4 or q.shape[-1] < self.dim:
             raise ValueError(f"expected [B, S, heads, D] with D >= {self.dim}, got {tuple(q.shape)}")

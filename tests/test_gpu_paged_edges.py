@@ -173,6 +173,16 @@ def test_only_what_wants_a_gradient_gets_one(which, path):
         cache.append(y[1], ups[1], pos, torch.zeros(1, 1, dtype=torch.int32, device=DEV))
 
 
+# ------------------------------------------------------------------ two tensors
+def test_rotate_wants_two_tensors(path):
+    r = epure.Rotary(64, 30, device=DEV)
+    x, pos = normal(gen(7), 1, 5, 2, 64), torch.arange(5, device=DEV)
+    for q in (x, x.clone().requires_grad_()):
+        for a, b in ((q, None), (None, q)):
+            with pytest.raises(TypeError):
+                r.rotate(a, b, pos)
+
+
 # ------------------------------------------------------------------ a call of one and of two
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("rot", [64, 40])
