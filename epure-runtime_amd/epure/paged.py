@@ -275,9 +275,11 @@ class Rotary:
         if q.numel() == 0 and (k is None or k.numel() == 0):
             return qo, ko
         tok, _keep = _tokens(q.shape[:2], positions)
+        # a first tensor always has heads; k takes q's place where only it has
+        xh, xo, yh, yo = (_heads(q), qo, kh, ko) if q.shape[2] else (_heads(k), ko, None, None)
         _run("ep_rotate", _abi.lib.ep_rotate(
-            _heads(q), kh, self._rotation(), tok, q.shape[3], int(inverse), qo.data_ptr(),
-            ko.data_ptr() if ko is not None else None, _abi.stream_handle(q.device)))
+            xh, yh, self._rotation(), tok, q.shape[3], int(inverse), xo.data_ptr(),
+            yo.data_ptr() if yo is not None else None, _abi.stream_handle(q.device)))
         return qo, ko
 
 

@@ -183,6 +183,22 @@ def test_rotate_wants_two_tensors(path):
                 r.rotate(a, b, pos)
 
 
+# ------------------------------------------------------------------ no heads
+@pytest.mark.parametrize("heads", [(0, 2), (2, 0), (0, 0)])
+@pytest.mark.parametrize("grad", [False, True])
+def test_one_of_two_tensors_without_heads(heads, grad, path):
+    r = epure.Rotary(64, 30, device=DEV)
+    g = gen(8)
+    x = [normal(g, 1, 5, h, 64).requires_grad_(grad) for h in heads]
+    pos = torch.arange(5, device=DEV)
+    y = r.rotate(*x, pos)
+    for a, b in zip(x, y):
+        assert b.shape == a.shape and (a.shape[2] == 0 or torch.equal(b, r(a, pos)))
+    if grad:
+        for a, d in zip(x, torch.autograd.grad(y, x, [torch.ones_like(t) for t in y])):
+            assert d.shape == a.shape
+
+
 # ------------------------------------------------------------------ a call of one and of two
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("rot", [64, 40])
