@@ -547,7 +547,12 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
                 float w[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    w[e] = __builtin_amdgcn_exp2f(x[mt][e] - (base - VOP::kShift));
+                    // The shift goes on the difference: on a score past 2^24 it would be
+                    // rounded, and the largest weight could pass f16's largest number.
+                    w[e] = x[mt][e] - base;
+                    if constexpr (VOP::kShift != 0.0f)
+                        w[e] += VOP::kShift;
+                    w[e] = __builtin_amdgcn_exp2f(w[e]);
                     l[mt] += w[e];
                     if constexpr (k8)
                         w[e] = edge && !(seen[mt] >> e & 1) ? 0.0f : w[e] * vs[e];

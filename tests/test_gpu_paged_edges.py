@@ -211,3 +211,26 @@ def test_one_tensor_turns_as_two_do_past_the_tables_too(layout, rot, path):
         one = r(x, pos)
         assert torch.equal(one.view(torch.int16), y.view(torch.int16))
         assert torch.equal(one.isnan().all(-1).all(-1), pos >= 20) and torch.equal(one.isnan().any(-1).any(-1), pos >= 20)
+
+
+# ------------------------------------------------------------------ huge scores
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("length", [1, 33, 2000])
+def test_huge_f16_scores_keep_their_weights(length, sign):
+    """Equal scores of up to 2^28 either way: each position weighs 1 /
+    length, whatever the score's last bits are.  Keys of one sequence are
+    equal, so its scores are, bit for bit."""
+    g = gen(10)
+    B, D = 3, 64
+    pages = -(-length // 16)
+    cache = epure.PagedKVCache(B * pages, 16, 1, D, F16, DEV)
+    table = torch.randperm(B * pages, generator=g, device=DEV).to(torch.int32).view(B, pages)
+    pos = torch.arange(length, device=DEV).expand(B, -1)
+    k = torch.randint(1000, 3000, (B, 1, 1, D), generator=g, device=DEV).to(F16).expand(B, length, 1, D)
+    v = normal(g, B, length, 1, D, dtype=F16)
+    cache.append(k, v, pos, table)
+    q = torch.randint(20, 8000, (B, 1, 16, 1), generator=g, device=DEV).to(F16).expand(B, 1, 16, D).contiguous()
+    out = cache.attend(q, pos[:, -1:], table, scale=sign * 0.125).cpu().double()
+    want = v.cpu().double().mean(1, keepdim=True).expand(B, 1, 16, D)
+    mag = v.cpu().double().abs().mean(1, keepdim=True).expand(B, 1, 16, D)
+    assert ((out - want).abs() <= op.attend_tolerance(want, mag, 0.0, F16, D)).all()
