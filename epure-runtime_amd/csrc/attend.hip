@@ -19,7 +19,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int RM)
     __shared__ float s_m[64], s_l[64];
     __shared__ f32x4_t s_y[256];
     const uint32_t Hq = a.c.heads * a.G, D = a.c.D, tid = threadIdx.x;
-    const uint32_t token = blockIdx.x / Hq, head = blockIdx.x - token * Hq, h = head / a.G, gq = head - h * a.G;
+    const uint32_t out_row = a.first_wg + blockIdx.x, token = out_row / Hq, head = out_row - token * Hq, h = head / a.G, gq = head - h * a.G;
     const uint32_t b = token / (uint32_t)a.tok.S, s = token - b * (uint32_t)a.tok.S;
     const uint32_t row = s * a.G + gq, block = row / RM, r = row - block * RM;
     const int2 d = a.desc[(b * a.blocks + block) * a.c.heads + h];
@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int RM)
     uint2 w;
     w.x = OP::pack(y[0], y[1]);
     w.y = OP::pack(y[2], y[3]);
-    *(uint2 *)((char *)a.out + 2 * ((int64_t)blockIdx.x * D + c)) = w;
+    *(uint2 *)((char *)a.out + 2 * ((int64_t)out_row * D + c)) = w;
 }
 
 struct Plan {
@@ -133,6 +133,19 @@ Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_
     return p;
 }
 
+// A launch has fewer than 2^32 threads: a grid beyond that is cut into several.
+template <typename F>
+int in_launches(int64_t grid, unsigned threads, AttendArgs a, F launch)
+{
+    const int64_t most = 0xffffffff / threads;
+    for (int64_t at = 0; at < grid; at += most) {
+        a.first_wg = (uint32_t)at;
+        launch(a, (unsigned)std::min(grid - at, most));
+        EP_HIP_CHECK(hipGetLastError());
+    }
+    return EP_OK;
+}
+
 }  // namespace
 
 size_t attend_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCache &c)
@@ -182,28 +195,30 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
     a.desc = (int2 *)ws;
     a.part_ml = (float2 *)((char *)ws + p.desc);
     a.part_o = (float *)((char *)ws + p.desc + p.ml);
-    const unsigned grid = p.workers ? (unsigned)p.workers : (unsigned)p.segments;
-    if (c.dtype == EP_BF16)
-        attend_bf16(a, p.mt, grid, stream);
-    else if (c.dtype == EP_F16)
-        attend_f16(a, p.mt, grid, stream);
-    else if (c.dtype == EP_I8)
-        attend_i8(a, q->dtype, p.mt, grid, stream);
-    else
-        attend_e4m3(a, q->dtype, p.mt, grid, stream);
-    EP_HIP_CHECK(hipGetLastError());
-    if (p.workers) {
+    const int64_t grid = p.workers ? p.workers : p.segments;
+    int rc = in_launches(grid, 64 * kAttWaves, a, [&](const AttendArgs &part, unsigned n) {
+        if (c.dtype == EP_BF16)
+            attend_bf16(part, p.mt, n, stream);
+        else if (c.dtype == EP_F16)
+            attend_f16(part, p.mt, n, stream);
+        else if (c.dtype == EP_I8)
+            attend_i8(part, q->dtype, p.mt, n, stream);
+        else
+            attend_e4m3(part, q->dtype, p.mt, n, stream);
+    });
+    if (rc == EP_OK && p.workers) {
         // Four groups of lanes where segments are in a few pieces (128 rows x 32
         // heads: 2 us less than eight), eight where one is in hundreds (33 us
         // for 131072 positions on one head, 46 with four).
         const unsigned threads = p.segments * 8 >= p.workers ? 128 : 256;
-        if (q->dtype == EP_BF16)
-            join_kernel<OpBf16><<<(unsigned)out_rows, threads, 0, stream>>>(a, (int)rm);
-        else
-            join_kernel<OpF16><<<(unsigned)out_rows, threads, 0, stream>>>(a, (int)rm);
-        EP_HIP_CHECK(hipGetLastError());
+        rc = in_launches(out_rows, threads, a, [&](const AttendArgs &part, unsigned n) {
+            if (q->dtype == EP_BF16)
+                join_kernel<OpBf16><<<n, threads, 0, stream>>>(part, (int)rm);
+            else
+                join_kernel<OpF16><<<n, threads, 0, stream>>>(part, (int)rm);
+        });
     }
-    return EP_OK;
+    return rc;
 }
 
 }  // namespace ep

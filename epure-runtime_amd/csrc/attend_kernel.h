@@ -64,6 +64,7 @@ struct AttendArgs {
     int G, rows;             // query heads a cache head; rows of a sequence on one cache head (S G)
     int blocks;              // units of a sequence
     uint32_t units;
+    uint32_t first_wg;       // of this launch, where a call takes more workgroups than one launch can have
     int workers;             // workgroups that share all tiles evenly; 0: one workgroup a segment
     int few;                 // shares of a large call, of more than 16 tiles each
     int piece;               // tiles' time that beginning and ending a piece takes
@@ -712,8 +713,9 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
     // itself, 64 units at a time; the host bounds all counts to 32 bits.
     const uint32_t units = a.units;
     auto at_lane = [](uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); };
-    uint32_t u = blockIdx.x / (uint32_t)H;
-    int h = (int)(blockIdx.x - u * H), t0 = -1, t1 = 0, slot = -1;
+    const uint32_t segment = a.first_wg + blockIdx.x;
+    uint32_t u = segment / (uint32_t)H;
+    int h = (int)(segment - u * H), t0 = -1, t1 = 0, slot = -1;
     uint32_t f = 0, begin = 0, stop = 1, per = 1, total = 0;
     uint32_t first = 0, cost = 0, upto = 0;        // of the lane's unit; of all units up to it in this block of 64
     uint32_t u0 = 0, before = 0;         // the block's first unit; tiles ahead of it

@@ -119,9 +119,9 @@ int ep_kv_read(const ep_tokens *tokens, const ep_kv_cache *cache, void *k_out, v
  * cache has q's type; a table of at most 2^30 positions.  Scores, softmax and
  * sums are f32, the weights enter their product with 16 bits or more.  NaN
  * and infinities of positions that a token does not attend to do not reach
- * it; an infinite value that it attends to gives an infinity or NaN.  Any
- * number of new tokens is served; more than 32 query rows (tokens times heads
- * a cache head) read the cache once per 32.
+ * it; an infinite value that it attends to gives an infinity or NaN.  Up to
+ * 2^31 - 1 query rows (tokens times query heads) are served, 2^30 - 1 of a
+ * sequence on one cache head; more than 32 of those read the cache once per 32.
  * Workspace: ep_paged_attention_workspace() bytes (0 if the shape is
  * declined, or none is needed), 16-byte aligned, read and written by this call
  * alone.
