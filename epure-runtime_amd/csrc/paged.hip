@@ -524,14 +524,15 @@ Turn turn_of(const ep_rotation *rot, int inverse)
 // More than half of what the L2 caches hold together: their inputs pass there too.
 bool streams(int64_t values, int dtype) { return values * (dtype == EP_F32 ? 4 : 2) > (int64_t)16 << 20; }
 
-// Rows of a call (counted in 32 bits) and its grid.
+// Rows of a call and its grid: a launch has fewer than 2^32 threads.
 int grid_of(const PagedTokens &tok, int heads, int lanes, uint32_t &rows, unsigned &grid)
 {
-    const int64_t n = tok.B * tok.S * heads, per = 256 / lanes;
-    if (n > 0xffffff00)
-        return set_error(EP_DECLINE_SHAPE, "%lld rows are more than one launch takes", (long long)n);
+    const int64_t n = tok.B * tok.S * heads, per = 256 / lanes, groups = (n + per - 1) / per;
+    if (groups > 0xffffff)
+        return set_error(EP_DECLINE_SHAPE, "%lld rows on %d lanes each are more than one launch takes", (long long)n,
+                         lanes);
     rows = (uint32_t)n;
-    grid = (unsigned)((n + per - 1) / per);
+    grid = (unsigned)groups;
     return EP_OK;
 }
 

@@ -20,6 +20,10 @@
  *     width), or one whose page id lies outside [0, n_pages), stores
  *     nothing, and the output rows that need it are NaN.
  * No access leaves the buffers described, whatever they hold.
+ *
+ * A call of ep_rotate, ep_kv_append or ep_kv_read takes fewer than 2^32 lanes:
+ * its rows (tokens times heads, of q, k and v together) times D / 16 rounded
+ * up to a power of two.  One of more is declined.
  */
 #ifndef EPURE_PAGED_H
 #define EPURE_PAGED_H
