@@ -142,7 +142,8 @@ EP_DEV void turn_pair(float a, float b, float c, float s, float &ta, float &tb)
 
 // The 16 values of lane u of the row at x.  VEC: chunks are loaded whole (D
 // and, with a turn, dim / 2 in whole chunks, everything 16-byte aligned); else
-// value by value.  load() needs no position and goes ahead of what waits for
+// value by value (16384 tokens of 40 heads of 80 values: 254 us with 40 of them
+// turned, 57 with all).  load() needs no position and goes ahead of what waits for
 // one; values() then turns by position p (in the tables) where `turned`.
 template <typename T, bool VEC>
 struct LaneRow {
