@@ -105,10 +105,11 @@ _SCALING_KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "fa
                  "attention_factor", "mscale", "mscale_all_dim", "truncate"}
 
 
-def rope_frequencies(dim, theta=10000.0, scaling=None):
+def rope_frequencies(dim, theta=None, scaling=None):
     """Angle per position of the dim / 2 pairs (float64) and the attention factor.
 
-    ``scaling`` follows the models' configuration: a dict whose ``rope_type``
+    ``theta`` defaults to the scaling's ``rope_theta``, or 10000; both given
+    have to agree.  ``scaling`` follows the models' configuration: a dict whose ``rope_type``
     is "default", "linear" (``factor``), "llama3" (``factor``,
     ``low_freq_factor``, ``high_freq_factor``,
     ``original_max_position_embeddings``: frequencies of fewer turns within
@@ -125,6 +126,11 @@ def rope_frequencies(dim, theta=10000.0, scaling=None):
         unknown = sorted(k for k, v in scaling.items() if v is not None and k not in _SCALING_KEYS)
         if unknown:
             raise ValueError(f"rope scaling: {', '.join(map(str, unknown))} not served")
+        own = scaling.get("rope_theta")
+        if own is not None and theta is not None and float(own) != float(theta):
+            raise ValueError(f"theta {theta} given, rope_theta {own} in the scaling")
+        theta = own if theta is None else theta
+    theta = 10000.0 if theta is None else theta
     f = float(theta) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
     kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
     if kind == "default":
@@ -206,7 +212,7 @@ class Rotary:
     float64 for positions below ``max_pos`` and kept as float32 tables (the
     attention factor multiplied in)."""
 
-    def __init__(self, dim, max_pos, theta=10000.0, layout="half", scaling=None, device="cuda"):
+    def __init__(self, dim, max_pos, theta=None, layout="half", scaling=None, device="cuda"):
         if dim < 2 or dim % 2:
             raise ValueError(f"the rotated dim must be even and positive, got {dim}")
         if max_pos < 1:

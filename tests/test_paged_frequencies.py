@@ -73,3 +73,18 @@ def test_keys_that_a_scaling_does_not_use_are_none_of_its_business():
         a, b = (epure.rope_frequencies(64, 1e4, {**base, **more}) for more in
                 ({}, {"original_max_position_embeddings": 4096, "partial_rotary_factor": 0.5, "mscale": 1.0}))
         assert torch.equal(a[0], b[0]) and a[1] == b[1] == 1.0
+
+
+@pytest.mark.parametrize("base", [YARN, LLAMA3, LINEAR, {"rope_type": "default"}])
+def test_theta_in_the_scaling(base):
+    """Newer configurations keep rope_theta beside the scaling: taken if no
+    other is given, refused if another is."""
+    want = epure.rope_frequencies(64, 5e5, base)
+    for got in (epure.rope_frequencies(64, scaling={**base, "rope_theta": 5e5}),
+                epure.rope_frequencies(64, 5e5, {**base, "rope_theta": 500000})):
+        assert torch.equal(got[0], want[0]) and got[1] == want[1]
+    with pytest.raises(ValueError, match="theta"):
+        epure.rope_frequencies(64, 1e4, {**base, "rope_theta": 5e5})
+    assert torch.equal(epure.rope_frequencies(64)[0], epure.rope_frequencies(64, 1e4)[0])
+    r = epure.Rotary(64, 20, scaling={**base, "rope_theta": 5e5}, device="cpu")
+    assert torch.equal(r.cos, epure.Rotary(64, 20, 5e5, scaling=base, device="cpu").cos)
