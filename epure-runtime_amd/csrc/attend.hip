@@ -10,22 +10,16 @@
 namespace ep {
 namespace {
 
-// Joins the pieces of a segment that several workers took, one query row a
-// workgroup: D / 4 lanes take a piece, the next ones the next, each with its
-// own running maximum, so that sums, maxima and outputs load together.
-template <typename OP>
-__global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int RM)
+// Joins `n` pieces of one output row a workgroup, piece k of it at row at(k)
+// of the parts: D / 4 lanes take a piece, the next ones the next, each with its
+// own running maximum, so that sums, maxima and outputs load together.  p: the
+// row's position; none: what a row without any weight gives.
+template <typename OP, typename AT>
+EP_DEV void join_row(const AttendArgs &a, int64_t out_row, int p, int n, AT at, float none)
 {
     __shared__ float s_m[64], s_l[64];
     __shared__ f32x4_t s_y[256];
-    const uint32_t Hq = a.c.heads * a.G, D = a.c.D, tid = threadIdx.x;
-    const uint32_t out_row = a.first_wg + blockIdx.x, token = out_row / Hq, head = out_row - token * Hq, h = head / a.G, gq = head - h * a.G;
-    const uint32_t b = token / (uint32_t)a.tok.S, s = token - b * (uint32_t)a.tok.S;
-    const uint32_t row = s * a.G + gq, block = row / RM, r = row - block * RM;
-    const int2 d = a.desc[(b * a.blocks + block) * a.c.heads + h];
-    const int p = attend_position(a, b, s);
-    if (d.y <= 1)       // one worker wrote the output
-        return;
+    const uint32_t D = a.c.D, tid = threadIdx.x;
     const uint32_t quads = D / 4, groups = blockDim.x / quads, grp = tid / quads, c = 4 * (tid - grp * quads);
     float m = -INFINITY, l = 0.0f;
     f32x4_t y = {0, 0, 0, 0};
@@ -39,20 +33,18 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int RM)
             y[i] = y[i] * f + y2[i] * f2;
     };
     if (grp < groups)
-        for (int k0 = grp; k0 < d.y; k0 += 4 * groups) {
+        for (int k0 = grp; k0 < n; k0 += 4 * groups) {
             float2 ml[4];
             f32x4_t v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                // piece 0 is in slot d.x, piece k in the first slot of its worker; past the end the last again
-                const int k = min(k0 + i * (int)groups, d.y - 1);
-                const int64_t at = (int64_t)(k == 0 ? d.x : (d.x & ~1) + 2 * k) * a.slot_rows + r;
-                ml[i] = a.part_ml[at];
-                v[i] = *(const f32x4_t *)(a.part_o + at * D + c);
+                const int64_t row = at(min(k0 + i * (int)groups, n - 1));      // past the end the last again
+                ml[i] = a.part_ml[row];
+                v[i] = *(const f32x4_t *)(a.part_o + row * D + c);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (k0 + i * (int)groups < d.y)
+                if (k0 + i * (int)groups < n)
                     add(ml[i].x, ml[i].y, v[i]);
         }
     s_y[tid] = y;
@@ -63,16 +55,70 @@ __global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int RM)
     __syncthreads();
     if (grp != 0)
         return;
-    for (uint32_t k = 1; k < groups && (int)k < d.y; ++k)
+    for (uint32_t k = 1; k < groups && (int)k < n; ++k)
         add(s_m[k], s_l[k], s_y[k * quads + tid]);
     const float inv = 1.0f / l;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        y[i] = p < 0 ? 0.0f : p >= a.cap || l == 0.0f ? __uint_as_float(0x7fc00000u) : y[i] * inv;
+        y[i] = p < 0 ? 0.0f : p >= a.cap ? __uint_as_float(0x7fc00000u) : l == 0.0f ? none : y[i] * inv;
     uint2 w;
     w.x = OP::pack(y[0], y[1]);
     w.y = OP::pack(y[2], y[3]);
-    *(uint2 *)((char *)a.out + 2 * ((int64_t)out_row * D + c)) = w;
+    *(uint2 *)((char *)a.out + 2 * (out_row * D + c)) = w;
+}
+
+// An output row: its token (b, s), cache head and place in the group.
+struct OutRow {
+    uint32_t row, token, b, s, h, gq;
+};
+EP_DEV OutRow out_row_of(const AttendArgs &a)
+{
+    const uint32_t Hq = a.c.heads * a.G, row = a.first_wg + blockIdx.x, token = row / Hq, head = row - token * Hq, h = head / a.G;
+    const uint32_t b = token / (uint32_t)a.tok.S;
+    return {row, token, b, token - b * (uint32_t)a.tok.S, h, head - h * a.G};
+}
+
+// Piece k of a segment that several workers took: piece 0 in slot d.x, piece k
+// in the first slot of its worker.
+EP_DEV int64_t piece_slot(int2 d, int k) { return k == 0 ? d.x : (d.x & ~1) + 2 * k; }
+
+template <typename OP>
+__global__ void __launch_bounds__(256) join_kernel(AttendArgs a, int RM)
+{
+    const OutRow o = out_row_of(a);
+    const uint32_t row = o.s * a.G + o.gq, block = row / RM, r = row - block * RM;
+    const int2 d = a.desc[(o.b * a.blocks + block) * a.c.heads + o.h];
+    const int p = attend_position(a, o.b, o.s);
+    if (d.y <= 1)       // one worker wrote the output
+        return;
+    join_row<OP>(a, o.row, p, d.y, [&](int k) { return piece_slot(d, k) * a.slot_rows + r; }, __uint_as_float(0x7fc00000u));
+}
+
+// The pieces over a sequence's own pages, then those over the shared ones.
+template <typename OP>
+__global__ void __launch_bounds__(256) join_parts_kernel(AttendParts a, int RM)
+{
+    const OutRow o = out_row_of(a);
+    const uint32_t H = a.c.heads;
+    const uint32_t row = o.s * a.G + o.gq, block = row / RM, r = row - block * RM;
+    const uint32_t all = o.token * a.G + o.gq, front = all / RM, rf = all - front * RM;
+    const uint32_t seg = (a.front + o.b * a.blocks + block) * H + o.h, seg_f = front * H + o.h;
+    const int2 d = a.workers ? a.desc[seg] : make_int2((int)seg, 1);
+    const int2 f = a.workers ? a.desc[seg_f] : make_int2((int)seg_f, 1);
+    const int p = attend_position(a, o.b, o.s);
+    join_row<OP>(a, o.row, p, d.y + f.y, [&](int k) {
+        return (k < d.y ? piece_slot(d, k) : piece_slot(f, k - d.y)) * a.slot_rows + (k < d.y ? r : rf);
+    }, __uint_as_float(0x7fc00000u));
+}
+
+template <typename OP>
+__global__ void __launch_bounds__(256) join_blocks_kernel(AttendBlocks a)
+{
+    const OutRow o = out_row_of(a);
+    const uint32_t block = o.gq / 16, r = o.gq - 16 * block;
+    const int64_t seg = ((int64_t)o.token * a.blocks + block) * a.c.heads + o.h;
+    const int p = attend_position(a, o.b, o.s);
+    join_row<OP>(a, o.row, p, a.cuts, [&](int k) { return (seg * a.cuts + k) * a.slot_rows + r; }, 0.0f);
 }
 
 struct Plan {
@@ -134,8 +180,8 @@ Plan plan(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_
 }
 
 // A launch has fewer than 2^32 threads: a grid beyond that is cut into several.
-template <typename F>
-int in_launches(int64_t grid, unsigned threads, AttendArgs a, F launch)
+template <typename ARGS, typename F>
+int in_launches(int64_t grid, unsigned threads, ARGS a, F launch)
 {
     const int64_t most = 0xffffffff / threads;
     for (int64_t at = 0; at < grid; at += most) {
@@ -146,28 +192,16 @@ int in_launches(int64_t grid, unsigned threads, AttendArgs a, F launch)
     return EP_OK;
 }
 
-}  // namespace
+// Four groups of lanes where segments are in a few pieces (128 rows x 32
+// heads: 2 us less than eight), eight where one is in hundreds (33 us for
+// 131072 positions on one head, 46 with four).
+unsigned join_threads(int64_t segments, int workers) { return segments * 8 >= workers ? 128 : 256; }
 
-size_t attend_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCache &c)
+// What every call's kernels are given.
+void fill(AttendArgs &a, const ep_heads *q, const PagedTokens &tok, const PagedCache &c, float scale, int64_t window,
+          void *out)
 {
-    if (tok.B == 0 || tok.S == 0)
-        return 0;
-    const Plan p = plan(q, tok, c, 0);
-    return p.desc + p.ml + p.o;
-}
-
-int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, float scale, int64_t window,
-                  void *out, void *ws, size_t ws_bytes, hipStream_t stream)
-{
-    const Plan p = plan(q, tok, c, window);
-    const int64_t cap = tok.width << c.page_shift, rows = tok.S * (q->heads / c.heads), rm = 16 * p.mt;   // cap: below 2^30
-    const int64_t out_rows = tok.B * tok.S * q->heads;
-    if (rows > 0x3fffffff || p.segments > 0x7fffffff || out_rows > 0x7fffffff)
-        return set_error(EP_DECLINE_SHAPE, "%lld query rows are more than one call takes", (long long)out_rows);
-    if (ws_bytes < p.desc + p.ml + p.o || (p.workers && !ws))
-        return set_error(EP_ERR_WORKSPACE, "attention: workspace of %zu bytes, %zu wanted", ws_bytes,
-                         p.desc + p.ml + p.o);
-    AttendArgs a{};
+    const int64_t cap = tok.width << c.page_shift;      // below 2^30
     a.q = q->ptr;
     a.q_sb = q->stride_b;
     a.q_ss = q->stride_s;
@@ -179,6 +213,123 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
     a.window = window > 0 && window < cap ? (int)window : (int)cap;
     a.out = out;
     a.G = q->heads / c.heads;
+}
+
+// The workspace's parts: descriptors, maxima and sums, outputs.
+template <typename PLAN>
+int give(AttendArgs &a, const PLAN &p, void *ws, size_t ws_bytes)
+{
+    if (ws_bytes < p.desc + p.ml + p.o || (p.desc + p.ml + p.o && !ws))
+        return set_error(EP_ERR_WORKSPACE, "attention: workspace of %zu bytes, %zu wanted", ws_bytes,
+                         p.desc + p.ml + p.o);
+    a.desc = (int2 *)ws;
+    a.part_ml = (float2 *)((char *)ws + p.desc);
+    a.part_o = (float *)((char *)ws + p.desc + p.ml);
+    return EP_OK;
+}
+
+bool too_many_rows(int64_t rows, int64_t segments, int64_t out_rows)
+{
+    return rows > 0x3fffffff || segments > 0x7fffffff || out_rows > 0x7fffffff;
+}
+
+struct PartsPlan {
+    int mt, workers;
+    int64_t blocks, front, segments;
+    size_t desc, ml, o;
+    int slot_rows;
+};
+
+// Units of the whole batch over the shared pages, then the sequences' own:
+// as plan() does, but that every segment leaves a part.
+PartsPlan plan_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared, int64_t window)
+{
+    PartsPlan p{};
+    const int64_t rows = tok.S * (q->heads / c.heads), all = tok.B * rows;
+    p.mt = all <= 16 ? 1 : 2;
+    const int64_t rm = 16 * p.mt;
+    p.blocks = (rows + rm - 1) / rm;
+    p.front = (all + rm - 1) / rm;
+    p.segments = (p.front + tok.B * p.blocks) * c.heads;
+    p.slot_rows = (int)std::min(all, rm);
+    const int64_t tiles = (std::max(shared, tok.width - shared) << c.page_shift) / kAttTile + 1;
+    const int64_t most = window > 0 && window <= tiles * kAttTile
+                             ? std::min(tiles, (window + tok.S) / kAttTile + 2) : tiles;
+    if (most > std::min<int64_t>(16 + p.segments / 8, 32) && p.segments < 0x40000000 && tiles + kMostPiece < 0x7fff0000 / p.segments)
+        p.workers = 256 * attend_occupancy(attend_columns(c.D), p.mt, c.dtype != EP_I8);
+    const size_t slots = ((size_t)2 * p.workers + p.segments) * p.slot_rows;
+    p.desc = p.workers ? up16(p.segments * sizeof(int2)) : 0;
+    p.ml = up16(slots * sizeof(float2));
+    p.o = slots * c.D * sizeof(float);
+    return p;
+}
+
+struct BlocksPlan {
+    int64_t blocks, segments;
+    int cuts, slot_rows;
+    size_t desc, ml, o;
+};
+
+// A list's tiles are cut into as many pieces as fill the compute units twice,
+// of eight tiles at least (two a wave).
+BlocksPlan plan_blocks(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t take)
+{
+    BlocksPlan p{};
+    const int64_t G = q->heads / c.heads, tiles = (take * c.page + kAttTile - 1) / kAttTile;
+    p.blocks = (G + 15) / 16;
+    p.segments = tok.B * tok.S * p.blocks * c.heads;
+    p.cuts = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(p.segments, 1), tiles / (2 * kAttWaves)));
+    p.slot_rows = (int)std::min<int64_t>(G, 16);
+    if (p.cuts > 1) {
+        const size_t slots = (size_t)p.segments * p.cuts * p.slot_rows;
+        p.ml = up16(slots * sizeof(float2));
+        p.o = slots * c.D * sizeof(float);
+    }
+    return p;
+}
+
+// Sharing pays where there is more than one sequence to share.
+bool shares(const PagedTokens &tok, int64_t shared) { return tok.B > 1 && shared > 0; }
+
+}  // namespace
+
+size_t attend_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCache &c)
+{
+    if (tok.B == 0 || tok.S == 0)
+        return 0;
+    const Plan p = plan(q, tok, c, 0);
+    return p.desc + p.ml + p.o;
+}
+
+size_t attend_parts_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared)
+{
+    if (!shares(tok, shared) || tok.S == 0)
+        return attend_workspace(q, tok, c);
+    const PartsPlan p = plan_parts(q, tok, c, shared, 0);
+    return p.desc + p.ml + p.o;
+}
+
+size_t attend_blocks_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t take)
+{
+    if (tok.B == 0 || tok.S == 0 || take == 0)
+        return 0;
+    const BlocksPlan p = plan_blocks(q, tok, c, take);
+    return p.ml + p.o;
+}
+
+int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, float scale, int64_t window,
+                  void *out, void *ws, size_t ws_bytes, hipStream_t stream)
+{
+    const Plan p = plan(q, tok, c, window);
+    const int64_t rows = tok.S * (q->heads / c.heads), rm = 16 * p.mt;
+    const int64_t out_rows = tok.B * tok.S * q->heads;
+    if (too_many_rows(rows, p.segments, out_rows))
+        return set_error(EP_DECLINE_SHAPE, "%lld query rows are more than one call takes", (long long)out_rows);
+    AttendWhole a{};
+    int rc = give(a, p, ws, ws_bytes);
+    if (rc != EP_OK)
+        return rc;
+    fill(a, q, tok, c, scale, window, out);
     a.rows = (int)rows;
     a.blocks = (int)((rows + rm - 1) / rm);
     a.units = (uint32_t)(tok.B * a.blocks);
@@ -192,11 +343,8 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
     // caches hold a few such pools (16 x 2-4 thousand int8 positions: 28.7, 26.9).
     a.keys_once = a.blocks == 1 && c.n_pages * c.heads * c.page * row_bytes(c) > (int64_t)80 << 20;
     a.slot_rows = (int)(rows < rm ? rows : rm);
-    a.desc = (int2 *)ws;
-    a.part_ml = (float2 *)((char *)ws + p.desc);
-    a.part_o = (float *)((char *)ws + p.desc + p.ml);
     const int64_t grid = p.workers ? p.workers : p.segments;
-    int rc = in_launches(grid, 64 * kAttWaves, a, [&](const AttendArgs &part, unsigned n) {
+    rc = in_launches(grid, 64 * kAttWaves, a, [&](const AttendWhole &part, unsigned n) {
         if (c.dtype == EP_BF16)
             attend_bf16(part, p.mt, n, stream);
         else if (c.dtype == EP_F16)
@@ -207,17 +355,88 @@ int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c
             attend_e4m3(part, q->dtype, p.mt, n, stream);
     });
     if (rc == EP_OK && p.workers) {
-        // Four groups of lanes where segments are in a few pieces (128 rows x 32
-        // heads: 2 us less than eight), eight where one is in hundreds (33 us
-        // for 131072 positions on one head, 46 with four).
-        const unsigned threads = p.segments * 8 >= p.workers ? 128 : 256;
-        rc = in_launches(out_rows, threads, a, [&](const AttendArgs &part, unsigned n) {
+        const unsigned threads = join_threads(p.segments, p.workers);
+        rc = in_launches(out_rows, threads, a, [&](const AttendWhole &part, unsigned n) {
             if (q->dtype == EP_BF16)
                 join_kernel<OpBf16><<<n, threads, 0, stream>>>(part, (int)rm);
             else
                 join_kernel<OpF16><<<n, threads, 0, stream>>>(part, (int)rm);
         });
     }
+    return rc;
+}
+
+int launch_attend_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared, float scale,
+                        int64_t window, void *out, void *ws, size_t ws_bytes, hipStream_t stream)
+{
+    if (!shares(tok, shared))
+        return launch_attend(q, tok, c, scale, window, out, ws, ws_bytes, stream);
+    const PartsPlan p = plan_parts(q, tok, c, shared, window);
+    const int64_t rows = tok.S * (q->heads / c.heads), rm = 16 * p.mt;
+    const int64_t out_rows = tok.B * tok.S * q->heads;
+    if (too_many_rows(tok.B * rows, p.segments + 2 * p.workers, out_rows))
+        return set_error(EP_DECLINE_SHAPE, "%lld query rows are more than one call takes", (long long)out_rows);
+    AttendParts a{};
+    int rc = give(a, p, ws, ws_bytes);
+    if (rc != EP_OK)
+        return rc;
+    fill(a, q, tok, c, scale, window, out);
+    a.rows = (int)rows;
+    a.blocks = (int)p.blocks;
+    a.front = (int)p.front;
+    a.front_rows = (int)(tok.B * rows);
+    a.shared = (int)shared;
+    a.from = (int)(shared << c.page_shift);
+    a.units = (uint32_t)(p.front + tok.B * p.blocks);
+    a.workers = p.workers;
+    a.few = p.workers;
+    a.piece = piece_tiles(c, p.workers);
+    a.slot_rows = p.slot_rows;
+    const int64_t grid = p.workers ? p.workers : p.segments;
+    rc = in_launches(grid, 64 * kAttWaves, a, [&](const AttendParts &part, unsigned n) {
+        attend_parts(part, q->dtype, p.mt, n, stream);
+    });
+    if (rc == EP_OK) {
+        const unsigned threads = join_threads(p.segments, p.workers);
+        rc = in_launches(out_rows, threads, a, [&](const AttendParts &part, unsigned n) {
+            if (q->dtype == EP_BF16)
+                join_parts_kernel<OpBf16><<<n, threads, 0, stream>>>(part, (int)rm);
+            else
+                join_parts_kernel<OpF16><<<n, threads, 0, stream>>>(part, (int)rm);
+        });
+    }
+    return rc;
+}
+
+int launch_attend_blocks(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, const int32_t *list,
+                         int64_t take, float scale, int64_t window, void *out, void *ws, size_t ws_bytes,
+                         hipStream_t stream)
+{
+    const BlocksPlan p = plan_blocks(q, tok, c, take);
+    const int64_t out_rows = tok.B * tok.S * q->heads;
+    if (take > (0x3fffffff >> c.page_shift) || p.segments * p.cuts > 0x7fffffff || out_rows > 0x7fffffff)
+        return set_error(EP_DECLINE_SHAPE, "%lld query rows over %lld pages each are more than one call takes",
+                         (long long)out_rows, (long long)take);
+    AttendBlocks a{};
+    int rc = give(a, p, ws, ws_bytes);
+    if (rc != EP_OK)
+        return rc;
+    fill(a, q, tok, c, scale, window, out);
+    a.blocks = (int)p.blocks;
+    a.list = list;
+    a.take = (int)take;
+    a.cuts = p.cuts;
+    a.slot_rows = p.slot_rows;
+    rc = in_launches(p.segments * p.cuts, 64 * kAttWaves, a, [&](const AttendBlocks &part, unsigned n) {
+        attend_blocks(part, q->dtype, n, stream);
+    });
+    if (rc == EP_OK && p.cuts > 1)
+        rc = in_launches(out_rows, 128, a, [&](const AttendBlocks &part, unsigned n) {
+            if (q->dtype == EP_BF16)
+                join_blocks_kernel<OpBf16><<<n, 128, 0, stream>>>(part);
+            else
+                join_blocks_kernel<OpF16><<<n, 128, 0, stream>>>(part);
+        });
     return rc;
 }
 

@@ -3,7 +3,7 @@
 
 namespace ep {
 
-void attend_i8(const AttendArgs &a, int q_dtype, int mt, unsigned grid, hipStream_t st)
+void attend_i8(const AttendWhole &a, int q_dtype, int mt, unsigned grid, hipStream_t st)
 {
     if (q_dtype == EP_BF16)
         attend_by_rows<OpBf16, EP_I8>(a, mt, grid, st);

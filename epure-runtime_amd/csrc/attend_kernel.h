@@ -75,6 +75,31 @@ struct AttendArgs {
     float *part_o;           // [2 workers][slot_rows][D]
 };
 
+// What a call's units, rows and positions are:
+//   kWhole: a unit is up to 16 MT rows of one sequence, which see its pages
+//     from position 0 on (the pieces' outputs join where there are several);
+//   kParts: the tables' first `shared` pages are those of sequence 0.  The
+//     first `front` units are rows of the whole batch, over those pages; the
+//     rest is as in kWhole, over the pages behind them, positions counted
+//     from there.  Every output stays a part: the join adds them up;
+//   kBlocks: a unit is up to 16 rows of one token, and tile after tile goes
+//     over the `take` pages that a list names for it, in `cuts` equal pieces.
+enum AttendMode { kWhole, kParts, kBlocks };
+
+struct AttendWhole : AttendArgs {
+    static constexpr AttendMode kMode = kWhole;
+};
+struct AttendParts : AttendArgs {
+    static constexpr AttendMode kMode = kParts;
+    int front, front_rows;   // units over the shared pages; query rows of the batch on one cache head
+    int shared, from;        // pages, and positions in them
+};
+struct AttendBlocks : AttendArgs {
+    static constexpr AttendMode kMode = kBlocks;
+    const int32_t *list;     // [B][S][heads][take]
+    int take, cuts;
+};
+
 // v, computed anew where it is used: what follows from it is not kept in
 // registers across the loops.
 EP_DEV int opaque(int v)
@@ -102,26 +127,90 @@ EP_DEV int attend_position(const AttendArgs &a, int64_t b, int s)
 
 EP_DEV int first_seen(const AttendArgs &a, int p) { return p >= a.window ? p - a.window + 1 : 0; }
 
+// A unit: its first row and how many rows it counts among, the token of row 0,
+// the sequence whose table it reads, and the positions [from, limit) of it.
+struct AttendUnit {
+    int r0, rows;
+    int64_t b, t0;
+    int from, limit;
+};
+template <int RM, typename ARGS>
+EP_DEV AttendUnit attend_unit(const ARGS &a, uint32_t u)
+{
+    if constexpr (ARGS::kMode == kParts) {
+        if (u < (uint32_t)a.front)
+            return {(int)u * RM, a.front_rows, 0, 0, 0, a.from};
+        u -= a.front;
+    }
+    const uint32_t b = u / (uint32_t)a.blocks;
+    const int r0 = (int)(u - b * a.blocks) * RM;
+    if constexpr (ARGS::kMode == kBlocks)
+        return {r0, a.G, b / (uint32_t)a.tok.S, b, 0, a.cap};
+    else if constexpr (ARGS::kMode == kParts)
+        return {r0, a.rows, b, (int64_t)b * a.tok.S, a.from, a.cap - a.from};
+    else
+        return {r0, a.rows, b, 0, 0, a.cap};
+}
+
+// Token (b, s) of row `row` of a unit.
+struct AttendToken {
+    int64_t b;
+    int s, head;     // head: within the group
+};
+template <typename ARGS>
+EP_DEV AttendToken attend_token(const ARGS &a, const AttendUnit &u, int row)
+{
+    const int t = (uint32_t)row / (uint32_t)a.G, head = row - t * a.G;
+    if constexpr (ARGS::kMode == kWhole)
+        return {u.b, t, head};
+    else {
+        const uint32_t at = (uint32_t)(u.t0 + t), b = at / (uint32_t)a.tok.S;
+        return {b, (int)(at - b * (uint32_t)a.tok.S), head};
+    }
+}
+
+// What a row at position p sees of its unit's positions, counted from the
+// unit's first; false: nothing.
+template <typename ARGS>
+EP_DEV bool attend_span(const ARGS &a, const AttendUnit &u, int p, int &first, int &last)
+{
+    bool some = p >= 0 && p < a.cap;
+    first = first_seen(a, p);
+    last = p;
+    if constexpr (ARGS::kMode == kParts) {
+        first = max(first - u.from, 0);
+        last = min(p - u.from, u.limit - 1);
+        some = some && first <= last;
+    }
+    first = some ? first : a.cap;
+    last = some ? last : -1;
+    return some;
+}
+
 // Tiles that the rows of unit u reach (one at least: its outputs are written
 // with that tile), and the first of them.
-template <int RM>
-EP_DEV uint32_t unit_tiles(const AttendArgs &a, uint32_t u, uint32_t &first)
+template <int RM, typename ARGS>
+EP_DEV uint32_t unit_tiles(const ARGS &a, uint32_t u, uint32_t &first)
 {
-    const uint32_t b = u / (uint32_t)a.blocks;
-    const int r0 = (int)(u - b * a.blocks) * RM, r1 = min(r0 + RM, a.rows);
+    const AttendUnit unit = attend_unit<RM>(a, u);
+    const int r0 = unit.r0, r1 = min(r0 + RM, unit.rows);
     const int s0 = (uint32_t)r0 / (uint32_t)a.G, s1 = (uint32_t)(r1 - 1) / (uint32_t)a.G;
     int lo = a.cap, hi = -1;
     for (int s = s0; s <= s1; s += 4) {
         int p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)      // four loads in flight; the last token again past the end
-            p[i] = attend_position(a, b, min(s + i, s1));
+        for (int i = 0; i < 4; ++i) {    // four loads in flight; the last token again past the end
+            const AttendToken t = attend_token(a, unit, min(s + i, s1) * a.G);
+            p[i] = attend_position(a, t.b, t.s);
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (p[i] >= 0 && p[i] < a.cap) {
-                hi = max(hi, p[i]);
-                lo = min(lo, first_seen(a, p[i]));
+        for (int i = 0; i < 4; ++i) {
+            int f, l;
+            if (attend_span(a, unit, p[i], f, l)) {
+                hi = max(hi, l);
+                lo = min(lo, f);
             }
+        }
     }
     first = hi < 0 ? 0u : (uint32_t)(lo / kAttTile);
     return hi < 0 ? 1u : (uint32_t)(hi / kAttTile) - first + 1;
@@ -252,10 +341,11 @@ constexpr int attend_columns(int D) { return D <= 64 ? 4 : D <= 128 ? 8 : D <= 1
 
 // QOP: type of the queries; CODE: EP_I8, EP_E4M3, or QOP's type.  KS: steps of
 // 32 values of a head, CW: output columns a lane (16 CW >= D), MT: 16-row
-// tiles of query rows.
-template <typename QOP, int CODE, int KS, int CW, int MT, bool RAGGED>
-__global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGED && CODE != EP_I8)) attend_kernel(AttendArgs a)
+// tiles of query rows.  RAGGED: rows of a unit may differ in what they see.
+template <typename QOP, int CODE, int KS, int CW, int MT, bool RAGGED, typename ARGS>
+EP_DEV void attend_body(const ARGS &a)
 {
+    constexpr AttendMode MODE = ARGS::kMode;
     constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
     constexpr int ES = k8 ? 1 : 2, KL = k8 ? KS / 2 : KS, RM = 16 * MT, DP = 16 * CW, VW = CW * ES / 4;
     static_assert(!k8 || KS % 2 == 0, "8-bit keys are read in chunks of two steps");
@@ -288,34 +378,54 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
     // ---- one piece: tiles [t0, t1) of the positions; t0 < 0: all that the
     // unit's rows reach.  slot < 0: the outputs are written.
     auto piece = [&](uint32_t u, int h, int t0, int t1, int slot) {
-        const uint32_t ub = u / (uint32_t)a.blocks;
-        const int r0 = (int)(u - ub * a.blocks) * RM;
-        const int64_t b = ub;
+        const AttendUnit unit = attend_unit<RM>(a, u);
+        const int r0 = unit.r0;
         const int lx = opaque(lane), ln = lx & 15, lg = lx >> 4;
-        const int32_t *table = a.tok.table + b * a.tok.table_stride;
-        auto load_ids = [&](int j) {
-            const int64_t at = (int64_t)(j * kAttTile + 16 * (lane & 1)) >> a.c.page_shift;
-            return a.tok.width > 0 ? table[at < a.tok.width ? at : a.tok.width - 1] : -1;
+        const int32_t *table = a.tok.table + unit.b * a.tok.table_stride;
+        int64_t width = a.tok.width;     // pages of this unit's table
+        if constexpr (MODE == kParts)
+            if (unit.from) {
+                table += a.shared;
+                width -= a.shared;
+            }
+        // kBlocks: the page in the list that half (lane & 1) of tile j lies in, -1: none
+        auto load_block = [&](int j) {
+            if constexpr (MODE == kBlocks) {
+                const int32_t *list = a.list + (unit.t0 * H + h) * a.take;
+                const int at = (j * kAttTile + 16 * (lane & 1)) >> a.c.page_shift;
+                const int block = list[min(at, a.take - 1)];
+                return at < a.take && block >= 0 && block < width ? block : -1;
+            }
+            return 0;
+        };
+        auto load_ids = [&](int j, int block) {
+            const int64_t at = MODE == kBlocks ? block : (int64_t)(j * kAttTile + 16 * (lane & 1)) >> a.c.page_shift;
+            return width > 0 ? table[at < 0 ? 0 : at < width ? at : width - 1] : -1;
         };
         // Pages, positions and queries load together where the first tile is
         // known: a share's piece, or no window.
         const bool known = t0 >= 0 || a.window >= a.cap;
-        int j = max(t0, 0) + wave, ids = 0;
-        if (known)
-            ids = load_ids(j);
+        int j = max(t0, 0) + wave, ids = 0, block = 0;
+        if (known) {
+            block = load_block(j);
+            ids = load_ids(j, block);
+        }
         int pos[MT], first[MT], last[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const int row = r0 + 16 * mt + ln;
-            pos[mt] = row < a.rows ? attend_position(a, b, (uint32_t)row / (uint32_t)a.G) : -1;
+            pos[mt] = -1;
+            if (row < unit.rows) {
+                const AttendToken t = attend_token(a, unit, row);
+                pos[mt] = attend_position(a, t.b, t.s);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);       // loads return in order: the positions' wait must not cover the queries
         // (mt, k): values of step k of row n, zero past D
         auto query = [&](int mt, int k) {
-            const int row = min(r0 + 16 * mt + ln, a.rows - 1);
-            const int s = (uint32_t)row / (uint32_t)a.G, gq = row - s * a.G;
+            const AttendToken t = attend_token(a, unit, min(r0 + 16 * mt + ln, unit.rows - 1));
             const int d = k8 ? 64 * (k / 2) + 16 * lg + 8 * (k & 1) : 32 * k + 8 * lg;
-            const int64_t at = b * a.q_sb + s * a.q_ss + (int64_t)(h * a.G + gq) * a.q_sh + (d < D ? d : 0);
+            const int64_t at = t.b * a.q_sb + t.s * a.q_ss + (int64_t)(h * a.G + t.head) * a.q_sh + (d < D ? d : 0);
             return *(const u32x4_t *)((const char *)a.q + 2 * at);
         };
         auto in_head = [&](int k, u32x4_t w) {
@@ -337,13 +447,12 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const int p = pos[mt];
-            const bool some = p >= 0 && p < a.cap;
-            first[mt] = some ? first_seen(a, p) : a.cap;
-            last[mt] = some ? p : -1;
+            const bool some = attend_span(a, unit, p, first[mt], last[mt]);
             lo = max(lo, some ? -first[mt] : -a.cap);
             hi = max(hi, last[mt]);
-            in_lo = max(in_lo, some ? first[mt] : 0);
-            in_hi = max(in_hi, some ? -p : -a.cap);
+            // kParts: a row that sees nothing here masks every tile (a padded one may hold anything)
+            in_lo = max(in_lo, some ? first[mt] : MODE == kParts && p >= 0 ? a.cap : 0);
+            in_hi = max(in_hi, some ? -last[mt] : -a.cap);
             if (wave == 0 && lg == 0)
                 s_p[16 * mt + ln] = p;
         }
@@ -355,7 +464,8 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
         const int end = t0 >= 0 ? t1 : hi < 0 ? 1 : hi / kAttTile + 1;
         if (!known) {
             j = (hi < 0 ? 0 : lo / kAttTile) + wave;
-            ids = load_ids(j);
+            block = load_block(j);
+            ids = load_ids(j, block);
         }
 
         // ---- loads
@@ -364,12 +474,19 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
         float ks[8], vs[8];
         bool good[2];
         int64_t at[2];       // row of each half's first position
-        auto locate = [&](int ids, int j) {
+        int base[2];         // kBlocks: that position (a.cap: none)
+        auto locate = [&](int ids, int block, int j) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int64_t id = __builtin_amdgcn_readlane(ids, t);
+                const int row = (j * kAttTile + 16 * t) & (a.c.page - 1);
                 good[t] = j < end && id >= 0 && id < a.c.n_pages;
-                at[t] = (id * H + h) * a.c.page + ((j * kAttTile + 16 * t) & (a.c.page - 1));
+                at[t] = (id * H + h) * a.c.page + row;
+                if constexpr (MODE == kBlocks) {
+                    const int k = __builtin_amdgcn_readlane(block, t);
+                    good[t] = good[t] && k >= 0;
+                    base[t] = k < 0 ? a.cap : (k << a.c.page_shift) + row;
+                }
             }
         };
         auto load_scales = [&](const float *src, float *out) {
@@ -456,8 +573,10 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
             for (int t = 0; t < CW; ++t)
                 o[mt][t] = (f32x4_t){0, 0, 0, 0};
         }
-        locate(ids, j);
-        ids = load_ids(j + kAttWaves);
+        locate(ids, block, j);
+        block = load_block(j + kAttWaves);
+        ids = load_ids(j + kAttWaves, block);
+        int ahead = load_block(j + 2 * kAttWaves);      // kBlocks: its page id waits for it
         __builtin_amdgcn_sched_barrier(0);
         load_k();
         __builtin_amdgcn_sched_barrier(0);       // loads return in order: the keys' wait must not cover the values
@@ -475,8 +594,10 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
         for (; j < end; j += kAttWaves) {
             if constexpr (kQueriesInLds)
                 asm volatile("" ::: "memory");      // the queries are read again for each tile
-            const int j0 = j * kAttTile;
+            // positions of the tile's halves
+            const int j0 = MODE == kBlocks ? base[0] : j * kAttTile, j1 = MODE == kBlocks ? base[1] : j0 + 16;
             const bool bad0 = !good[0], bad1 = !good[1];
+            auto position = [&](int e) { return (e < 4 ? j0 : j1) + 4 * g + e % 4; };
             f32x4_t sc[MT][2];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
@@ -504,14 +625,16 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
                     x[mt][e] = sc[mt][e / 4][e % 4] * (k8 ? ks[e] * a.scale : a.scale);
             // the next tile's keys (none past the end: empty descriptors)
             __builtin_amdgcn_sched_barrier(0);
-            locate(ids, j + kAttWaves);
-            ids = load_ids(j + 2 * kAttWaves);
+            locate(ids, block, j + kAttWaves);
+            block = ahead;
+            ids = load_ids(j + 2 * kAttWaves, block);
+            ahead = load_block(j + 3 * kAttWaves);
             load_k();
             __builtin_amdgcn_sched_barrier(0);
 
             // A tile that some row sees in part (or that names a page the pool
             // lacks: its scores are NaN) masks its scores one by one.
-            const bool edge = j0 < in_lo || j0 + kAttTile - 1 > in_hi || bad0 || bad1;
+            const bool edge = min(j0, j1) < in_lo || max(j0, j1) + 15 > in_hi || bad0 || bad1;
             uint32_t seen[MT];
             if (edge) {
 #pragma unroll
@@ -519,7 +642,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
                     seen[mt] = 0;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const int p = j0 + 16 * (e / 4) + 4 * g + e % 4;
+                        const int p = position(e);
                         const bool in = p >= first[mt] && p <= last[mt];
                         seen[mt] |= (uint32_t)in << e;
                         x[mt][e] = !in ? -INFINITY : (e < 4 ? bad0 : bad1) ? nan : x[mt][e];
@@ -591,7 +714,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
             if (edge) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r) {
-                    const int p = j0 + 16 * (r / 4) + 4 * g + r % 4;
+                    const int p = position(r);
                     const uint32_t keep = p >= lo && p <= hi ? ~0u : 0u;
 #pragma unroll
                     for (int c = 0; c < VW; ++c)
@@ -646,7 +769,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
         // and what is read is weighed.  The barriers order LDS only, so that no
         // store to memory is waited for.
         const int ex = opaque(lane), en = ex & 15, eg = ex >> 4, tid = opaque(threadIdx.x);
-        const int rows = min(RM, a.rows - r0);
+        const int rows = min(RM, unit.rows - r0);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             if constexpr (kHitsApart)
@@ -688,25 +811,37 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
                 for (int i = 0; i < 4; ++i)
                     y[i] = fmaf(v[i], f, y[i]);
             }
-            if (slot >= 0) {
+            if (MODE == kParts || slot >= 0) {
                 const int64_t at = (int64_t)slot * a.slot_rows + r;
                 *(f32x4_t *)(a.part_o + at * D + d) = y;
                 if (d == 0)
                     a.part_ml[at] = make_float2(mx, sum);
                 continue;
             }
-            const int p = s_p[r], s = (uint32_t)(r0 + r) / (uint32_t)a.G, gq = r0 + r - s * a.G;
-            const float inv = 1.0f / sum;      // no weight at all (every score -inf) gives NaN
+            const AttendToken t = attend_token(a, unit, r0 + r);
+            const int p = s_p[r];
+            const float inv = 1.0f / sum;      // no weight at all (every score -inf) gives NaN; zeros where a list names no page
+            const float none = MODE == kBlocks ? 0.0f : nan;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                y[i] = p < 0 ? 0.0f : p >= a.cap || sum == 0.0f ? nan : y[i] * inv;
+                y[i] = p < 0 ? 0.0f : p >= a.cap ? nan : sum == 0.0f ? none : y[i] * inv;
             uint2 w;
             w.x = QOP::pack(y[0], y[1]);
             w.y = QOP::pack(y[2], y[3]);
-            *(uint2 *)((char *)a.out + 2 * (((b * a.tok.S + s) * H * a.G + h * a.G + gq) * D + d)) = w;
+            *(uint2 *)((char *)a.out + 2 * (((t.b * a.tok.S + t.s) * H * a.G + h * a.G + t.head) * D + d)) = w;
         }
         lds_barrier();
     };
+
+    // ---- a list's segment, cut into equal pieces
+    if constexpr (MODE == kBlocks) {
+        const uint32_t at = a.first_wg + blockIdx.x, seg = at / (uint32_t)a.cuts, cut = at - seg * a.cuts;
+        const int tiles = (int)(((int64_t)a.take * a.c.page + kAttTile - 1) / kAttTile);
+        const uint32_t u = seg / (uint32_t)H;
+        piece(u, (int)(seg - u * H), (int)((int64_t)tiles * cut / a.cuts), (int)((int64_t)tiles * (cut + 1) / a.cuts),
+              a.cuts > 1 ? (int)at : -1);
+        return;
+    }
 
     // ---- one segment a workgroup (workers == 0), or an even share of all tiles
     // in the order unit, cache head, tile.  Every wave counts the units' tiles by
@@ -715,7 +850,7 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
     auto at_lane = [](uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); };
     const uint32_t segment = a.first_wg + blockIdx.x;
     uint32_t u = segment / (uint32_t)H;
-    int h = (int)(segment - u * H), t0 = -1, t1 = 0, slot = -1;
+    int h = (int)(segment - u * H), t0 = -1, t1 = 0, slot = MODE == kParts ? (int)segment : -1;
     uint32_t f = 0, begin = 0, stop = 1, per = 1, total = 0;
     uint32_t first = 0, cost = 0, upto = 0;        // of the lane's unit; of all units up to it in this block of 64
     uint32_t u0 = 0, before = 0;         // the block's first unit; tiles ahead of it
@@ -774,22 +909,44 @@ __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGE
             const int base = (int)at_lane(first, i) - (int)head0;
             t0 = base + (int)f0;
             t1 = base + (int)f1;
+            // A piece that begins before its worker's share does is kept in the
+            // worker's first slot, else in its second; a whole segment that has
+            // to stay a part, in one of its own behind them.
+            const bool whole = f0 == head0 && f1 == next;
+            slot = 2 * (int)blockIdx.x + (head0 - a.piece >= begin);
+            if (MODE == kParts && whole)
+                slot = 2 * a.workers + (int)(u * H) + h;
             if (f0 == head0 && threadIdx.x == 0) {
                 const uint32_t w1 = min((next - 1) / per, (uint32_t)a.workers - 1);
-                a.desc[u * H + h] = make_int2(2 * (int)blockIdx.x + (head0 - a.piece >= begin), (int)(w1 - blockIdx.x + 1));
+                a.desc[u * H + h] = make_int2(slot, (int)(w1 - blockIdx.x + 1));
             }
-            // A piece that begins before its worker's share does is kept in the
-            // worker's first slot, else in its second.
-            slot = f0 == head0 && f1 == next ? -1 : 2 * (int)blockIdx.x + (head0 - a.piece >= begin);
+            if (MODE == kWhole && whole)
+                slot = -1;
         } else
             f = stop;
         piece(u, h, t0, t1, slot);
     }
 }
 
+template <typename QOP, int CODE, int KS, int CW, int MT, bool RAGGED>
+__global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGED && CODE != EP_I8)) attend_kernel(AttendWhole a)
+{
+    attend_body<QOP, CODE, KS, CW, MT, RAGGED>(a);
+}
+template <typename QOP, int CODE, int KS, int CW, int MT>
+__global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, CODE != EP_I8)) attend_parts_kernel(AttendParts a)
+{
+    attend_body<QOP, CODE, KS, CW, MT, true>(a);
+}
+template <typename QOP, int CODE, int KS, int CW>
+__global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, 1, false)) attend_blocks_kernel(AttendBlocks a)
+{
+    attend_body<QOP, CODE, KS, CW, 1, false>(a);
+}
+
 // Instantiations of one pair of types, by D and rows (attend_gen_*.hip).
 template <typename QOP, int CODE, int MT, bool RAGGED>
-void attend_by_size(const AttendArgs &a, unsigned grid, hipStream_t st)
+void attend_by_size(const AttendWhole &a, unsigned grid, hipStream_t st)
 {
     constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
     const int D = a.c.D;
@@ -808,7 +965,7 @@ void attend_by_size(const AttendArgs &a, unsigned grid, hipStream_t st)
 }
 
 template <typename QOP, int CODE>
-void attend_by_rows(const AttendArgs &a, int mt, unsigned grid, hipStream_t st)
+void attend_by_rows(const AttendWhole &a, int mt, unsigned grid, hipStream_t st)
 {
     if (mt == 1 && a.tok.S == 1)
         attend_by_size<QOP, CODE, 1, false>(a, grid, st);
@@ -818,9 +975,51 @@ void attend_by_rows(const AttendArgs &a, int mt, unsigned grid, hipStream_t st)
         attend_by_size<QOP, CODE, 2, true>(a, grid, st);
 }
 
-void attend_bf16(const AttendArgs &a, int mt, unsigned grid, hipStream_t st);
-void attend_f16(const AttendArgs &a, int mt, unsigned grid, hipStream_t st);
-void attend_i8(const AttendArgs &a, int q_dtype, int mt, unsigned grid, hipStream_t st);
-void attend_e4m3(const AttendArgs &a, int q_dtype, int mt, unsigned grid, hipStream_t st);
+template <typename QOP, int CODE, int KS, int CW>
+void attend_other(const AttendParts &a, int mt, unsigned grid, hipStream_t st)
+{
+    if (mt == 1)
+        attend_parts_kernel<QOP, CODE, KS, CW, 1><<<grid, 64 * kAttWaves, 0, st>>>(a);
+    else
+        attend_parts_kernel<QOP, CODE, KS, CW, 2><<<grid, 64 * kAttWaves, 0, st>>>(a);
+}
+template <typename QOP, int CODE, int KS, int CW>
+void attend_other(const AttendBlocks &a, int, unsigned grid, hipStream_t st)
+{
+    attend_blocks_kernel<QOP, CODE, KS, CW><<<grid, 64 * kAttWaves, 0, st>>>(a);
+}
+
+// The other kernels, by D (attend_gen_parts.hip, attend_gen_blocks.hip).
+template <typename QOP, int CODE, typename ARGS>
+void attend_other_by_size(const ARGS &a, int mt, unsigned grid, hipStream_t st)
+{
+    const int D = a.c.D;
+    if (D <= 64)
+        attend_other<QOP, CODE, 2, 4>(a, mt, grid, st);
+    else if (D <= 128)
+        attend_other<QOP, CODE, 4, 8>(a, mt, grid, st);
+    else if (D <= 192 && attend_columns(D) == 12)
+        attend_other<QOP, CODE, 6, 12>(a, mt, grid, st);
+    else if (D <= 192)
+        attend_other<QOP, CODE, 6, 16>(a, mt, grid, st);
+    else
+        attend_other<QOP, CODE, 8, 16>(a, mt, grid, st);
+}
+template <int CODE, typename ARGS>
+void attend_other_by_query(const ARGS &a, int q_dtype, int mt, unsigned grid, hipStream_t st)
+{
+    if (q_dtype == EP_BF16)
+        attend_other_by_size<OpBf16, CODE>(a, mt, grid, st);
+    else
+        attend_other_by_size<OpF16, CODE>(a, mt, grid, st);
+}
+
+void attend_bf16(const AttendWhole &a, int mt, unsigned grid, hipStream_t st);
+void attend_f16(const AttendWhole &a, int mt, unsigned grid, hipStream_t st);
+void attend_i8(const AttendWhole &a, int q_dtype, int mt, unsigned grid, hipStream_t st);
+void attend_e4m3(const AttendWhole &a, int q_dtype, int mt, unsigned grid, hipStream_t st);
+// ... and of the other kernels: types from the arguments
+void attend_parts(const AttendParts &a, int q_dtype, int mt, unsigned grid, hipStream_t st);
+void attend_blocks(const AttendBlocks &a, int q_dtype, unsigned grid, hipStream_t st);
 
 }  // namespace ep

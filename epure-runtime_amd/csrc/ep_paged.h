@@ -1,5 +1,5 @@
 // Descriptors and launchers of the paged-cache kernels (paged.hip,
-// attend.hip).  Not part of the public ABI.
+// attend.hip, select.hip).  Not part of the public ABI.
 #pragma once
 
 #include "ep_common.h"
@@ -48,5 +48,16 @@ int launch_kv_read(const PagedTokens &tok, const PagedCache &c, void *k_out, voi
 size_t attend_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCache &c);
 int launch_attend(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, float scale, int64_t window,
                   void *out, void *ws, size_t ws_bytes, hipStream_t stream);
+size_t attend_parts_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared);
+int launch_attend_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared, float scale,
+                        int64_t window, void *out, void *ws, size_t ws_bytes, hipStream_t stream);
+size_t attend_blocks_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t take);
+int launch_attend_blocks(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, const int32_t *list,
+                         int64_t take, float scale, int64_t window, void *out, void *ws, size_t ws_bytes,
+                         hipStream_t stream);
+int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, hipStream_t stream);
+size_t select_workspace(const PagedTokens &tok, const PagedCache &c, int64_t take);
+int launch_kv_select(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, const void *bounds, int64_t take,
+                     int32_t *blocks, void *ws, size_t ws_bytes, hipStream_t stream);
 
 }  // namespace ep

@@ -1,5 +1,5 @@
 // extern "C" entry points of include/epure_paged.h: every check that the
-// host can make, then the launch.  Kernels: paged.hip, attend.hip.
+// host can make, then the launch.  Kernels: paged.hip, attend.hip, select.hip.
 #include <hip/hip_runtime.h>
 
 #include "ep_internal.h"
@@ -72,7 +72,8 @@ PagedTokens tokens_of(const ep_tokens *t)
     return PagedTokens{t->positions, t->pos_stride_b, t->pos_stride_s, t->table, t->table_stride, t->width, t->B, t->S};
 }
 
-int check_attend(const ep_heads *q, const ep_tokens *t, const ep_kv_cache *cache, PagedCache &c)
+// Query rows over a cache, of any of the types that attention takes.
+int check_query(const ep_heads *q, const ep_tokens *t, const ep_kv_cache *cache, PagedCache &c)
 {
     int rc = check_tokens(t, true);
     if (rc == EP_OK)
@@ -86,13 +87,33 @@ int check_attend(const ep_heads *q, const ep_tokens *t, const ep_kv_cache *cache
                          (long long)t->width, c.page);
     if (q->dtype == EP_F32)
         return set_error(EP_DECLINE_DTYPE, "attention: q must be f16 or bf16");
-    if ((c.dtype == EP_F16 || c.dtype == EP_BF16) && c.dtype != q->dtype)
-        return set_error(EP_DECLINE_DTYPE, "attention: a 16-bit cache must have q's type");
     if (q->heads % c.heads)
         return set_error(EP_ERR_ARG, "%d query heads over %d cache heads", q->heads, c.heads);
     if (!aligned16(q->ptr) || (t->B > 1 && q->stride_b % 8) || (t->S > 1 && q->stride_s % 8) ||
         (q->heads > 1 && q->stride_h % 8))
         return set_error(EP_DECLINE_SHAPE, "attention: q's heads must be 16-byte aligned");
+    return EP_OK;
+}
+
+int check_attend(const ep_heads *q, const ep_tokens *t, const ep_kv_cache *cache, PagedCache &c)
+{
+    const int rc = check_query(q, t, cache, c);
+    if (rc == EP_OK && (c.dtype == EP_F16 || c.dtype == EP_BF16) && c.dtype != q->dtype)
+        return set_error(EP_DECLINE_DTYPE, "attention: a 16-bit cache must have q's type");
+    return rc;
+}
+
+// Pages taken of a context: their positions fit 30 bits.
+int check_take(int64_t take, const ep_tokens *t, const PagedCache &c)
+{
+    if (take < 1)
+        return set_error(EP_ERR_ARG, "%lld pages a token", (long long)take);
+    if (take > 0x3fffffff >> c.page_shift)
+        return set_error(EP_DECLINE_SHAPE, "%lld pages of %d rows a token: up to 2^30 positions are served",
+                         (long long)take, c.page);
+    // rows times pages: the scores and lists of a call
+    if (t->B * t->S > (INT64_MAX / 8) / ((int64_t)c.heads * (t->width > take ? t->width : take)))
+        return set_error(EP_DECLINE_SHAPE, "lists of %lld pages are more than one call takes", (long long)take);
     return EP_OK;
 }
 
@@ -192,6 +213,115 @@ int ep_paged_attention(const ep_heads *q, const ep_tokens *tokens, const ep_kv_c
     if (!aligned16(out) || !aligned16(workspace))
         return set_error(EP_DECLINE_SHAPE, "attention: output and workspace must be 16-byte aligned");
     return launch_attend(q, tokens_of(tokens), c, scale, window, out, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+size_t ep_paged_attention_shared_workspace(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache,
+                                           int64_t shared)
+{
+    set_error(EP_OK, "");
+    PagedCache c;
+    if (check_attend(q, tokens, cache, c) != EP_OK || shared < 0 || shared > tokens->width)
+        return 0;
+    return attend_parts_workspace(q, tokens_of(tokens), c, shared);
+}
+
+int ep_paged_attention_shared(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache, int64_t shared,
+                              float scale, int64_t window, void *out, void *workspace, size_t workspace_bytes,
+                              void *stream)
+{
+    set_error(EP_OK, "");
+    PagedCache c;
+    const int rc = check_attend(q, tokens, cache, c);
+    if (rc != EP_OK)
+        return rc;
+    if (shared < 0 || shared > tokens->width)
+        return set_error(EP_ERR_ARG, "%lld shared pages in tables of %lld", (long long)shared, (long long)tokens->width);
+    if (tokens->B == 0 || tokens->S == 0)
+        return EP_OK;
+    if (!out)
+        return set_error(EP_ERR_ARG, "attention: null output");
+    if (!aligned16(out) || !aligned16(workspace))
+        return set_error(EP_DECLINE_SHAPE, "attention: output and workspace must be 16-byte aligned");
+    return launch_attend_parts(q, tokens_of(tokens), c, shared, scale, window, out, workspace, workspace_bytes,
+                               (hipStream_t)stream);
+}
+
+int ep_kv_bounds(const ep_tokens *tokens, const ep_kv_cache *cache, void *bounds, void *stream)
+{
+    set_error(EP_OK, "");
+    PagedCache c;
+    int rc = check_tokens(tokens, true);
+    if (rc == EP_OK)
+        rc = check_cache(cache, c);
+    if (rc != EP_OK)
+        return rc;
+    if (!bounds || !aligned16(bounds))
+        return set_error(EP_ERR_ARG, "bounds must be 16-byte aligned storage");
+    if (tokens->B == 0 || tokens->S == 0)
+        return EP_OK;
+    return launch_kv_bounds(tokens_of(tokens), c, bounds, (hipStream_t)stream);
+}
+
+size_t ep_kv_select_workspace(const ep_tokens *tokens, const ep_kv_cache *cache, int64_t take)
+{
+    set_error(EP_OK, "");
+    PagedCache c;
+    if (check_tokens(tokens, true) != EP_OK || check_cache(cache, c) != EP_OK || check_take(take, tokens, c) != EP_OK)
+        return 0;
+    return select_workspace(tokens_of(tokens), c, take);
+}
+
+int ep_kv_select(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache, const void *bounds, int64_t take,
+                 int32_t *blocks, void *workspace, size_t workspace_bytes, void *stream)
+{
+    set_error(EP_OK, "");
+    PagedCache c;
+    int rc = check_query(q, tokens, cache, c);
+    if (rc == EP_OK)
+        rc = check_take(take, tokens, c);
+    if (rc != EP_OK)
+        return rc;
+    if (!bounds || !aligned16(bounds))
+        return set_error(EP_ERR_ARG, "bounds must be 16-byte aligned storage");
+    if (tokens->B == 0 || tokens->S == 0)
+        return EP_OK;
+    if (!blocks)
+        return set_error(EP_ERR_ARG, "select: null output");
+    if (!aligned16(workspace))
+        return set_error(EP_DECLINE_SHAPE, "select: the workspace must be 16-byte aligned");
+    return launch_kv_select(q, tokens_of(tokens), c, bounds, take, blocks, workspace, workspace_bytes,
+                            (hipStream_t)stream);
+}
+
+size_t ep_paged_attention_blocks_workspace(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache,
+                                           int64_t take)
+{
+    set_error(EP_OK, "");
+    PagedCache c;
+    if (check_attend(q, tokens, cache, c) != EP_OK || check_take(take, tokens, c) != EP_OK)
+        return 0;
+    return attend_blocks_workspace(q, tokens_of(tokens), c, take);
+}
+
+int ep_paged_attention_blocks(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache,
+                              const int32_t *blocks, int64_t take, float scale, int64_t window, void *out,
+                              void *workspace, size_t workspace_bytes, void *stream)
+{
+    set_error(EP_OK, "");
+    PagedCache c;
+    int rc = check_attend(q, tokens, cache, c);
+    if (rc == EP_OK)
+        rc = check_take(take, tokens, c);
+    if (rc != EP_OK)
+        return rc;
+    if (tokens->B == 0 || tokens->S == 0)
+        return EP_OK;
+    if (!out || !blocks)
+        return set_error(EP_ERR_ARG, "attention: null output or list of pages");
+    if (!aligned16(out) || !aligned16(workspace))
+        return set_error(EP_DECLINE_SHAPE, "attention: output and workspace must be 16-byte aligned");
+    return launch_attend_blocks(q, tokens_of(tokens), c, blocks, take, scale, window, out, workspace, workspace_bytes,
+                                (hipStream_t)stream);
 }
 
 }  // extern "C"

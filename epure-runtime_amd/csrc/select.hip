@@ -1,0 +1,514 @@
+// Bounds of a paged cache's keys, and the pages of a context that matter most
+// to a token by them (include/epure_paged.h).  Attention over those pages is
+// attend_kernel.h.
+//
+//   lo_d, hi_d = least and largest key value of column d over a page's rows
+//   score(page) = sum_d hi_d sum_g max(q_gd, 0) + lo_d sum_g min(q_gd, 0)
+//
+// over the query heads g that share the cache head: every product q_gd k_d of a
+// row of the page is at most its term, so the group's scores of no position
+// there sum to more.  The heads enter as two vectors, so the work does not
+// grow with them: 2 D multiply-adds a page.
+//
+// The choice is a whole number, so the scores are sums in 64 bits: the
+// products of 16-bit values are exact there, and pages next to the border
+// do not change places with the order of a sum, as they would in 32 bits.
+#include "ep_common.h"
+#include "ep_internal.h"
+#include "ep_paged.h"
+
+namespace ep {
+namespace {
+
+constexpr int kChunkTokens = 64;    // tokens a workgroup of the bounds looks over
+constexpr int kChunkPages = 128;    // pages a workgroup scores
+constexpr int kHeldKeys = 4096;     // scores that the choice keeps in LDS (32 KiB)
+
+struct BoundsArgs {
+    PagedTokens tok;
+    PagedCache c;
+    void *bounds;
+    uint32_t first_wg, chunks;
+};
+
+// Eight adjacent values of a cache row as f32.
+template <int CODE>
+EP_DEV void row_values(const PagedCache &c, int64_t row, int d, float *v)
+{
+    if constexpr (CODE == EP_I8 || CODE == EP_E4M3) {
+        const float s = c.k_scale[row];
+        uint32_t w[2];
+        __builtin_memcpy(w, __builtin_assume_aligned((const uint8_t *)c.k + row * c.D + d, 8), 8);
+        decode4(w[0], CODE, v);
+        decode4(w[1], CODE, v + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] *= s;
+    } else {
+        uint16_t r[8];
+        __builtin_memcpy(r, __builtin_assume_aligned((const uint16_t *)c.k + row * c.D + d, 16), 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = CODE == EP_F16 ? (float)f16_from_bits(r[i]) : bf16_to_f32(r[i]);
+    }
+}
+
+// A NaN stays: a page that holds one is not to be passed over.
+EP_DEV float least(float a, float b) { return b < a || b != b ? b : a; }
+EP_DEV float largest(float a, float b) { return b > a || b != b ? b : a; }
+
+// One workgroup looks over 64 tokens of a sequence and one cache head.  Of the
+// tokens on one page the one at the largest position (of two there, the later
+// in the call) rebuilds the page's bounds from its rows up to that position:
+// what the page held before the call counts as the new rows do, nothing that it
+// held for an earlier sequence does, and it does not matter how often it is done.
+template <int CODE>
+__global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
+{
+    __shared__ float s_lo[256 * 8], s_hi[256 * 8];
+    const uint32_t at = a.first_wg + blockIdx.x, H = a.c.heads;
+    const uint32_t part = at / H, h = at - part * H, b = part / a.chunks, chunk = part - b * a.chunks;
+    const int tid = threadIdx.x, lane = tid & 63, D = a.c.D;
+    const int64_t *pos = a.tok.pos + (int64_t)b * a.tok.pos_sb;
+    const int64_t s = (int64_t)chunk * kChunkTokens + lane, ps = a.tok.pos_ss;
+    const int64_t p = s < a.tok.S ? pos[s * ps] : -1, after = s + 1 < a.tok.S ? pos[(s + 1) * ps] : -1;
+    const int64_t index = p >> a.c.page_shift;
+    int32_t id = -1;
+    if (p >= 0 && index < a.tok.width)
+        id = a.tok.table[b * a.tok.table_stride + index];
+    // the next token is the next row of the page: not the last one there
+    const bool inner = after == p + 1 && after >> a.c.page_shift == index;
+    uint64_t left = __ballot(id >= 0 && id < a.c.n_pages && !inner);
+    const int lanes = D / 8, group = tid / lanes, u = tid - group * lanes, groups = 256 / lanes;
+    for (; left; left &= left - 1) {
+        const int l = __builtin_ctzll(left);
+        const int64_t mine = __shfl(p, l, 64), page = mine >> a.c.page_shift, who = (int64_t)chunk * kChunkTokens + l;
+        if (a.tok.S > 1) {
+            int later = 0;
+            for (int64_t t = tid; t < a.tok.S; t += 256) {
+                const int64_t o = pos[t * ps];
+                later |= o >= 0 && o >> a.c.page_shift == page && (o > mine || (o == mine && t > who));
+            }
+            if (__syncthreads_or(later))
+                continue;
+        }
+        const int64_t row0 = ((int64_t)__shfl(id, l, 64) * H + h) * a.c.page;
+        const int rows = (int)(mine & (a.c.page - 1)) + 1;
+        float lo[8], hi[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            lo[i] = INFINITY;
+            hi[i] = -INFINITY;
+        }
+        if (group < groups)
+            for (int r = group; r < rows; r += 4 * groups) {
+                float v[4][8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)      // four rows in flight; past the end the last again
+                    row_values<CODE>(a.c, row0 + min(r + k * groups, rows - 1), 8 * u, v[k]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        lo[i] = least(lo[i], v[k][i]);
+                        hi[i] = largest(hi[i], v[k][i]);
+                    }
+            }
+        __syncthreads();         // the buffers' last readers are done
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            s_lo[8 * tid + i] = lo[i];      // [group][D], as 8 (group lanes + u) + i = group D + 8 u + i
+            s_hi[8 * tid + i] = hi[i];
+        }
+        __syncthreads();
+        const int64_t out = ((int64_t)__shfl(id, l, 64) * H + h) * 2 * D;
+        for (int e = tid; e < 2 * D; e += 256) {
+            const bool top = e >= D;
+            const int d = top ? e - D : e;
+            float x = top ? s_hi[d] : s_lo[d];
+            for (int k = 1; k < groups; ++k)
+                x = top ? largest(x, s_hi[k * D + d]) : least(x, s_lo[k * D + d]);
+            if constexpr (CODE == EP_F16)
+                ((f16_t *)a.bounds)[out + e] = (f16_t)x;
+            else if constexpr (CODE == EP_BF16)
+                ((uint16_t *)a.bounds)[out + e] = f32_to_bf16(x);
+            else
+                ((float *)a.bounds)[out + e] = x;
+        }
+    }
+}
+
+struct SelectArgs {
+    const void *q;
+    int64_t q_sb, q_ss, q_sh;
+    int q_dtype, G;
+    PagedTokens tok;
+    PagedCache c;
+    const void *bounds;
+    uint64_t *keys;          // [rows][width]
+    int32_t *blocks;         // [rows][take]
+    uint32_t first_wg, chunks;
+    int take, lanes;         // lanes: that hold a page's D columns, eight each, a power of two
+};
+
+// Row r: a token's cache head, and the page that the token lies on (-1: none).
+struct SelectRow {
+    uint32_t token, h;
+    int64_t b, s, own;
+};
+EP_DEV SelectRow select_row(const SelectArgs &a, uint32_t r)
+{
+    SelectRow o;
+    o.token = r / (uint32_t)a.c.heads;
+    o.h = r - o.token * a.c.heads;
+    o.b = o.token / (uint32_t)a.tok.S;
+    o.s = o.token - o.b * a.tok.S;
+    const int64_t p = a.tok.pos[o.b * a.tok.pos_sb + o.s * a.tok.pos_ss], page = p >> a.c.page_shift;
+    o.own = p < 0 || page >= a.tok.width ? -1 : page;
+    return o;
+}
+
+template <int CTRL>
+EP_DEV double dpp_f64(double v)
+{
+    const uint64_t b = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)b, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+    return __longlong_as_double(((uint64_t)hi << 32) | lo);
+}
+
+// Sum over `lanes` adjacent lanes (a power of two, at most 32).
+EP_DEV double lanes_sum(double v, int lanes)
+{
+    if (lanes > 1)
+        v += dpp_f64<0xb1>(v);      // quad_perm [1,0,3,2]
+    if (lanes > 2)
+        v += dpp_f64<0x4e>(v);      // quad_perm [2,3,0,1]
+    if (lanes > 4)
+        v += dpp_f64<0x141>(v);     // row_half_mirror
+    if (lanes > 8)
+        v += dpp_f64<0x140>(v);     // row_mirror
+    if (lanes > 16)
+        v += __shfl_xor(v, 16, 64);
+    return v;
+}
+
+// Scores as integers of the same order: a NaN above all (a page that holds
+// one, or that the pool lacks, is not to be passed over).
+EP_DEV uint64_t order_key(double v)
+{
+    const uint64_t b = __double_as_longlong(v + 0.0);       // one zero
+    if (v != v)
+        return ~0ull;
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+
+// Eight bounds of either kind, one of them low or high.
+template <bool WIDE>
+struct Bounds8 {
+    u32x4_t w[WIDE ? 2 : 1];
+    EP_DEV void load(const void *p, int64_t at)
+    {
+        const u32x4_t *src = (const u32x4_t *)((const char *)p + at * (WIDE ? 4 : 2));
+        w[0] = src[0];
+        if constexpr (WIDE)
+            w[1] = src[1];
+    }
+    EP_DEV float at(int i, bool f16) const
+    {
+        if constexpr (WIDE)
+            return __uint_as_float(w[i / 4][i % 4]);
+        const uint16_t b = (uint16_t)(w[0][i / 2] >> (16 * (i % 2)));
+        return f16 ? (float)f16_from_bits(b) : bf16_to_f32(b);
+    }
+};
+
+template <bool WIDE>
+__global__ void __launch_bounds__(256) score_kernel(SelectArgs a)
+{
+    const uint32_t at = a.first_wg + blockIdx.x, r = at / a.chunks, chunk = at - r * a.chunks;
+    const SelectRow row = select_row(a, r);
+    const int64_t page0 = (int64_t)chunk * kChunkPages, page1 = page0 + kChunkPages < row.own ? page0 + kChunkPages : row.own;
+    if (row.own < a.take || page0 >= page1)      // all pages are taken, or none of these is asked about
+        return;
+    const int L = a.lanes, tid = threadIdx.x, u = tid & (L - 1), D = a.c.D;
+    const bool in = 8 * u < D;
+    const int d = in ? 8 * u : 0;
+    // this lane's eight columns of the group's queries
+    double up[8], down[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        up[i] = down[i] = 0.0;
+    for (int g = 0; g < a.G; ++g) {
+        const int64_t src = row.b * a.q_sb + row.s * a.q_ss + (int64_t)(row.h * a.G + g) * a.q_sh + d;
+        uint16_t w[8];
+        __builtin_memcpy(w, __builtin_assume_aligned((const uint16_t *)a.q + src, 16), 16);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = a.q_dtype == EP_F16 ? (float)f16_from_bits(w[i]) : bf16_to_f32(w[i]);
+            // a NaN reaches both sums
+            up[i] += v < 0.0f ? 0.0 : (double)v;
+            down[i] += v > 0.0f ? 0.0 : (double)v;
+        }
+    }
+    const int32_t *table = a.tok.table + row.b * a.tok.table_stride;
+    uint64_t *keys = a.keys + (int64_t)r * a.tok.width;
+    const int step = 256 / L;
+    const bool f16 = a.c.dtype == EP_F16;
+    for (int64_t k0 = page0 + tid / L; k0 < page1; k0 += 2 * step) {
+        int32_t id[2];
+        Bounds8<WIDE> lo[2], hi[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int64_t page = k0 + k * step;
+            id[k] = table[page < page1 ? page : k0];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const bool ok = id[k] >= 0 && id[k] < a.c.n_pages;
+            const int64_t src = ((int64_t)(ok ? id[k] : 0) * a.c.heads + row.h) * 2 * D + d;
+            lo[k].load(a.bounds, src);
+            hi[k].load(a.bounds, src + D);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                sum = fma((double)lo[k].at(i, f16), down[i], fma((double)hi[k].at(i, f16), up[i], sum));
+            sum = lanes_sum(in ? sum : 0.0, L);
+            const int64_t page = k0 + k * step;
+            if (u == 0 && page < page1)
+                keys[page] = id[k] >= 0 && id[k] < a.c.n_pages ? order_key(sum) : ~0ull;
+        }
+    }
+}
+
+// Exclusive sum over the workgroup's 256 threads of two counts.
+EP_DEV uint2 exclusive_sums(uint32_t x, uint32_t y, uint2 *s_part, uint2 &total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t px = x, py = y;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t ox = __shfl_up(px, d, 64), oy = __shfl_up(py, d, 64);
+        px += lane >= d ? ox : 0u;
+        py += lane >= d ? oy : 0u;
+    }
+    __syncthreads();
+    if (lane == 63)
+        s_part[wave] = make_uint2(px, py);
+    __syncthreads();
+    uint2 before = make_uint2(0, 0);
+    total = before;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        before.x += w < wave ? s_part[w].x : 0u;
+        before.y += w < wave ? s_part[w].y : 0u;
+        total.x += s_part[w].x;
+        total.y += s_part[w].y;
+    }
+    return make_uint2(before.x + px - x, before.y + py - y);
+}
+
+// A row's choice, one workgroup: the (take - 1) largest keys ahead of the own
+// page, found digit by digit from the top.  A round counts 2048 digits of
+// what lies between the least and the largest key still in question, so that
+// the first one parts them about as well as their number allows; of equal keys
+// the first are taken.
+__global__ void __launch_bounds__(256) choose_kernel(SelectArgs a)
+{
+    __shared__ uint64_t s_key[kHeldKeys];
+    __shared__ uint32_t s_count[2048];
+    __shared__ uint64_t s_end[2][4];
+    __shared__ uint2 s_part[4];
+    __shared__ uint32_t s_found[3];
+    const uint32_t r = a.first_wg + blockIdx.x;
+    const SelectRow row = select_row(a, r);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, take = a.take;
+    int32_t *out = a.blocks + (int64_t)r * take;
+    const int64_t n = row.own;
+    if (n < take) {
+        for (int i = tid; i < take; i += 256)
+            out[i] = i <= n ? i : -1;
+        return;
+    }
+    if (take == 1) {
+        if (tid == 0)
+            out[0] = (int32_t)n;
+        return;
+    }
+    const uint64_t *keys = a.keys + (int64_t)r * a.tok.width;
+    const bool held = n <= kHeldKeys;
+    uint64_t lo = ~0ull, hi = 0;
+    for (int64_t i = tid; i < n; i += 256) {
+        const uint64_t k = keys[i];
+        if (held)
+            s_key[i] = k;
+        lo = k < lo ? k : lo;
+        hi = k > hi ? k : hi;
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d /= 2) {
+        const uint64_t l = __shfl_xor(lo, d, 64), h = __shfl_xor(hi, d, 64);
+        lo = l < lo ? l : lo;
+        hi = h > hi ? h : hi;
+    }
+    if (lane == 0) {
+        s_end[0][wave] = lo;
+        s_end[1][wave] = hi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        lo = s_end[0][w] < lo ? s_end[0][w] : lo;
+        hi = s_end[1][w] > hi ? s_end[1][w] : hi;
+    }
+    auto key = [&](int64_t i) { return held ? s_key[i] : keys[i]; };
+    uint64_t span = hi - lo;
+    uint32_t need = take - 1;
+    bool all = false;        // every key from lo on is taken; else `need` of those equal to lo
+    for (;;) {
+        const int bits = span ? 64 - __builtin_clzll(span) : 0, shift = bits > 11 ? bits - 11 : 0;
+        for (int i = tid; i < 2048; i += 256)
+            s_count[i] = 0;
+        __syncthreads();
+        for (int64_t i = tid; i < n; i += 256) {
+            const uint64_t k = key(i) - lo;         // below lo: past the span
+            if (k <= span)
+                atomicAdd(&s_count[k >> shift], 1u);
+        }
+        __syncthreads();
+        // thread t holds digits 2047 - 8 t .. 2040 - 8 t
+        uint32_t c[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            c[i] = s_count[2047 - 8 * tid - i];
+            sum += c[i];
+        }
+        uint2 total;
+        uint32_t above = exclusive_sums(sum, 0, s_part, total).x;
+        if (above < need && above + sum >= need)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (above < need && above + c[i] >= need) {
+                    s_found[0] = 2047 - 8 * tid - i;
+                    s_found[1] = above;
+                    s_found[2] = c[i];
+                }
+                above += c[i];
+            }
+        __syncthreads();
+        lo += (uint64_t)s_found[0] << shift;
+        need -= s_found[1];
+        all = s_found[2] == need;
+        if (all || shift == 0)
+            break;
+        span = (1ull << shift) - 1;
+    }
+    // in order: thread t writes what it takes of its n / 256 keys
+    const int64_t per = (n + 255) / 256, i0 = tid * per < n ? tid * per : n, i1 = i0 + per < n ? i0 + per : n;
+    uint32_t over = 0, equal = 0;
+    for (int64_t i = i0; i < i1; ++i) {
+        const uint64_t k = key(i);
+        over += all ? k >= lo : k > lo;
+        equal += !all && k == lo;
+    }
+    uint2 total;
+    const uint2 before = exclusive_sums(over, equal, s_part, total);
+    uint32_t ties = before.y, to = before.x + (ties < need ? ties : need);
+    if (all)
+        to = before.x;
+    for (int64_t i = i0; i < i1; ++i) {
+        const uint64_t k = key(i);
+        bool in = all ? k >= lo : k > lo;
+        if (!all && k == lo)
+            in = ties++ < need;
+        if (in)
+            out[to++] = (int32_t)i;
+    }
+    if (tid == 0)
+        out[take - 1] = (int32_t)n;
+}
+
+// A launch has fewer than 2^32 threads: a grid beyond that is cut into several.
+template <typename ARGS, typename F>
+int in_launches(int64_t grid, ARGS a, F launch)
+{
+    const int64_t most = 0xffffffff / 256;
+    for (int64_t at = 0; at < grid; at += most) {
+        a.first_wg = (uint32_t)at;
+        launch(a, (unsigned)(grid - at < most ? grid - at : most));
+        EP_HIP_CHECK(hipGetLastError());
+    }
+    return EP_OK;
+}
+
+}  // namespace
+
+int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, hipStream_t stream)
+{
+    const int64_t chunks = (tok.S + kChunkTokens - 1) / kChunkTokens;
+    const int64_t parts = tok.B * chunks;
+    if (parts > 0x7fffffff / c.heads)
+        return set_error(EP_DECLINE_SHAPE, "bounds of %lld x %lld tokens are more than one call takes", (long long)tok.B,
+                         (long long)tok.S);
+    return in_launches(parts * c.heads, BoundsArgs{tok, c, bounds, 0, (uint32_t)chunks}, [&](const BoundsArgs &a, unsigned n) {
+        if (c.dtype == EP_BF16)
+            bounds_kernel<EP_BF16><<<n, 256, 0, stream>>>(a);
+        else if (c.dtype == EP_F16)
+            bounds_kernel<EP_F16><<<n, 256, 0, stream>>>(a);
+        else if (c.dtype == EP_I8)
+            bounds_kernel<EP_I8><<<n, 256, 0, stream>>>(a);
+        else
+            bounds_kernel<EP_E4M3><<<n, 256, 0, stream>>>(a);
+    });
+}
+
+// No scores where every page is taken.
+size_t select_workspace(const PagedTokens &tok, const PagedCache &c, int64_t take)
+{
+    return tok.width > take ? (size_t)tok.B * tok.S * c.heads * tok.width * sizeof(uint64_t) : 0;
+}
+
+int launch_kv_select(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, const void *bounds, int64_t take,
+                     int32_t *blocks, void *ws, size_t ws_bytes, hipStream_t stream)
+{
+    const int64_t rows = tok.B * tok.S * c.heads, chunks = (tok.width + kChunkPages - 1) / kChunkPages;
+    if (rows > 0x7fffffff || (chunks > 0 && rows > 0x7fffffff / chunks))
+        return set_error(EP_DECLINE_SHAPE, "%lld rows over %lld pages are more than one call takes", (long long)rows,
+                         (long long)tok.width);
+    const size_t want = select_workspace(tok, c, take);
+    if (ws_bytes < want || (want && !ws))
+        return set_error(EP_ERR_WORKSPACE, "select: workspace of %zu bytes, %zu wanted", ws_bytes, want);
+    SelectArgs a{};
+    a.q = q->ptr;
+    a.q_sb = q->stride_b;
+    a.q_ss = q->stride_s;
+    a.q_sh = q->stride_h;
+    a.q_dtype = q->dtype;
+    a.G = q->heads / c.heads;
+    a.tok = tok;
+    a.c = c;
+    a.bounds = bounds;
+    a.keys = (uint64_t *)ws;
+    a.blocks = blocks;
+    a.chunks = (uint32_t)chunks;
+    a.take = (int)take;
+    a.lanes = 2;
+    while (a.lanes * 8 < c.D)
+        a.lanes *= 2;
+    int rc = EP_OK;
+    if (want && take > 1)
+        rc = in_launches(rows * chunks, a, [&](const SelectArgs &part, unsigned n) {
+            if (c.dtype == EP_F16 || c.dtype == EP_BF16)
+                score_kernel<false><<<n, 256, 0, stream>>>(part);
+            else
+                score_kernel<true><<<n, 256, 0, stream>>>(part);
+        });
+    if (rc == EP_OK)
+        rc = in_launches(rows, a, [&](const SelectArgs &part, unsigned n) { choose_kernel<<<n, 256, 0, stream>>>(part); });
+    return rc;
+}
+
+}  // namespace ep

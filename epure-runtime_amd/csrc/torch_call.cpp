@@ -315,7 +315,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "epure_torch", nullptr, -1, methods
 PyMODINIT_FUNC PyInit_epure_torch(void)
 {
     PyObject *m = PyModule_Create(&module);
-    if (m && PyModule_AddFunctions(m, paged_methods) != 0) {
+    if (m && (PyModule_AddFunctions(m, paged_methods) != 0 || PyModule_AddFunctions(m, draft_methods) != 0)) {
         Py_DECREF(m);
         return nullptr;
     }

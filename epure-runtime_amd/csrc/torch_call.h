@@ -1,4 +1,5 @@
-// What the native call paths share (torch_call.cpp, torch_paged.cpp).
+// What the native call paths share (torch_call.cpp, torch_paged.cpp,
+// torch_draft.cpp).
 #pragma once
 
 #include <torch/csrc/Exceptions.h>
@@ -32,5 +33,6 @@ PyObject *failed(const char *what, int rc);
 bool args_are(Py_ssize_t n, Py_ssize_t want);
 
 extern PyMethodDef paged_methods[];  // torch_paged.cpp
+extern PyMethodDef draft_methods[];  // torch_draft.cpp
 
 }  // namespace epure_torch

@@ -6,6 +6,7 @@
 // takes the way through Python (epure/paged.py), which checks and raises.
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <c10/core/DeviceGuard.h>
 
 #include "torch_call.h"
 #include "epure_paged.h"
@@ -18,6 +19,13 @@ decltype(&ep_kv_append) fn_append;
 decltype(&ep_kv_read) fn_read;
 decltype(&ep_paged_attention_workspace) fn_attend_ws;
 decltype(&ep_paged_attention) fn_attend;
+decltype(&ep_paged_attention_shared_workspace) fn_shared_ws;
+decltype(&ep_paged_attention_shared) fn_shared;
+decltype(&ep_kv_bounds) fn_bounds;
+decltype(&ep_kv_select_workspace) fn_select_ws;
+decltype(&ep_kv_select) fn_select;
+decltype(&ep_paged_attention_blocks_workspace) fn_blocks_ws;
+decltype(&ep_paged_attention_blocks) fn_blocks;
 
 // A plain GPU tensor argument on `dev` (any where dev < 0), or nullptr.  One
 // with a forward-mode tangent is not plain: nothing here would carry it on.
@@ -104,6 +112,18 @@ bool cache_of(PyObject *const *args, c10::DeviceIndex &dev, ep_kv_cache &c)
         }
     c = ep_kv_cache{k->data_ptr(), v->data_ptr(), scale[0], scale[1], code,
                     (int)k->size(1), (int)k->size(2), (int)k->size(3), k->size(0)};
+    return true;
+}
+
+// Storage of a cache's bounds (include/epure_paged.h).
+bool bounds_of(PyObject *arg, c10::DeviceIndex &dev, const ep_kv_cache &c, void *&out)
+{
+    const at::Tensor *t = gpu_tensor(arg, dev);
+    const auto want = c.dtype == EP_F16 ? at::kHalf : c.dtype == EP_BF16 ? at::kBFloat16 : at::kFloat;
+    if (!t || t->scalar_type() != want || !t->is_contiguous() || t->dim() != 4 || t->size(0) != c.n_pages ||
+        t->size(1) != c.heads || t->size(2) != 2 || t->size(3) != c.D || needs_grad({t}))
+        return false;
+    out = t->data_ptr();
     return true;
 }
 
@@ -277,16 +297,14 @@ PyObject *rotate(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 // ------------------------------------------------------------------ the cache
 // append(k, v, positions, table, q or None, cos or None, sin or None,
 // interleaved, cache k, v, k_scale, v_scale): q turned, or None.
-PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+PyObject *append_to(PyObject *const *args, PyObject *bounds_arg)
 {
-    HANDLE_TH_ERRORS
-    if (!args_are(nargs, 12))
-        return nullptr;
     if (!plain_call())
         Py_RETURN_NOTIMPLEMENTED;
     c10::DeviceIndex dev = -1;
     ep_kv_cache c;
-    if (!cache_of(args + 8, dev, c))
+    void *bounds = nullptr;
+    if (!cache_of(args + 8, dev, c) || (bounds_arg && !bounds_of(bounds_arg, dev, c, bounds)))
         Py_RETURN_NOTIMPLEMENTED;
     const bool some_q = args[4] != Py_None, turns = args[5] != Py_None;
     const at::Tensor *k = gpu_tensor(args[0], dev), *v = gpu_tensor(args[1], dev), *pos = gpu_tensor(args[2], dev);
@@ -320,9 +338,35 @@ PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         Py_RETURN_NOTIMPLEMENTED;
     if (rc < 0)
         return failed("ep_kv_append", rc);
+    if (bounds) {
+        Py_BEGIN_ALLOW_THREADS
+        rc = fn_bounds(&tok, &c, bounds, stream);
+        Py_END_ALLOW_THREADS
+        if (rc != EP_OK)
+            return failed("ep_kv_bounds", rc);
+    }
     if (!some_q)
         Py_RETURN_NONE;
     return THPVariable_Wrap(qo);
+}
+
+PyObject *append(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    return args_are(nargs, 12) ? append_to(args, nullptr) : nullptr;
+    END_HANDLE_TH_ERRORS
+}
+
+// append_bounds(append's arguments, cache k_bounds): the same, and the bounds of the pages written
+PyObject *append_bounds(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    if (!args_are(nargs, 13))
+        return nullptr;
+    c10::DeviceIndex dev = -1;
+    const at::Tensor *k = gpu_tensor(args[0], dev);
+    const c10::OptionalDeviceGuard guard(k ? c10::optional<c10::Device>(k->device()) : c10::nullopt);
+    return append_to(args, args[12]);
     END_HANDLE_TH_ERRORS
 }
 
@@ -416,6 +460,113 @@ PyObject *attend(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
+// Query rows, positions and table of an attention over c.
+bool query_of(PyObject *const *args, c10::DeviceIndex &dev, const ep_kv_cache &c, const at::Tensor *&q, ep_tokens &tok)
+{
+    q = gpu_tensor(args[0], dev);
+    const at::Tensor *pos = gpu_tensor(args[1], dev), *table = gpu_tensor(args[2], dev);
+    return q && pos && table && heads_ok(*q) && q->size(3) == c.D && tokens_of(*pos, q->size(0), q->size(1), tok) &&
+           table_of(*table, tok) && !needs_grad({q}) && c.heads > 0 && q->size(2) % c.heads == 0;
+}
+
+// attend_more(q, positions, table, scale or None, window or None, shared
+// pages, blocks or None, cache k, v, k_scale, v_scale): the attention's output
+PyObject *attend_more(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    if (!args_are(nargs, 11))
+        return nullptr;
+    if (!plain_call())
+        Py_RETURN_NOTIMPLEMENTED;
+    c10::DeviceIndex dev = -1;
+    ep_kv_cache c;
+    ep_tokens tok;
+    const at::Tensor *q;
+    if (!cache_of(args + 7, dev, c) || !query_of(args, dev, c, q, tok))
+        Py_RETURN_NOTIMPLEMENTED;
+    const bool listed = args[6] != Py_None;
+    const at::Tensor *blocks = listed ? gpu_tensor(args[6], dev) : nullptr;
+    if (listed && (!blocks || blocks->scalar_type() != at::kInt || blocks->dim() != 4 || !blocks->is_contiguous() ||
+                   blocks->size(0) != tok.B || blocks->size(1) != tok.S || blocks->size(2) != c.heads ||
+                   blocks->size(3) < 1))
+        Py_RETURN_NOTIMPLEMENTED;
+    const double scale = args[3] == Py_None ? 1.0 / std::sqrt((double)c.D) : PyFloat_AsDouble(args[3]);
+    const int64_t window = args[4] == Py_None ? 0 : PyLong_AsLongLong(args[4]), shared = PyLong_AsLongLong(args[5]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NOTIMPLEMENTED;
+    }
+    if ((args[4] != Py_None && window < 1) || shared < 0 || shared > tok.width || (listed && shared > 0))
+        Py_RETURN_NOTIMPLEMENTED;
+    bool ok;
+    void *stream = stream_of(*q, &ok);
+    if (!ok)
+        return nullptr;
+    const c10::DeviceGuard guard(q->device());
+    const ep_heads qh = heads_of(*q);
+    const int64_t take = listed ? blocks->size(3) : 0;
+    const size_t n = listed ? fn_blocks_ws(&qh, &tok, &c, take) : fn_shared_ws(&qh, &tok, &c, shared);
+    const at::Tensor out = like(*q), ws = bytes_like(*q, n);
+    void *at = n ? ws.data_ptr() : nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    if (listed)
+        rc = fn_blocks(&qh, &tok, &c, (const int32_t *)blocks->const_data_ptr(), take, (float)scale, window,
+                       out.data_ptr(), at, n, stream);
+    else
+        rc = fn_shared(&qh, &tok, &c, shared, (float)scale, window, out.data_ptr(), at, n, stream);
+    Py_END_ALLOW_THREADS
+    if (rc == EP_ERR_ARG || rc > 0)     // q's type or alignment
+        Py_RETURN_NOTIMPLEMENTED;
+    if (rc < 0)
+        return failed(listed ? "ep_paged_attention_blocks" : "ep_paged_attention_shared", rc);
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// select(q, positions, table, n, cache k, v, k_scale, v_scale, k_bounds): blocks
+PyObject *select(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    if (!args_are(nargs, 9))
+        return nullptr;
+    if (!plain_call())
+        Py_RETURN_NOTIMPLEMENTED;
+    c10::DeviceIndex dev = -1;
+    ep_kv_cache c;
+    ep_tokens tok;
+    const at::Tensor *q;
+    void *bounds;
+    if (!cache_of(args + 4, dev, c) || !bounds_of(args[8], dev, c, bounds) || !query_of(args, dev, c, q, tok))
+        Py_RETURN_NOTIMPLEMENTED;
+    const int64_t take = PyLong_AsLongLong(args[3]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NOTIMPLEMENTED;
+    }
+    if (take < 1)
+        Py_RETURN_NOTIMPLEMENTED;
+    bool ok;
+    void *stream = stream_of(*q, &ok);
+    if (!ok)
+        return nullptr;
+    const c10::DeviceGuard guard(q->device());
+    const ep_heads qh = heads_of(*q);
+    const size_t n = fn_select_ws(&tok, &c, take);
+    const at::Tensor out = at::empty({tok.B, tok.S, c.heads, take}, q->options().dtype(at::kInt).requires_grad(false));
+    const at::Tensor ws = bytes_like(*q, n);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = fn_select(&qh, &tok, &c, bounds, take, (int32_t *)out.data_ptr(), n ? ws.data_ptr() : nullptr, n, stream);
+    Py_END_ALLOW_THREADS
+    if (rc == EP_ERR_ARG || rc > 0)
+        Py_RETURN_NOTIMPLEMENTED;
+    if (rc < 0)
+        return failed("ep_kv_select", rc);
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 // bind_paged(rotate, append, read, attention_workspace, attention): addresses
 PyObject *bind_paged(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 {
@@ -431,6 +582,24 @@ PyObject *bind_paged(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     Py_RETURN_NONE;
 }
 
+// bind_select(shared attention's workspace and call, bounds, select's workspace
+// and call, listed attention's workspace and call): addresses
+PyObject *bind_select(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    if (!args_are(nargs, 7))
+        return nullptr;
+    fn_shared_ws = (decltype(fn_shared_ws))PyLong_AsVoidPtr(args[0]);
+    fn_shared = (decltype(fn_shared))PyLong_AsVoidPtr(args[1]);
+    fn_bounds = (decltype(fn_bounds))PyLong_AsVoidPtr(args[2]);
+    fn_select_ws = (decltype(fn_select_ws))PyLong_AsVoidPtr(args[3]);
+    fn_select = (decltype(fn_select))PyLong_AsVoidPtr(args[4]);
+    fn_blocks_ws = (decltype(fn_blocks_ws))PyLong_AsVoidPtr(args[5]);
+    fn_blocks = (decltype(fn_blocks))PyLong_AsVoidPtr(args[6]);
+    if (PyErr_Occurred())
+        return nullptr;
+    Py_RETURN_NONE;
+}
+
 }  // namespace
 
 PyMethodDef paged_methods[] = {
@@ -439,6 +608,10 @@ PyMethodDef paged_methods[] = {
     {"append", (PyCFunction)(void (*)(void))append, METH_FASTCALL, nullptr},
     {"read", (PyCFunction)(void (*)(void))read, METH_FASTCALL, nullptr},
     {"attend", (PyCFunction)(void (*)(void))attend, METH_FASTCALL, nullptr},
+    {"bind_select", (PyCFunction)(void (*)(void))bind_select, METH_FASTCALL, nullptr},
+    {"append_bounds", (PyCFunction)(void (*)(void))append_bounds, METH_FASTCALL, nullptr},
+    {"attend_more", (PyCFunction)(void (*)(void))attend_more, METH_FASTCALL, nullptr},
+    {"select", (PyCFunction)(void (*)(void))select, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

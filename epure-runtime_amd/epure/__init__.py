@@ -1,12 +1,14 @@
 """epure (MI355X build) -- the fused codebook dequant-matmul behind every
 packed linear, on hand-written gfx950 HIP kernels, and what a served batch
-needs between the linears (rotary positions, a paged key-value cache, attention).
+needs between the linears (rotary positions, a paged key-value cache, attention,
+drafted tokens verified).
 
 Public names follow the reference package (epure/__init__.py:31-37) for the
 parts this build covers: the packed store, linear and embedding, the fine-tuning
 helpers, and the ``epure.kernels`` backend contract.
 """
 from . import container
+from .drafts import verify_draft
 from .finetune import (
     ScaleTuner,
     make_trainable,
@@ -33,6 +35,6 @@ __all__ = [
     "apply_packed", "tie_packed_lm_head",
     "make_trainable", "packed_weights", "snapshot_indices", "verify_frozen",
     "trainable_forward", "ScaleTuner", "container",
-    "Rotary", "rope_frequencies", "PagedKVCache",
+    "Rotary", "rope_frequencies", "PagedKVCache", "verify_draft",
     "__version__",
 ]

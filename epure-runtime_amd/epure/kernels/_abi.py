@@ -47,6 +47,15 @@ class Rotation(ctypes.Structure):
     _fields_ = [("cos_t", _p), ("sin_t", _p), ("max_pos", _c_i64), ("dim", _c_int), ("interleaved", _c_int)]
 
 
+# Descriptor of include/epure_draft.h.
+class Draft(ctypes.Structure):
+    _fields_ = [("B", _c_i64), ("V", _c_i64), ("n", _c_int), ("dtype", _c_int), ("target", _p),
+                ("target_stride_b", _c_i64), ("target_stride_s", _c_i64), ("draft", _p), ("draft_stride_b", _c_i64),
+                ("draft_stride_s", _c_i64), ("drafted", _p), ("drafted_stride_b", _c_i64), ("drafted_stride_s", _c_i64),
+                ("uniforms", _p), ("uniforms_stride_b", _c_i64), ("uniforms_stride_s", _c_i64)]
+
+
+_draft = ctypes.POINTER(Draft)
 _heads, _tokens = ctypes.POINTER(Heads), ctypes.POINTER(Tokens)
 _cache, _rotation = ctypes.POINTER(KVCache), ctypes.POINTER(Rotation)
 
@@ -137,6 +146,21 @@ _SIGS = {
     "ep_paged_attention": (_c_int, [
         _heads, _tokens, _cache, ctypes.c_float, _c_i64,  # q, tokens, cache, scale, window
         _p, _p, _sz, _p]),                       # out, workspace, bytes, stream
+    "ep_paged_attention_shared_workspace": (_sz, [_heads, _tokens, _cache, _c_i64]),
+    "ep_paged_attention_shared": (_c_int, [
+        _heads, _tokens, _cache, _c_i64, ctypes.c_float, _c_i64,  # q, tokens, cache, shared, scale, window
+        _p, _p, _sz, _p]),                       # out, workspace, bytes, stream
+    "ep_kv_bounds": (_c_int, [_tokens, _cache, _p, _p]),
+    "ep_kv_select_workspace": (_sz, [_tokens, _cache, _c_i64]),
+    "ep_kv_select": (_c_int, [_heads, _tokens, _cache, _p, _c_i64, _p, _p, _sz, _p]),
+    "ep_paged_attention_blocks_workspace": (_sz, [_heads, _tokens, _cache, _c_i64]),
+    "ep_paged_attention_blocks": (_c_int, [
+        _heads, _tokens, _cache, _p, _c_i64,     # q, tokens, cache, blocks, take
+        ctypes.c_float, _c_i64,                  # scale, window
+        _p, _p, _sz, _p]),                       # out, workspace, bytes, stream
+    # include/epure_draft.h
+    "ep_verify_draft_workspace": (_sz, [_draft]),
+    "ep_verify_draft": (_c_int, [_draft, _p, _p, _p, _sz, _p]),
 }
 
 XSRC_PLAIN, XSRC_RMSNORM, XSRC_SWIGLU = 0, 1, 2
@@ -149,7 +173,7 @@ TORCH_PATH = os.path.join(os.path.dirname(LIB_PATH), "epure_torch.so")
 
 
 def _load_call(handle):
-    """The extension that calls ``handle``'s matmul and paged-cache entry points on tensors."""
+    """The extension that calls ``handle``'s matmul, paged-cache and draft entry points on tensors."""
     loader = importlib.machinery.ExtensionFileLoader("epure_torch", TORCH_PATH)
     ext = importlib.util.module_from_spec(
         importlib.util.spec_from_file_location("epure_torch", TORCH_PATH, loader=loader))
@@ -159,6 +183,10 @@ def _load_call(handle):
              addr("ep_last_error"), getattr(torch._C, "_cuda_getCurrentRawStream", None))
     ext.bind_paged(addr("ep_rotate"), addr("ep_kv_append"), addr("ep_kv_read"),
                    addr("ep_paged_attention_workspace"), addr("ep_paged_attention"))
+    ext.bind_select(addr("ep_paged_attention_shared_workspace"), addr("ep_paged_attention_shared"), addr("ep_kv_bounds"),
+                    addr("ep_kv_select_workspace"), addr("ep_kv_select"),
+                    addr("ep_paged_attention_blocks_workspace"), addr("ep_paged_attention_blocks"))
+    ext.bind_draft(addr("ep_verify_draft_workspace"), addr("ep_verify_draft"))
     return ext
 
 

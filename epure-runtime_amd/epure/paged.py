@@ -18,6 +18,7 @@ raises.
 """
 import ctypes
 import math
+import operator
 
 import torch
 from torch.autograd import forward_ad
@@ -297,9 +298,14 @@ class PagedKVCache:
     position) stands for code * scale, its scale in ``k_scale`` / ``v_scale``
     ``[n_pages, heads, page]`` (float32).  ``page`` is a power of two from 16
     to 1024, D a multiple of 16 up to 256.  Nothing is derived through a
-    cache: a call that would have to raises."""
+    cache: a call that would have to raises.
 
-    def __init__(self, n_pages, page, heads, dim, dtype=torch.bfloat16, device="cuda"):
+    With ``bounds`` the cache keeps, in ``k_bounds`` ``[n_pages, heads, 2, D]``
+    (its own type; float32 in an 8-bit cache), the smallest and the largest
+    value of each column of a page's keys: ``append`` brings those of the pages
+    it writes up to date, ``select`` reads them."""
+
+    def __init__(self, n_pages, page, heads, dim, dtype=torch.bfloat16, device="cuda", bounds=False):
         if dtype not in _abi.CACHE_DT:
             raise TypeError(f"cache type {dtype} is not served: {[str(d) for d in _abi.CACHE_DT]}")
         shape = (n_pages, heads, page, dim)
@@ -308,16 +314,20 @@ class PagedKVCache:
                                   device=device).view(dtype)
         scales = [torch.ones(shape[:3], dtype=torch.float32, device=device) if dtype.itemsize == 1 else None
                   for _ in range(2)]
-        self._take(new(), new(), *scales)
+        limits = torch.zeros(n_pages, heads, 2, dim, dtype=dtype if dtype.itemsize == 2 else torch.float32,
+                             device=device) if bounds else None
+        self._take(new(), new(), *scales, limits)
 
     @classmethod
-    def of(cls, k, v, k_scale=None, v_scale=None):
-        """A cache over tensors that exist (shared, not copied)."""
+    def of(cls, k, v, k_scale=None, v_scale=None, k_bounds=None):
+        """A cache over tensors that exist (shared, not copied).  ``k_bounds``
+        are taken as they are: those of pages that hold rows already have to
+        be right."""
         self = cls.__new__(cls)
-        self._take(k, v, k_scale, v_scale)
+        self._take(k, v, k_scale, v_scale, k_bounds)
         return self
 
-    def _take(self, k, v, k_scale, v_scale):
+    def _take(self, k, v, k_scale, v_scale, k_bounds=None):
         if k.dtype not in _abi.CACHE_DT:
             raise TypeError(f"cache type {k.dtype} is not served: {[str(d) for d in _abi.CACHE_DT]}")
         if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
@@ -335,14 +345,18 @@ class PagedKVCache:
                 raise ValueError("8-bit caches have scales, 16-bit ones none")
             if scaled and (s.shape != k.shape[:3] or s.dtype != torch.float32 or s.device != k.device):
                 raise ValueError("scales must be float32 [n_pages, heads, page] on the cache's device")
-        for t in (k, v, k_scale, v_scale):
+        if k_bounds is not None and (k_bounds.shape != (n, h, 2, d) or k_bounds.device != k.device or
+                                     k_bounds.dtype != (torch.float32 if scaled else k.dtype)):
+            raise ValueError(f"bounds must be [n_pages, heads, 2, D] in {torch.float32 if scaled else k.dtype} "
+                             "on the cache's device")
+        for t in (k, v, k_scale, v_scale, k_bounds):
             if t is not None and (not t.is_contiguous() or t.data_ptr() % 16):
                 raise ValueError("cache tensors must be contiguous and 16-byte aligned")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.k, self.v, self.k_scale, self.v_scale, self.k_bounds = k, v, k_scale, v_scale, k_bounds
         self.n_pages, self.heads, self.page, self.dim, self.dtype = n, h, page, d, k.dtype
 
     def _held(self):
-        return self.k, self.v, self.k_scale, self.v_scale
+        return self.k, self.v, self.k_scale, self.v_scale, self.k_bounds
 
     def _cache(self):
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
@@ -356,12 +370,21 @@ class PagedKVCache:
         given, [B, S, q heads, D]) on its way out; returns q turned, or None
         without q.  A turned key is rounded once, to the cache's type.  Tokens
         of one call at the same place of a page race: what it holds then is
-        neither's for certain."""
+        neither's for certain.
+
+        Bounds, where the cache keeps them, are rebuilt for each page written,
+        from its rows up to the largest of the call's positions on it: a
+        sequence that goes back to an earlier position and appends from there
+        leaves no trace of what it held."""
         call = _native()
         if call is not None:
             cos, sin, inter = (None, None, False) if rotary is None else \
                 (rotary.cos, rotary.sin, rotary.layout == "interleaved")
-            r = call.append(k, v, positions, table, q, cos, sin, inter, self.k, self.v, self.k_scale, self.v_scale)
+            held = (self.k, self.v, self.k_scale, self.v_scale)
+            if self.k_bounds is None:
+                r = call.append(k, v, positions, table, q, cos, sin, inter, *held)
+            else:
+                r = call.append_bounds(k, v, positions, table, q, cos, sin, inter, *held, self.k_bounds)
             if r is not NotImplemented:
                 return r
         _no_grad(q, k, v, *self._held())
@@ -387,6 +410,10 @@ class PagedKVCache:
         _run("ep_kv_append", _abi.lib.ep_kv_append(
             _heads(q) if some_q else None, _heads(k), _heads(v), rotary._rotation() if rotary is not None else None,
             tok, self._cache(), qo.data_ptr() if some_q else None, _abi.stream_handle(k.device)))
+        if self.k_bounds is not None:
+            with torch.cuda.device(k.device):
+                _run("ep_kv_bounds", _abi.lib.ep_kv_bounds(tok, self._cache(), self.k_bounds.data_ptr(),
+                                                           _abi.stream_handle(k.device)))
         return qo
 
     def read(self, positions, table, dtype=torch.bfloat16):
@@ -411,39 +438,119 @@ class PagedKVCache:
                                                    _abi.dtype_code(dtype), _abi.stream_handle(k.device)))
         return k, v
 
-    def attend(self, q, positions, table, scale=None, window=None):
-        """Attention of q's tokens ([B, S, q heads, D], float16 or bfloat16)
-        over positions ``max(0, p - window + 1) .. p`` of their sequences, p
-        their own position (append them first); [B, S, q heads, D] in q's
-        type.  ``scale`` defaults to D ** -0.5, ``window`` to all.  A 16-bit
-        cache must have q's type.  Meant for one new token, or a few."""
-        call = _native()
-        if call is not None:
-            r = call.attend(q, positions, table, scale, window, self.k, self.v, self.k_scale, self.v_scale)
-            if r is not NotImplemented:
-                return r
-        _no_grad(q, *self._held())
-        _require(self.k, q, positions, table)
+    def _queries(self, q):
+        """q as the kernels read it: 16-byte aligned heads."""
         q = _heads4("q", q)
         if q.shape[3] != self.dim or q.shape[2] == 0 or q.shape[2] % self.heads:
             raise ValueError(f"q must be [B, S, n * {self.heads}, {self.dim}], got {tuple(q.shape)}")
         if q.dtype == torch.float32:
             raise TypeError("attention takes float16 or bfloat16 queries")
+        if q.data_ptr() % 16 or any(n > 1 and s % 8 for n, s in zip(q.shape[:3], q.stride()[:3])):
+            q = q.contiguous() if not q.is_contiguous() else q.clone()
+        return q
+
+    def select(self, q, positions, table, n):
+        """The n pages of each token's context that matter most to it, for
+        each cache head: int32 [B, S, heads, n], indices into the sequence's
+        row of the table, ascending, -1 behind the last where there are fewer.
+
+        A page's score is the largest that the sum of q . k over the query
+        heads of the cache head could be for keys within the page's bounds:
+        the sum over columns of ``hi * sum(max(q, 0)) + lo * sum(min(q, 0))``
+        (in float64; of equal scores the lower page, a NaN above all).  The page
+        of the token's own position is always taken, those behind it never.
+        The cache has to keep bounds (``bounds=True``), q is float16 or
+        bfloat16; ``attend(..., blocks=...)`` takes what is returned."""
+        if self.k_bounds is None:
+            raise ValueError("select needs a cache that keeps bounds (bounds=True)")
+        call = _native()
+        if call is not None:
+            r = call.select(q, positions, table, n, self.k, self.v, self.k_scale, self.v_scale, self.k_bounds)
+            if r is not NotImplemented:
+                return r
+        _no_grad(q, *self._held())
+        _require(self.k, q, positions, table)
+        n = operator.index(n)
+        if n < 1:
+            raise ValueError(f"select takes at least one page, got {n}")
+        q = self._queries(q)
+        tok, _keep = _tokens(q.shape[:2], positions, table)
+        blocks = torch.empty(*q.shape[:2], self.heads, n, dtype=torch.int32, device=q.device)
+        if blocks.numel() == 0:
+            return blocks
+        cache = self._cache()
+        with torch.cuda.device(q.device):
+            size = _abi.lib.ep_kv_select_workspace(tok, cache, n)
+            ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+            _run("ep_kv_select", _abi.lib.ep_kv_select(
+                _heads(q), tok, cache, self.k_bounds.data_ptr(), n, blocks.data_ptr(),
+                ws.data_ptr() if size else None, size, _abi.stream_handle(q.device)))
+        return blocks
+
+    def attend(self, q, positions, table, scale=None, window=None, shared=0, blocks=None):
+        """Attention of q's tokens ([B, S, q heads, D], float16 or bfloat16)
+        over positions ``max(0, p - window + 1) .. p`` of their sequences, p
+        their own position (append them first); [B, S, q heads, D] in q's
+        type.  ``scale`` defaults to D ** -0.5, ``window`` to all.  A 16-bit
+        cache must have q's type.  Meant for one new token, or a few.
+
+        ``shared``: the first so many pages are the same in every row of the
+        table (a prefix in common; those of row 0 are read).  They are computed
+        once for the whole batch instead of once a sequence.
+
+        ``blocks`` (int32 [B, S, heads, n]): each token sees only what lies on
+        these pages of its sequence, indices into its row of the table as
+        ``select`` gives them, in any order; negative ones, and ones past the
+        table, name none, one that is there twice counts twice, and a token
+        that sees no position gets zeros.  Not together with ``shared``."""
+        call = _native()
+        if call is not None:
+            held = (self.k, self.v, self.k_scale, self.v_scale)
+            if blocks is None and not shared:
+                r = call.attend(q, positions, table, scale, window, *held)
+            else:
+                r = call.attend_more(q, positions, table, scale, window, shared, blocks, *held)
+            if r is not NotImplemented:
+                return r
+        _no_grad(q, *self._held())
+        _require(self.k, q, positions, table, *(() if blocks is None else (blocks,)))
+        q = self._queries(q)
         if self.dtype.itemsize == 2 and q.dtype != self.dtype:
             raise TypeError(f"q is {q.dtype} over a cache of {self.dtype}")
         if window is not None and window < 1:
             raise ValueError(f"window must be positive, got {window}")
-        if q.data_ptr() % 16 or any(n > 1 and s % 8 for n, s in zip(q.shape[:3], q.stride()[:3])):
-            q = q.contiguous() if not q.is_contiguous() else q.clone()
         tok, _keep = _tokens(q.shape[:2], positions, table)
+        shared = operator.index(shared)
+        if not 0 <= shared <= tok.width:
+            raise ValueError(f"{shared} shared pages in a table of {tok.width}")
+        if blocks is not None:
+            if shared:
+                raise ValueError("shared pages and blocks are not served together")
+            if blocks.dtype != torch.int32:
+                raise TypeError(f"blocks must be int32, got {blocks.dtype}")
+            if blocks.dim() != 4 or blocks.shape[:3] != (*q.shape[:2], self.heads) or blocks.shape[3] < 1:
+                raise ValueError(f"blocks must be [{q.shape[0]}, {q.shape[1]}, {self.heads}, pages], "
+                                 f"got {tuple(blocks.shape)}")
+            blocks = blocks.contiguous()
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         if q.numel() == 0:
             return out
         qh, cache = _heads(q), self._cache()
-        n = _abi.lib.ep_paged_attention_workspace(qh, tok, cache)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        _run("ep_paged_attention", _abi.lib.ep_paged_attention(
-            qh, tok, cache, self.dim ** -0.5 if scale is None else float(scale),
-            min(int(window or 0), 2 ** 63 - 1), out.data_ptr(),     # 64 bits there: more would wrap
-            ws.data_ptr() if n else None, n, _abi.stream_handle(q.device)))
+        scale = self.dim ** -0.5 if scale is None else float(scale)
+        window = min(int(window or 0), 2 ** 63 - 1)     # 64 bits there: more would wrap
+        lib = _abi.lib
+        if blocks is not None:
+            n = blocks.shape[3]
+            name, which, want = "ep_paged_attention_blocks", (blocks.data_ptr(), n), lambda: \
+                lib.ep_paged_attention_blocks_workspace(qh, tok, cache, n)
+        elif shared:
+            name, which, want = "ep_paged_attention_shared", (shared,), lambda: \
+                lib.ep_paged_attention_shared_workspace(qh, tok, cache, shared)
+        else:
+            name, which, want = "ep_paged_attention", (), lambda: lib.ep_paged_attention_workspace(qh, tok, cache)
+        with torch.cuda.device(q.device):
+            size = want()
+            ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+            _run(name, getattr(lib, name)(qh, tok, cache, *which, scale, window, out.data_ptr(),
+                                          ws.data_ptr() if size else None, size, _abi.stream_handle(q.device)))
         return out

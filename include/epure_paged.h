@@ -134,6 +134,59 @@ size_t ep_paged_attention_workspace(const ep_heads *q, const ep_tokens *tokens, 
 int ep_paged_attention(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache, float scale,
                        int64_t window, void *out, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * The same attention for a batch whose tables begin with the same `shared`
+ * pages (0 .. width; those of sequence 0 are read, whatever the other rows
+ * name): these pages are computed once for the rows of the whole batch, then
+ * each sequence's own, and the two are joined.  Every token's position may lie
+ * in either.  At most 2^30 - 1 rows (tokens times query heads) on one cache
+ * head.  Workspace: as above.
+ */
+size_t ep_paged_attention_shared_workspace(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache,
+                                           int64_t shared);
+int ep_paged_attention_shared(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache, int64_t shared,
+                              float scale, int64_t window, void *out, void *workspace, size_t workspace_bytes,
+                              void *stream);
+
+/*
+ * Bounds of the keys a cache holds: bounds [n_pages][heads][2][D] (dense,
+ * 16-byte aligned; the cache's type, for 8-bit caches f32), the least and the
+ * largest value of each column over a page's rows.  After ep_kv_append of the
+ * same tokens: each page that one of them lies on gets those of its rows from
+ * 0 to the largest position of the call's tokens on it (a NaN among them is
+ * both).  Tokens that store nothing because of the page table change nothing.
+ */
+int ep_kv_bounds(const ep_tokens *tokens, const ep_kv_cache *cache, void *bounds, void *stream);
+
+/*
+ * blocks [B, S, q's cache heads, take] int32 (dense): for each token at position
+ * p and each cache head the pages of the sequence (indices into its row of the
+ * table, ascending, -1 behind the last) to attend to: page p / page, and of
+ * those before it the take - 1 of the largest score
+ *   sum_d hi_d sum_g max(q_gd, 0) + lo_d sum_g min(q_gd, 0),
+ * g over the query heads of the cache head, in 64 bits; of equal scores the
+ * lower page.  A score that is NaN, or of a page outside [0, n_pages), is above
+ * all.  Tokens of negative positions and of positions past the table: all -1.
+ * q: as in ep_paged_attention; its type need not be the cache's.  Workspace:
+ * ep_kv_select_workspace() bytes, 16-byte aligned.
+ */
+size_t ep_kv_select_workspace(const ep_tokens *tokens, const ep_kv_cache *cache, int64_t take);
+int ep_kv_select(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache, const void *bounds, int64_t take,
+                 int32_t *blocks, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * ep_paged_attention over the pages that blocks [B, S, cache heads, take]
+ * (int32, dense, take >= 1) names for each token and cache head, in any order:
+ * the positions max(0, p - window + 1) .. p on them.  An index that is
+ * negative, or not below the table's width, names none; one that is there
+ * twice counts twice.  A token that sees no position gets zeros.
+ */
+size_t ep_paged_attention_blocks_workspace(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache,
+                                           int64_t take);
+int ep_paged_attention_blocks(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache,
+                              const int32_t *blocks, int64_t take, float scale, int64_t window, void *out,
+                              void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -118,3 +118,64 @@ def attend_tolerance(out, mag, big, dtype, D):
     some thousand positions in blocks (2^-16 each): 2^-14 covers them."""
     delta = (D + 4) * 2.0 ** -24 * big
     return half_step(out, dtype) + (2.0 ** -14 + 2 * delta) * mag
+
+
+def bounds(rows):
+    """[2, D] of the keys [rows, D] of a page: least and largest of each column, NaN where there is one."""
+    return torch.stack((rows.amin(0), rows.amax(0)))
+
+
+def select(q, lim, positions, page, take):
+    """int32 [B, S, heads, take]: the pages to attend to.  ``lim`` [B, W, heads, 2, D]
+    are the bounds of each sequence's pages in order (NaN: a page that
+    the pool lacks)."""
+    q, lim = q.detach().cpu().double(), lim.detach().cpu().double()
+    B, S, H, D = q.shape
+    heads = lim.shape[2]
+    G = H // heads
+    out = torch.full((B, S, heads, take), -1, dtype=torch.int32)
+    for b in range(B):
+        for s in range(S):
+            p = int(positions[b, s])
+            if p < 0 or p // page >= lim.shape[1]:
+                continue
+            own = p // page
+            for h in range(heads):
+                rows = q[b, s, h * G:(h + 1) * G]
+                up, down = rows.clamp(min=0).sum(0), rows.clamp(max=0).sum(0)
+                score = (lim[b, :own, h, 1] * up + lim[b, :own, h, 0] * down).sum(-1).tolist()
+                best = sorted(range(own), key=lambda j: (score[j] == score[j], -score[j], j) if score[j] == score[j]
+                              else (False, 0.0, j))[:take - 1]
+                for i, j in enumerate(sorted(best) + [own]):
+                    out[b, s, h, i] = j
+    return out
+
+
+def attend_blocks(q, k, v, positions, blocks, page, scale, window=None):
+    """As ``attend``, over the positions on the pages that ``blocks`` [B, S,
+    heads, n] names for each token and cache head: (output, sum of weight *
+    |v|, largest sum of |q k| times scale)."""
+    q, k, v = (t.detach().cpu().double() for t in (q, k, v))
+    B, S, H, D = q.shape
+    G, L = H // k.shape[2], k.shape[1]
+    out, mag = torch.zeros_like(q), torch.zeros_like(q)
+    big = torch.zeros(B, S, H, 1, dtype=torch.float64)
+    for b in range(B):
+        for s in range(S):
+            p = int(positions[b, s])
+            if p < 0:
+                continue
+            if p >= L:
+                out[b, s] = math.nan
+                continue
+            lo = max(0, p - window + 1) if window else 0
+            for h in range(H):
+                at = [j for i in blocks[b, s, h // G].tolist() if 0 <= i < L // page
+                      for j in range(max(i * page, lo), min((i + 1) * page, p + 1))]
+                if not at:
+                    continue
+                kk, vv = k[b, at, h // G], v[b, at, h // G]
+                w = torch.softmax(kk @ q[b, s, h] * scale, 0)
+                out[b, s, h], mag[b, s, h] = w @ vv, w @ vv.abs()
+                big[b, s, h] = (kk.abs() @ q[b, s, h].abs()).max() * abs(scale)
+    return out, mag, big
