@@ -5,7 +5,7 @@
 
 #include <algorithm>
 
-#include "attend_kernel.h"
+#include "attend_front.h"
 
 namespace ep {
 namespace {
@@ -101,13 +101,16 @@ __global__ void __launch_bounds__(256) join_parts_kernel(AttendParts a, int RM)
     const OutRow o = out_row_of(a);
     const uint32_t H = a.c.heads;
     const uint32_t row = o.s * a.G + o.gq, block = row / RM, r = row - block * RM;
-    const uint32_t all = o.token * a.G + o.gq, front = all / RM, rf = all - front * RM;
+    const uint32_t all = o.token * a.G + o.gq, rows_f = a.front ? RM : kFrontRows, front = all / rows_f, rf = all - front * rows_f;
     const uint32_t seg = (a.front + o.b * a.blocks + block) * H + o.h, seg_f = front * H + o.h;
     const int2 d = a.workers ? a.desc[seg] : make_int2((int)seg, 1);
-    const int2 f = a.workers ? a.desc[seg_f] : make_int2((int)seg_f, 1);
+    const int2 f = !a.front ? make_int2(0, a.front_splits) : a.workers ? a.desc[seg_f] : make_int2((int)seg_f, 1);
     const int p = attend_position(a, o.b, o.s);
     join_row<OP>(a, o.row, p, d.y + f.y, [&](int k) {
-        return (k < d.y ? piece_slot(d, k) : piece_slot(f, k - d.y)) * a.slot_rows + (k < d.y ? r : rf);
+        if (k < d.y)
+            return piece_slot(d, k) * a.slot_rows + r;
+        k -= d.y;
+        return a.front ? piece_slot(f, k) * a.slot_rows + rf : a.front_at + ((int64_t)seg_f * a.front_splits + k) * kFrontRows + rf;
     }, __uint_as_float(0x7fc00000u));
 }
 
@@ -238,29 +241,59 @@ struct PartsPlan {
     int64_t blocks, front, segments;
     size_t desc, ml, o;
     int slot_rows;
+    int64_t groups, splits, slots;       // of attend_front.h (groups 0: not used); slots of the others
 };
 
+// Pieces that the shared positions are cut into for `groups` row groups of all
+// cache heads: the fewest that fill the compute units' one workgroup each to nine
+// tenths, round by round, of two stages at least.
+int64_t front_splits(int64_t groups, int64_t stages)
+{
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(stages / 2, 256));
+    int64_t best = 1;
+    double best_full = 0.0;
+    for (int64_t s = 1; s <= most; ++s) {
+        const int64_t n = groups * s;
+        const double full = (double)n / (double)(256 * ((n + 255) / 256));
+        if (full > best_full) {
+            best = s;
+            best_full = full;
+        }
+        if (full >= 0.9)
+            break;
+    }
+    return best;
+}
+
 // Units of the whole batch over the shared pages, then the sequences' own:
-// as plan() does, but that every segment leaves a part.
+// as plan() does, but that every segment leaves a part.  More rows than one unit
+// takes go through LDS (attend_front.h).
 PartsPlan plan_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared, int64_t window)
 {
     PartsPlan p{};
     const int64_t rows = tok.S * (q->heads / c.heads), all = tok.B * rows;
-    p.mt = all <= 16 ? 1 : 2;
+    const bool dense = all > 32;
+    p.mt = (dense ? rows : all) <= 16 ? 1 : 2;
     const int64_t rm = 16 * p.mt;
     p.blocks = (rows + rm - 1) / rm;
-    p.front = (all + rm - 1) / rm;
+    p.front = dense ? 0 : (all + rm - 1) / rm;
     p.segments = (p.front + tok.B * p.blocks) * c.heads;
-    p.slot_rows = (int)std::min(all, rm);
-    const int64_t tiles = (std::max(shared, tok.width - shared) << c.page_shift) / kAttTile + 1;
+    p.slot_rows = (int)std::min(dense ? rows : all, rm);
+    if (dense) {
+        const int64_t tp = front_stage(front_steps(c.D), row_bytes(c) == c.D);
+        p.groups = (all + kFrontRows - 1) / kFrontRows;
+        p.splits = front_splits(p.groups * c.heads, ((shared << c.page_shift) + tp - 1) / tp);
+    }
+    const int64_t tiles = ((dense ? tok.width - shared : std::max(shared, tok.width - shared)) << c.page_shift) / kAttTile + 1;
     const int64_t most = window > 0 && window <= tiles * kAttTile
                              ? std::min(tiles, (window + tok.S) / kAttTile + 2) : tiles;
     if (most > std::min<int64_t>(16 + p.segments / 8, 32) && p.segments < 0x40000000 && tiles + kMostPiece < 0x7fff0000 / p.segments)
         p.workers = 256 * attend_occupancy(attend_columns(c.D), p.mt, c.dtype != EP_I8);
-    const size_t slots = ((size_t)2 * p.workers + p.segments) * p.slot_rows;
+    p.slots = ((int64_t)2 * p.workers + p.segments) * p.slot_rows;
+    const size_t part_rows = (size_t)p.slots + (size_t)p.groups * c.heads * p.splits * kFrontRows;
     p.desc = p.workers ? up16(p.segments * sizeof(int2)) : 0;
-    p.ml = up16(slots * sizeof(float2));
-    p.o = slots * c.D * sizeof(float);
+    p.ml = up16(part_rows * sizeof(float2));
+    p.o = part_rows * c.D * sizeof(float);
     return p;
 }
 
@@ -392,6 +425,32 @@ int launch_attend_parts(const ep_heads *q, const PagedTokens &tok, const PagedCa
     a.few = p.workers;
     a.piece = piece_tiles(c, p.workers);
     a.slot_rows = p.slot_rows;
+    a.front_splits = (int)p.splits;
+    a.front_at = p.slots;
+    if (p.groups) {
+        FrontArgs f{};
+        f.q = a.q;
+        f.q_sb = a.q_sb;
+        f.q_ss = a.q_ss;
+        f.q_sh = a.q_sh;
+        f.tok = tok;
+        f.c = c;
+        f.scale = a.scale;
+        f.window = a.window;
+        f.cap = a.cap;
+        f.G = a.G;
+        f.rows = a.front_rows;
+        f.limit = a.from;
+        f.groups = (int)p.groups;
+        f.splits = (int)p.splits;
+        f.part_ml = a.part_ml + p.slots;
+        f.part_o = a.part_o + p.slots * c.D;
+        const int64_t pairs = (int64_t)c.heads * p.splits;
+        rc = in_launches((pairs + 7) / 8 * 8 * p.groups, 64 * front_waves(front_steps(c.D)), f,
+                         [&](const FrontArgs &part, unsigned n) { attend_front(part, q->dtype, n, stream); });
+        if (rc != EP_OK)
+            return rc;
+    }
     const int64_t grid = p.workers ? p.workers : p.segments;
     rc = in_launches(grid, 64 * kAttWaves, a, [&](const AttendParts &part, unsigned n) {
         attend_parts(part, q->dtype, p.mt, n, stream);

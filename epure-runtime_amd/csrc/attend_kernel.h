@@ -81,7 +81,8 @@ struct AttendArgs {
 //   kParts: the tables' first `shared` pages are those of sequence 0.  The
 //     first `front` units are rows of the whole batch, over those pages; the
 //     rest is as in kWhole, over the pages behind them, positions counted
-//     from there.  Every output stays a part: the join adds them up;
+//     from there.  Every output stays a part: the join adds them up (more than
+//     32 rows a cache head over the shared pages are attend_front.h's);
 //   kBlocks: a unit is up to 16 rows of one token, and tile after tile goes
 //     over the `take` pages that a list names for it, in `cuts` equal pieces.
 enum AttendMode { kWhole, kParts, kBlocks };
@@ -93,6 +94,8 @@ struct AttendParts : AttendArgs {
     static constexpr AttendMode kMode = kParts;
     int front, front_rows;   // units over the shared pages; query rows of the batch on one cache head
     int shared, from;        // pages, and positions in them
+    int front_splits;        // front 0: pieces that attend_front.h cut the shared positions into,
+    int64_t front_at;        // and where they begin among the parts' rows
 };
 struct AttendBlocks : AttendArgs {
     static constexpr AttendMode kMode = kBlocks;
