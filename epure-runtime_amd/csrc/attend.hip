@@ -245,21 +245,21 @@ struct PartsPlan {
 };
 
 // Pieces that the shared positions are cut into for `groups` row groups of all
-// cache heads: the fewest that fill the compute units' one workgroup each to nine
-// tenths, round by round, of two stages at least.
-int64_t front_splits(int64_t groups, int64_t stages)
+// cache heads: the fewest that fill the room for workgroups, round by round (else
+// those that fill it best), of two stages at least.
+int64_t front_splits(int64_t groups, int64_t stages, int64_t room)
 {
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(stages / 2, 256));
     int64_t best = 1;
     double best_full = 0.0;
     for (int64_t s = 1; s <= most; ++s) {
         const int64_t n = groups * s;
-        const double full = (double)n / (double)(256 * ((n + 255) / 256));
+        const double full = (double)n / (double)(room * ((n + room - 1) / room));
         if (full > best_full) {
             best = s;
             best_full = full;
         }
-        if (full >= 0.9)
+        if (full >= 0.97)
             break;
     }
     return best;
@@ -280,9 +280,9 @@ PartsPlan plan_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache
     p.segments = (p.front + tok.B * p.blocks) * c.heads;
     p.slot_rows = (int)std::min(dense ? rows : all, rm);
     if (dense) {
-        const int64_t tp = front_stage(front_steps(c.D), row_bytes(c) == c.D);
+        const int64_t tp = kFrontStage;
         p.groups = (all + kFrontRows - 1) / kFrontRows;
-        p.splits = front_splits(p.groups * c.heads, ((shared << c.page_shift) + tp - 1) / tp);
+        p.splits = front_splits(p.groups * c.heads, ((shared << c.page_shift) + tp - 1) / tp, 256 * front_occupancy(front_steps(c.D)));
     }
     const int64_t tiles = ((dense ? tok.width - shared : std::max(shared, tok.width - shared)) << c.page_shift) / kAttTile + 1;
     const int64_t most = window > 0 && window <= tiles * kAttTile
@@ -446,7 +446,7 @@ int launch_attend_parts(const ep_heads *q, const PagedTokens &tok, const PagedCa
         f.part_ml = a.part_ml + p.slots;
         f.part_o = a.part_o + p.slots * c.D;
         const int64_t pairs = (int64_t)c.heads * p.splits;
-        rc = in_launches((pairs + 7) / 8 * 8 * p.groups, 64 * front_waves(front_steps(c.D)), f,
+        rc = in_launches((pairs + 7) / 8 * 8 * p.groups, 64 * kFrontWaves, f,
                          [&](const FrontArgs &part, unsigned n) { attend_front(part, q->dtype, n, stream); });
         if (rc != EP_OK)
             return rc;
