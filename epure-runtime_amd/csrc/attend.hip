@@ -247,8 +247,9 @@ struct PartsPlan {
 // Pieces that the shared positions are cut into for `groups` row groups of all
 // cache heads: the fewest that fill the room for workgroups, round by round (else
 // those that fill it best), of two stages at least.
-int64_t front_splits(int64_t groups, int64_t stages, int64_t room)
+int64_t front_splits(int64_t groups, int64_t stages)
 {
+    const int64_t room = 256 * kFrontOccupancy;
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(stages / 2, 256));
     int64_t best = 1;
     double best_full = 0.0;
@@ -265,14 +266,27 @@ int64_t front_splits(int64_t groups, int64_t stages, int64_t room)
     return best;
 }
 
+// Whether the shared pages go through LDS (attend_front.h).  That costs a launch
+// and some 14 us more before and behind the products, which then go 2.5 times
+// as fast (8-bit rows 1.6): 32 x 4 rows on 8 heads over 8192 positions, 8192 tiles
+// of 32 by 32, take 38 us as units and 41 so; 128 x 4 over 16384 int8 positions,
+// 65536 tiles, 134 and 101; 64 x 4 over 65536, 131072 tiles, 351 and 180.
+bool through_lds(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared, int64_t window)
+{
+    const int64_t all = tok.B * tok.S * (q->heads / c.heads);
+    int64_t seen = shared << c.page_shift;
+    if (window > 0)
+        seen = std::min(seen, window);
+    return all > 32 && c.D <= kFrontWidest && (all + 31) / 32 * c.heads >= 16384 / std::max<int64_t>(seen / kAttTile, 1);
+}
+
 // Units of the whole batch over the shared pages, then the sequences' own:
-// as plan() does, but that every segment leaves a part.  More rows than one unit
-// takes go through LDS (attend_front.h).
-PartsPlan plan_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared, int64_t window)
+// as plan() does, but that every segment leaves a part.  dense: the former go
+// through LDS instead.
+PartsPlan plan_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared, int64_t window, bool dense)
 {
     PartsPlan p{};
     const int64_t rows = tok.S * (q->heads / c.heads), all = tok.B * rows;
-    const bool dense = all > 32;
     p.mt = (dense ? rows : all) <= 16 ? 1 : 2;
     const int64_t rm = 16 * p.mt;
     p.blocks = (rows + rm - 1) / rm;
@@ -280,9 +294,8 @@ PartsPlan plan_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache
     p.segments = (p.front + tok.B * p.blocks) * c.heads;
     p.slot_rows = (int)std::min(dense ? rows : all, rm);
     if (dense) {
-        const int64_t tp = kFrontStage;
         p.groups = (all + kFrontRows - 1) / kFrontRows;
-        p.splits = front_splits(p.groups * c.heads, ((shared << c.page_shift) + tp - 1) / tp, 256 * front_occupancy(front_steps(c.D)));
+        p.splits = front_splits(p.groups * c.heads, ((shared << c.page_shift) + kFrontStage - 1) / kFrontStage);
     }
     const int64_t tiles = ((dense ? tok.width - shared : std::max(shared, tok.width - shared)) << c.page_shift) / kAttTile + 1;
     const int64_t most = window > 0 && window <= tiles * kAttTile
@@ -338,8 +351,13 @@ size_t attend_parts_workspace(const ep_heads *q, const PagedTokens &tok, const P
 {
     if (!shares(tok, shared) || tok.S == 0)
         return attend_workspace(q, tok, c);
-    const PartsPlan p = plan_parts(q, tok, c, shared, 0);
-    return p.desc + p.ml + p.o;
+    // a window may turn the choice
+    size_t most = 0;
+    for (const bool dense : {false, through_lds(q, tok, c, shared, 0)}) {
+        const PartsPlan p = plan_parts(q, tok, c, shared, 0, dense);
+        most = std::max(most, p.desc + p.ml + p.o);
+    }
+    return most;
 }
 
 size_t attend_blocks_workspace(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t take)
@@ -404,7 +422,7 @@ int launch_attend_parts(const ep_heads *q, const PagedTokens &tok, const PagedCa
 {
     if (!shares(tok, shared))
         return launch_attend(q, tok, c, scale, window, out, ws, ws_bytes, stream);
-    const PartsPlan p = plan_parts(q, tok, c, shared, window);
+    const PartsPlan p = plan_parts(q, tok, c, shared, window, through_lds(q, tok, c, shared, window));
     const int64_t rows = tok.S * (q->heads / c.heads), rm = 16 * p.mt;
     const int64_t out_rows = tok.B * tok.S * q->heads;
     if (too_many_rows(tok.B * rows, p.segments + 2 * p.workers, out_rows))

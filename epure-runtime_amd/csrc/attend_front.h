@@ -37,8 +37,9 @@ struct FrontArgs {
 
 constexpr int kFrontWaves = 4, kFrontStage = 64;
 
-// Workgroups that a compute unit holds: by registers and LDS.
-constexpr int front_occupancy(int KS) { return KS <= 4 ? 2 : 1; }
+// Workgroups that a compute unit holds: by registers and LDS, which is why
+// wider heads are not taken here.
+constexpr int kFrontOccupancy = 2, kFrontWidest = 128;
 
 // How far (in powers of two) a row's weights may outgrow the maximum that they
 // are taken relative to before sums and maximum are brought up to date: most
@@ -51,7 +52,7 @@ constexpr float front_slack(float shift) { return shift == 0.0f ? 8.0f : 4.0f; }
 template <int KS>
 EP_DEV int front_chunk(int r, int c)
 {
-    return c ^ (KS % 4 == 0 ? r & 15 : KS == 3 ? (r >> 2) & 3 : (r >> 1) & 7);
+    return c ^ (KS == 4 ? r & 15 : KS == 3 ? (r >> 2) & 3 : (r >> 1) & 7);
 }
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -63,7 +64,7 @@ EP_DEV void lds_rows(const void *p, uint32_t bytes, uint16_t *lds, int off)
 }
 
 template <typename QOP, int CODE, int KS>
-__global__ void __launch_bounds__(64 * kFrontWaves, front_occupancy(KS)) front_kernel(FrontArgs a)
+__global__ void __launch_bounds__(64 * kFrontWaves, kFrontOccupancy) front_kernel(FrontArgs a)
 {
     constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
     constexpr int ES = k8 ? 1 : 2, NC = 2 * KS, DM = 32 * KS, TP = kFrontStage, NT = TP / 16;
@@ -206,11 +207,6 @@ __global__ void __launch_bounds__(64 * kFrontWaves, front_occupancy(KS)) front_k
     constexpr float kSlack = front_slack(VOP::kShift), kShift = VOP::kShift == 0.0f ? 0.0f : VOP::kShift - kSlack;
     float m[2], l[2];
     f32x4_t o[2][NC];
-    // Outputs that a value which is not finite has reached: written into the
-    // sums where it happens, or, in wide heads, a bit each (the sums' registers
-    // do not fit twice: 76 of 256 values would go through memory).
-    constexpr bool kHitsApart = KS > 4;
-    uint32_t hit[2][(NC + 7) / 8] = {};
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
         m[mt] = -INFINITY;
@@ -394,10 +390,7 @@ __global__ void __launch_bounds__(64 * kFrontWaves, front_occupancy(KS)) front_k
                             const f32x4_t hits = VOP::mfma(bad, one[mt], (f32x4_t){0, 0, 0, 0});
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                if constexpr (kHitsApart)
-                                    hit[mt][c / 8] |= (hits[i] > 0.0f ? 1u : 0u) << (4 * (c % 8) + i);
-                                else
-                                    o[mt][c][i] = hits[i] > 0.0f ? nan : o[mt][c][i];
+                                o[mt][c][i] = hits[i] > 0.0f ? nan : o[mt][c][i];
                         }
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt)
@@ -442,8 +435,12 @@ __global__ void __launch_bounds__(64 * kFrontWaves, front_occupancy(KS)) front_k
         next_id = page_of(j + x + 2);
         scores(is_odd, j + x);
         softmax(cuts, is_odd);
+        // what looks for values that are not finite takes the registers of the rows on their way
+        if (decltype(cuts)::value)
+            end_rows(other);
         sums(cuts, is_odd);
-        end_rows(other);
+        if (!decltype(cuts)::value)
+            end_rows(other);
         __syncthreads();             // the next stage is there, and this one's readers are done
     };
     if (count > 0) {
@@ -488,35 +485,23 @@ __global__ void __launch_bounds__(64 * kFrontWaves, front_occupancy(KS)) front_k
         for (int c = 0; c < NC; ++c) {
             f32x4_t z;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 4; ++i)
                 z[i] = o[mt][c][i] * up;
-                if constexpr (kHitsApart)
-                    z[i] = hit[mt][c / 8] >> (4 * (c % 8) + i) & 1 ? nan : z[i];
-            }
             if (16 * c < D)
                 *(f32x4_t *)(a.part_o + at * D + 16 * c + 4 * g) = z;
         }
     }
 }
 
-// Steps of 32 values that a kernel takes for heads of D values.
-constexpr int front_steps(int D) { return D <= 64 ? 2 : D <= 96 ? 3 : D <= 128 ? 4 : D <= 192 ? 6 : 8; }
-
-template <typename QOP, int CODE, int KS>
-void front_sized(const FrontArgs &a, unsigned grid, hipStream_t st)
-{
-    front_kernel<QOP, CODE, KS><<<grid, 64 * kFrontWaves, 0, st>>>(a);
-}
 template <typename QOP, int CODE>
 void front_by_size(const FrontArgs &a, unsigned grid, hipStream_t st)
 {
-    switch (front_steps(a.c.D)) {
-    case 2: return front_sized<QOP, CODE, 2>(a, grid, st);
-    case 3: return front_sized<QOP, CODE, 3>(a, grid, st);
-    case 4: return front_sized<QOP, CODE, 4>(a, grid, st);
-    case 6: return front_sized<QOP, CODE, 6>(a, grid, st);
-    default: return front_sized<QOP, CODE, 8>(a, grid, st);
-    }
+    if (a.c.D <= 64)
+        front_kernel<QOP, CODE, 2><<<grid, 64 * kFrontWaves, 0, st>>>(a);
+    else if (a.c.D <= 96)
+        front_kernel<QOP, CODE, 3><<<grid, 64 * kFrontWaves, 0, st>>>(a);
+    else
+        front_kernel<QOP, CODE, 4><<<grid, 64 * kFrontWaves, 0, st>>>(a);
 }
 
 void attend_front(const FrontArgs &a, int q_dtype, unsigned grid, hipStream_t st);
