@@ -316,15 +316,18 @@ struct BlocksPlan {
     size_t desc, ml, o;
 };
 
-// A list's tiles are cut into as many pieces as fill the compute units twice,
-// of eight tiles at least (two a wave).
+// A list of few tiles goes to a workgroup as a whole (as in plan(): 16, or up
+// to 32 the more lists there are); else it is cut into as many pieces as fill the
+// compute units twice, of eight tiles at least (two a wave).
 BlocksPlan plan_blocks(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t take)
 {
     BlocksPlan p{};
     const int64_t G = q->heads / c.heads, tiles = (take * c.page + kAttTile - 1) / kAttTile;
     p.blocks = (G + 15) / 16;
     p.segments = tok.B * tok.S * p.blocks * c.heads;
-    p.cuts = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(p.segments, 1), tiles / (2 * kAttWaves)));
+    p.cuts = 1;
+    if (tiles > std::min<int64_t>(16 + p.segments / 8, 32))
+        p.cuts = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(p.segments, 1), tiles / (2 * kAttWaves)));
     p.slot_rows = (int)std::min<int64_t>(G, 16);
     if (p.cuts > 1) {
         const size_t slots = (size_t)p.segments * p.cuts * p.slot_rows;

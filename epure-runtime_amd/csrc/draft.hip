@@ -10,7 +10,8 @@
 // Bound by the bytes of one row of the vocabulary a sequence (of p, and of q
 // where a token was turned down): a row is cut into pieces of 4096 values, and
 // as many workgroups sum them; a second launch finds the piece in which the sum
-// is passed and looks at it again.
+// is passed and looks at it again.  Which tokens stand every workgroup of the
+// first launch finds out by itself (a few loads).
 #include "ep_common.h"
 #include "ep_draft.h"
 #include "ep_internal.h"
@@ -24,6 +25,7 @@ struct DraftArgs {
     DraftTensors t;
     int64_t *accepted, *tokens;
     double2 *part;           // [B][pieces]: sum of r, sum of p
+    int64_t *ends;           // [B][2]: drafted tokens that stand; the one turned down, or -1
     uint32_t first_wg, pieces;
 };
 
@@ -115,6 +117,10 @@ __global__ void __launch_bounds__(256) sum_kernel(DraftArgs a)
             sum.y += s_sum[w].y;
         }
         a.part[(int64_t)b * a.pieces + piece] = sum;
+        if (piece == 0) {
+            a.ends[2 * (int64_t)b] = k;
+            a.ends[2 * (int64_t)b + 1] = x;
+        }
     }
 }
 
@@ -178,8 +184,8 @@ __global__ void __launch_bounds__(256) pick_kernel(DraftArgs a)
     const uint32_t b = a.first_wg + blockIdx.x;
     const int tid = threadIdx.x;
     const DraftTensors &t = a.t;
-    int64_t x;
-    const int k = stand<T>(t, b, x);
+    const int k = (int)a.ends[2 * (int64_t)b];
+    const int64_t x = a.ends[2 * (int64_t)b + 1];
     const double2 *part = a.part + (int64_t)b * a.pieces;
 
     // thread i has pieces [i per, (i + 1) per)
@@ -269,7 +275,7 @@ int64_t pieces_of(int64_t V) { return (V + kPiece - 1) / kPiece; }
 
 }  // namespace
 
-size_t verify_workspace(int64_t B, int64_t V) { return (size_t)B * pieces_of(V) * sizeof(double2); }
+size_t verify_workspace(int64_t B, int64_t V) { return (size_t)B * (pieces_of(V) + 1) * sizeof(double2); }
 
 int launch_verify(const DraftTensors &t, int64_t B, int dtype, int64_t *accepted, int64_t *tokens, void *ws,
                   size_t ws_bytes, hipStream_t stream)
@@ -277,7 +283,8 @@ int launch_verify(const DraftTensors &t, int64_t B, int dtype, int64_t *accepted
     const size_t want = verify_workspace(B, t.V);
     if (ws_bytes < want || !ws)
         return set_error(EP_ERR_WORKSPACE, "verification: workspace of %zu bytes, %zu wanted", ws_bytes, want);
-    DraftArgs a{t, accepted, tokens, (double2 *)ws, 0, (uint32_t)pieces_of(t.V)};
+    double2 *const part = (double2 *)ws;
+    DraftArgs a{t, accepted, tokens, part, (int64_t *)(part + B * pieces_of(t.V)), 0, (uint32_t)pieces_of(t.V)};
     if (B > 0x7fffffff / (int64_t)a.pieces)
         return set_error(EP_DECLINE_SHAPE, "%lld sequences over %lld tokens are more than one call takes", (long long)B,
                          (long long)t.V);

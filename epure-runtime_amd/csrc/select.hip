@@ -23,6 +23,7 @@ namespace {
 constexpr int kChunkTokens = 64;    // tokens a workgroup of the bounds looks over
 constexpr int kChunkPages = 128;    // pages a workgroup scores
 constexpr int kHeldKeys = 4096;     // scores that the choice keeps in LDS (32 KiB)
+constexpr int kFewPages = 512;      // of a table whose rows one workgroup each scores and chooses from
 
 struct BoundsArgs {
     PagedTokens tok;
@@ -85,9 +86,16 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
         const int64_t mine = __shfl(p, l, 64), page = mine >> a.c.page_shift, who = (int64_t)chunk * kChunkTokens + l;
         if (a.tok.S > 1) {
             int later = 0;
-            for (int64_t t = tid; t < a.tok.S; t += 256) {
-                const int64_t o = pos[t * ps];
-                later |= o >= 0 && o >> a.c.page_shift == page && (o > mine || (o == mine && t > who));
+            for (int64_t t0 = tid; t0 < a.tok.S; t0 += 8 * 256) {
+                int64_t o[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)      // eight loads in flight; past the end the first again
+                    o[i] = pos[(t0 + 256 * i < a.tok.S ? t0 + 256 * i : t0) * ps];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t t = t0 + 256 * i < a.tok.S ? t0 + 256 * i : t0;
+                    later |= o[i] >= 0 && o[i] >> a.c.page_shift == page && (o[i] > mine || (o[i] == mine && t > who));
+                }
             }
             if (__syncthreads_or(later))
                 continue;
@@ -223,6 +231,73 @@ struct Bounds8 {
     }
 };
 
+// Keys of pages [page0, page1) of a row, by the workgroup's threads: `put(page, key)`.
+template <bool WIDE, typename PUT>
+EP_DEV void score_pages(const SelectArgs &a, const SelectRow &row, int64_t page0, int64_t page1, PUT put)
+{
+    const int L = a.lanes, tid = threadIdx.x, u = tid & (L - 1), D = a.c.D;
+    const bool in = 8 * u < D;
+    const int d = in ? 8 * u : 0;
+    const int32_t *table = a.tok.table + row.b * a.tok.table_stride;
+    const int step = (int)blockDim.x / L;
+    int64_t k0 = page0 + tid / L;
+    int32_t id[2];
+    auto load_ids = [&]() {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)      // past the end some page of the row's
+            id[k] = table[k0 + k * step < page1 ? k0 + k * step : page0];
+    };
+    load_ids();
+    // this lane's eight columns of the group's queries, four heads in flight
+    double up[8], down[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        up[i] = down[i] = 0.0;
+    const char *q = (const char *)a.q + 2 * (row.b * a.q_sb + row.s * a.q_ss + (int64_t)row.h * a.G * a.q_sh + d);
+    for (int g0 = 0; g0 < a.G; g0 += 4) {
+        u32x4_t w[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            w[g] = *(const u32x4_t *)(q + 2 * (g0 + g < a.G ? g0 + g : g0) * a.q_sh);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            if (g0 + g < a.G)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint16_t x = (uint16_t)(w[g][i / 2] >> (16 * (i % 2)));
+                    const float v = a.q_dtype == EP_F16 ? (float)f16_from_bits(x) : bf16_to_f32(x);
+                    // a NaN reaches both sums
+                    up[i] += v < 0.0f ? 0.0 : (double)v;
+                    down[i] += v > 0.0f ? 0.0 : (double)v;
+                }
+    }
+    const bool f16 = a.c.dtype == EP_F16;
+    while (k0 < page1) {
+        Bounds8<WIDE> lo[2], hi[2];
+        bool ok[2];
+        const int64_t at = k0;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            ok[k] = id[k] >= 0 && id[k] < a.c.n_pages;
+            const int64_t src = ((int64_t)(ok[k] ? id[k] : 0) * a.c.heads + row.h) * 2 * D + d;
+            lo[k].load(a.bounds, src);
+            hi[k].load(a.bounds, src + D);
+        }
+        k0 += 2 * step;
+        load_ids();      // of the next round, while this one's bounds are on their way
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                sum = fma((double)lo[k].at(i, f16), down[i], fma((double)hi[k].at(i, f16), up[i], sum));
+            sum = lanes_sum(in ? sum : 0.0, L);
+            if (u == 0 && at + k * step < page1)
+                put(at + k * step, ok[k] ? order_key(sum) : ~0ull);
+        }
+    }
+}
+
 template <bool WIDE>
 __global__ void __launch_bounds__(256) score_kernel(SelectArgs a)
 {
@@ -231,61 +306,15 @@ __global__ void __launch_bounds__(256) score_kernel(SelectArgs a)
     const int64_t page0 = (int64_t)chunk * kChunkPages, page1 = page0 + kChunkPages < row.own ? page0 + kChunkPages : row.own;
     if (row.own < a.take || page0 >= page1)      // all pages are taken, or none of these is asked about
         return;
-    const int L = a.lanes, tid = threadIdx.x, u = tid & (L - 1), D = a.c.D;
-    const bool in = 8 * u < D;
-    const int d = in ? 8 * u : 0;
-    // this lane's eight columns of the group's queries
-    double up[8], down[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        up[i] = down[i] = 0.0;
-    for (int g = 0; g < a.G; ++g) {
-        const int64_t src = row.b * a.q_sb + row.s * a.q_ss + (int64_t)(row.h * a.G + g) * a.q_sh + d;
-        uint16_t w[8];
-        __builtin_memcpy(w, __builtin_assume_aligned((const uint16_t *)a.q + src, 16), 16);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = a.q_dtype == EP_F16 ? (float)f16_from_bits(w[i]) : bf16_to_f32(w[i]);
-            // a NaN reaches both sums
-            up[i] += v < 0.0f ? 0.0 : (double)v;
-            down[i] += v > 0.0f ? 0.0 : (double)v;
-        }
-    }
-    const int32_t *table = a.tok.table + row.b * a.tok.table_stride;
     uint64_t *keys = a.keys + (int64_t)r * a.tok.width;
-    const int step = 256 / L;
-    const bool f16 = a.c.dtype == EP_F16;
-    for (int64_t k0 = page0 + tid / L; k0 < page1; k0 += 2 * step) {
-        int32_t id[2];
-        Bounds8<WIDE> lo[2], hi[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int64_t page = k0 + k * step;
-            id[k] = table[page < page1 ? page : k0];
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const bool ok = id[k] >= 0 && id[k] < a.c.n_pages;
-            const int64_t src = ((int64_t)(ok ? id[k] : 0) * a.c.heads + row.h) * 2 * D + d;
-            lo[k].load(a.bounds, src);
-            hi[k].load(a.bounds, src + D);
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            double sum = 0.0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                sum = fma((double)lo[k].at(i, f16), down[i], fma((double)hi[k].at(i, f16), up[i], sum));
-            sum = lanes_sum(in ? sum : 0.0, L);
-            const int64_t page = k0 + k * step;
-            if (u == 0 && page < page1)
-                keys[page] = id[k] >= 0 && id[k] < a.c.n_pages ? order_key(sum) : ~0ull;
-        }
-    }
+    score_pages<WIDE>(a, row, page0, page1, [&](int64_t page, uint64_t key) { keys[page] = key; });
 }
 
-// Exclusive sum over the workgroup's 256 threads of two counts.
-EP_DEV uint2 exclusive_sums(uint32_t x, uint32_t y, uint2 *s_part, uint2 &total)
+constexpr int kChoose = 512;        // threads of a row's choice
+constexpr int kChooseWaves = kChoose / 64, kDigits = 2048;
+
+// Exclusive sums over the workgroup's threads of two counts.
+EP_DEV uint2 exclusive_sums(uint32_t x, uint32_t y, uint2 *s_part)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t px = x, py = y;
@@ -299,55 +328,32 @@ EP_DEV uint2 exclusive_sums(uint32_t x, uint32_t y, uint2 *s_part, uint2 &total)
     if (lane == 63)
         s_part[wave] = make_uint2(px, py);
     __syncthreads();
-    uint2 before = make_uint2(0, 0);
-    total = before;
+    uint2 before = make_uint2(px - x, py - y);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < kChooseWaves; ++w) {
         before.x += w < wave ? s_part[w].x : 0u;
         before.y += w < wave ? s_part[w].y : 0u;
-        total.x += s_part[w].x;
-        total.y += s_part[w].y;
     }
-    return make_uint2(before.x + px - x, before.y + py - y);
+    return before;
 }
 
-// A row's choice, one workgroup: the (take - 1) largest keys ahead of the own
-// page, found digit by digit from the top.  A round counts 2048 digits of
-// what lies between the least and the largest key still in question, so that
-// the first one parts them about as well as their number allows; of equal keys
-// the first are taken.
-__global__ void __launch_bounds__(256) choose_kernel(SelectArgs a)
+struct ChooseShared {
+    uint32_t count[kDigits];
+    uint64_t least[kChooseWaves], largest[kChooseWaves];
+    uint2 part[kChooseWaves];
+    uint32_t found[3];
+};
+
+// The (take - 1) largest of n keys, in order, and page n behind them: found
+// digit by digit from the top.  A round counts 2048 digits of what lies
+// between the least and the largest key still in question, so that the first
+// one parts them about as well as their number allows; of equal keys the first
+// are taken.  lo, hi: the least and the largest of the keys that this thread
+// has seen.
+template <typename KEY>
+EP_DEV void choose(ChooseShared &sh, int64_t n, int take, uint64_t lo, uint64_t hi, KEY key, int32_t *out)
 {
-    __shared__ uint64_t s_key[kHeldKeys];
-    __shared__ uint32_t s_count[2048];
-    __shared__ uint64_t s_end[2][4];
-    __shared__ uint2 s_part[4];
-    __shared__ uint32_t s_found[3];
-    const uint32_t r = a.first_wg + blockIdx.x;
-    const SelectRow row = select_row(a, r);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, take = a.take;
-    int32_t *out = a.blocks + (int64_t)r * take;
-    const int64_t n = row.own;
-    if (n < take) {
-        for (int i = tid; i < take; i += 256)
-            out[i] = i <= n ? i : -1;
-        return;
-    }
-    if (take == 1) {
-        if (tid == 0)
-            out[0] = (int32_t)n;
-        return;
-    }
-    const uint64_t *keys = a.keys + (int64_t)r * a.tok.width;
-    const bool held = n <= kHeldKeys;
-    uint64_t lo = ~0ull, hi = 0;
-    for (int64_t i = tid; i < n; i += 256) {
-        const uint64_t k = keys[i];
-        if (held)
-            s_key[i] = k;
-        lo = k < lo ? k : lo;
-        hi = k > hi ? k : hi;
-    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 #pragma unroll
     for (int d = 32; d >= 1; d /= 2) {
         const uint64_t l = __shfl_xor(lo, d, 64), h = __shfl_xor(hi, d, 64);
@@ -355,70 +361,66 @@ __global__ void __launch_bounds__(256) choose_kernel(SelectArgs a)
         hi = h > hi ? h : hi;
     }
     if (lane == 0) {
-        s_end[0][wave] = lo;
-        s_end[1][wave] = hi;
+        sh.least[wave] = lo;
+        sh.largest[wave] = hi;
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        lo = s_end[0][w] < lo ? s_end[0][w] : lo;
-        hi = s_end[1][w] > hi ? s_end[1][w] : hi;
+    for (int w = 0; w < kChooseWaves; ++w) {
+        lo = sh.least[w] < lo ? sh.least[w] : lo;
+        hi = sh.largest[w] > hi ? sh.largest[w] : hi;
     }
-    auto key = [&](int64_t i) { return held ? s_key[i] : keys[i]; };
     uint64_t span = hi - lo;
     uint32_t need = take - 1;
     bool all = false;        // every key from lo on is taken; else `need` of those equal to lo
     for (;;) {
         const int bits = span ? 64 - __builtin_clzll(span) : 0, shift = bits > 11 ? bits - 11 : 0;
-        for (int i = tid; i < 2048; i += 256)
-            s_count[i] = 0;
+        for (int i = tid; i < kDigits; i += kChoose)
+            sh.count[i] = 0;
         __syncthreads();
-        for (int64_t i = tid; i < n; i += 256) {
+        for (int64_t i = tid; i < n; i += kChoose) {
             const uint64_t k = key(i) - lo;         // below lo: past the span
             if (k <= span)
-                atomicAdd(&s_count[k >> shift], 1u);
+                atomicAdd(&sh.count[k >> shift], 1u);
         }
         __syncthreads();
-        // thread t holds digits 2047 - 8 t .. 2040 - 8 t
-        uint32_t c[8], sum = 0;
+        // thread t holds the digits from kDigits - 1 - E t down
+        constexpr int E = kDigits / kChoose;
+        uint32_t c[E], sum = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            c[i] = s_count[2047 - 8 * tid - i];
+        for (int i = 0; i < E; ++i) {
+            c[i] = sh.count[kDigits - 1 - E * tid - i];
             sum += c[i];
         }
-        uint2 total;
-        uint32_t above = exclusive_sums(sum, 0, s_part, total).x;
+        uint32_t above = exclusive_sums(sum, 0, sh.part).x;
         if (above < need && above + sum >= need)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < E; ++i) {
                 if (above < need && above + c[i] >= need) {
-                    s_found[0] = 2047 - 8 * tid - i;
-                    s_found[1] = above;
-                    s_found[2] = c[i];
+                    sh.found[0] = kDigits - 1 - E * tid - i;
+                    sh.found[1] = above;
+                    sh.found[2] = c[i];
                 }
                 above += c[i];
             }
         __syncthreads();
-        lo += (uint64_t)s_found[0] << shift;
-        need -= s_found[1];
-        all = s_found[2] == need;
+        lo += (uint64_t)sh.found[0] << shift;
+        need -= sh.found[1];
+        all = sh.found[2] == need;
         if (all || shift == 0)
             break;
         span = (1ull << shift) - 1;
     }
-    // in order: thread t writes what it takes of its n / 256 keys
-    const int64_t per = (n + 255) / 256, i0 = tid * per < n ? tid * per : n, i1 = i0 + per < n ? i0 + per : n;
+    // in order: thread t writes what it takes of its n / kChoose keys
+    const int64_t per = (n + kChoose - 1) / kChoose, i0 = tid * per < n ? tid * per : n, i1 = i0 + per < n ? i0 + per : n;
     uint32_t over = 0, equal = 0;
     for (int64_t i = i0; i < i1; ++i) {
         const uint64_t k = key(i);
         over += all ? k >= lo : k > lo;
         equal += !all && k == lo;
     }
-    uint2 total;
-    const uint2 before = exclusive_sums(over, equal, s_part, total);
-    uint32_t ties = before.y, to = before.x + (ties < need ? ties : need);
-    if (all)
-        to = before.x;
+    const uint2 before = exclusive_sums(over, equal, sh.part);
+    uint32_t ties = before.y, to = before.x + (all ? 0u : ties < need ? ties : need);
     for (int64_t i = i0; i < i1; ++i) {
         const uint64_t k = key(i);
         bool in = all ? k >= lo : k > lo;
@@ -431,11 +433,70 @@ __global__ void __launch_bounds__(256) choose_kernel(SelectArgs a)
         out[take - 1] = (int32_t)n;
 }
 
+// A row whose pages are all taken, or of which only its own is: done, true.
+EP_DEV bool chosen_at_once(int64_t n, int take, int32_t *out)
+{
+    if (n >= take && take > 1)
+        return false;
+    for (int i = threadIdx.x; i < take; i += kChoose)
+        out[i] = n >= take ? (int32_t)n : i <= n ? i : -1;
+    return true;
+}
+
+// A row's choice among scores in memory.
+__global__ void __launch_bounds__(kChoose) choose_kernel(SelectArgs a)
+{
+    __shared__ uint64_t s_key[kHeldKeys];
+    __shared__ ChooseShared sh;
+    const uint32_t r = a.first_wg + blockIdx.x;
+    const int64_t n = select_row(a, r).own;
+    int32_t *out = a.blocks + (int64_t)r * a.take;
+    if (chosen_at_once(n, a.take, out))
+        return;
+    const uint64_t *keys = a.keys + (int64_t)r * a.tok.width;
+    const bool held = n <= kHeldKeys;
+    uint64_t lo = ~0ull, hi = 0;
+    for (int64_t i0 = threadIdx.x; i0 < n; i0 += 4 * kChoose) {
+        uint64_t k[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)      // four loads in flight; past the end the first again
+            k[i] = keys[i0 + i * kChoose < n ? i0 + i * kChoose : i0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (held && i0 + i * kChoose < n)
+                s_key[i0 + i * kChoose] = k[i];
+            lo = k[i] < lo ? k[i] : lo;
+            hi = k[i] > hi ? k[i] : hi;
+        }
+    }
+    choose(sh, n, a.take, lo, hi, [&](int64_t i) { return held ? s_key[i] : keys[i]; }, out);
+}
+
+// Scores and choice of a row in one workgroup, where its pages are few.
+template <bool WIDE>
+__global__ void __launch_bounds__(kChoose) select_kernel(SelectArgs a)
+{
+    __shared__ uint64_t s_key[kFewPages];
+    __shared__ ChooseShared sh;
+    const uint32_t r = a.first_wg + blockIdx.x;
+    const SelectRow row = select_row(a, r);
+    int32_t *out = a.blocks + (int64_t)r * a.take;
+    if (chosen_at_once(row.own, a.take, out))
+        return;
+    uint64_t lo = ~0ull, hi = 0;
+    score_pages<WIDE>(a, row, 0, row.own, [&](int64_t page, uint64_t key) {
+        s_key[page] = key;
+        lo = key < lo ? key : lo;
+        hi = key > hi ? key : hi;
+    });
+    choose(sh, row.own, a.take, lo, hi, [&](int64_t i) { return s_key[i]; }, out);
+}
+
 // A launch has fewer than 2^32 threads: a grid beyond that is cut into several.
 template <typename ARGS, typename F>
-int in_launches(int64_t grid, ARGS a, F launch)
+int in_launches(int64_t grid, unsigned threads, ARGS a, F launch)
 {
-    const int64_t most = 0xffffffff / 256;
+    const int64_t most = 0xffffffff / threads;
     for (int64_t at = 0; at < grid; at += most) {
         a.first_wg = (uint32_t)at;
         launch(a, (unsigned)(grid - at < most ? grid - at : most));
@@ -453,7 +514,7 @@ int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, 
     if (parts > 0x7fffffff / c.heads)
         return set_error(EP_DECLINE_SHAPE, "bounds of %lld x %lld tokens are more than one call takes", (long long)tok.B,
                          (long long)tok.S);
-    return in_launches(parts * c.heads, BoundsArgs{tok, c, bounds, 0, (uint32_t)chunks}, [&](const BoundsArgs &a, unsigned n) {
+    return in_launches(parts * c.heads, 256, BoundsArgs{tok, c, bounds, 0, (uint32_t)chunks}, [&](const BoundsArgs &a, unsigned n) {
         if (c.dtype == EP_BF16)
             bounds_kernel<EP_BF16><<<n, 256, 0, stream>>>(a);
         else if (c.dtype == EP_F16)
@@ -465,10 +526,10 @@ int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, 
     });
 }
 
-// No scores where every page is taken.
+// No scores in memory where every page is taken, or pages are few.
 size_t select_workspace(const PagedTokens &tok, const PagedCache &c, int64_t take)
 {
-    return tok.width > take ? (size_t)tok.B * tok.S * c.heads * tok.width * sizeof(uint64_t) : 0;
+    return tok.width > take && take > 1 && tok.width > kFewPages ? (size_t)tok.B * tok.S * c.heads * tok.width * sizeof(uint64_t) : 0;
 }
 
 int launch_kv_select(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, const void *bounds, int64_t take,
@@ -498,16 +559,22 @@ int launch_kv_select(const ep_heads *q, const PagedTokens &tok, const PagedCache
     a.lanes = 2;
     while (a.lanes * 8 < c.D)
         a.lanes *= 2;
-    int rc = EP_OK;
-    if (want && take > 1)
-        rc = in_launches(rows * chunks, a, [&](const SelectArgs &part, unsigned n) {
-            if (c.dtype == EP_F16 || c.dtype == EP_BF16)
-                score_kernel<false><<<n, 256, 0, stream>>>(part);
+    const bool wide = c.dtype != EP_F16 && c.dtype != EP_BF16;
+    if (!want)
+        return in_launches(rows, kChoose, a, [&](const SelectArgs &part, unsigned n) {
+            if (wide)
+                select_kernel<true><<<n, kChoose, 0, stream>>>(part);
             else
-                score_kernel<true><<<n, 256, 0, stream>>>(part);
+                select_kernel<false><<<n, kChoose, 0, stream>>>(part);
         });
+    int rc = in_launches(rows * chunks, 256, a, [&](const SelectArgs &part, unsigned n) {
+        if (wide)
+            score_kernel<true><<<n, 256, 0, stream>>>(part);
+        else
+            score_kernel<false><<<n, 256, 0, stream>>>(part);
+    });
     if (rc == EP_OK)
-        rc = in_launches(rows, a, [&](const SelectArgs &part, unsigned n) { choose_kernel<<<n, 256, 0, stream>>>(part); });
+        rc = in_launches(rows, kChoose, a, [&](const SelectArgs &part, unsigned n) { choose_kernel<<<n, kChoose, 0, stream>>>(part); });
     return rc;
 }
 

@@ -106,8 +106,10 @@ def test_paged_calls_refuse(lib):
     assert lib.ep_kv_select(q, t, c, None, 2, P, P, 1 << 40, None) < 0
     assert lib.ep_kv_select(q, t, c, P + 8, 2, P, P, 1 << 40, None) < 0
     assert lib.ep_kv_select(q, t, c, P, 2, None, P, 1 << 40, None) < 0
-    assert lib.ep_kv_select(q, t, c, P, 2, P, None, 0, None) != 0
-    assert lib.ep_kv_select_workspace(t, c, 4) == 0 < lib.ep_kv_select_workspace(t, c, 3)   # all pages: no scores
+    assert lib.ep_kv_select(q, tokens(width=600), c, P, 2, P, None, 0, None) != 0
+    long = tokens(width=600)          # few pages, or all: no scores in memory
+    assert lib.ep_kv_select_workspace(t, c, 3) == lib.ep_kv_select_workspace(long, c, 600) == 0
+    assert lib.ep_kv_select_workspace(long, c, 1) == 0 < lib.ep_kv_select_workspace(long, c, 2)
     assert lib.ep_kv_select(heads(3, 64), t, c, P, 2, P, P, 1 << 40, None) < 0
     assert lib.ep_kv_bounds(t, c, None, None) < 0 and lib.ep_kv_bounds(t, c, P + 4, None) < 0
     many = tokens(B=1 << 15, S=1 << 15, width=1 << 20)
