@@ -57,7 +57,8 @@ EP_DEV int front_chunk(int r, int c)
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
-// 16 bytes a lane from offset `off` of the wave's `bytes` at p (past them: zeros) to 16 adjacent ones a lane in LDS.
+// 16 bytes a lane from offset `off` of the wave's `bytes` at p (past them: nothing, or zeros) to 16 adjacent ones a
+// lane in LDS.
 EP_DEV void lds_rows(const void *p, uint32_t bytes, uint16_t *lds, int off)
 {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_rsrc(p, bytes), (__attribute__((address_space(3))) void *)lds, 16, off, 0, 0, 0);
@@ -444,6 +445,13 @@ __global__ void __launch_bounds__(64 * kFrontWaves, kFrontOccupancy) front_kerne
         __syncthreads();             // the next stage is there, and this one's readers are done
     };
     if (count > 0) {
+        if (D < DM) {        // places that no load reaches
+            for (int x = tid; x < 2 * TP * DM / 8; x += 64 * kFrontWaves) {
+                *(u32x4_t *)&s_even[8 * x] = (u32x4_t){0, 0, 0, 0};
+                *(u32x4_t *)&s_odd[8 * x] = (u32x4_t){0, 0, 0, 0};
+            }
+            __syncthreads();
+        }
         id = __builtin_amdgcn_readfirstlane(page_of(j));
         next_id = page_of(j + 1);
         begin_rows(even, j);

@@ -193,8 +193,10 @@ class BatchDecoder:
         if uniforms is None:
             uniforms = torch.rand(B, n + 1, device=dev)
         for name, t, want in (("uniforms", uniforms, (B, n + 1)), ("draft", draft, (B, n, self.cfg.vocab))):
-            if t is not None and tuple(t.shape) != want:
+            if t is not None and tuple(t.shape) != want:        # before any sequence grows
                 raise ValueError(f"{name} {tuple(t.shape)} must be {list(want)}")
+            if t is not None and (t.dtype != torch.float32 or t.device != dev):
+                raise TypeError(f"{name} must be float32 on {dev}, got {t.dtype} on {t.device}")
         before = list(self.lengths)
         h = self._take([[] if t is None else [t, *d] for t, d in zip(last, drafts)])
         if h.shape[1] == 0:

@@ -495,7 +495,7 @@ class PagedKVCache:
         cache must have q's type.  Meant for one new token, or a few.
 
         ``shared``: the first so many pages are the same in every row of the
-        table (a prefix in common; those of row 0 are read).  They are computed
+        table (a prefix in common).  From 1024 positions on they are computed
         once for the whole batch instead of once a sequence.
 
         ``blocks`` (int32 [B, S, heads, n]): each token sees only what lies on

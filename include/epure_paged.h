@@ -136,11 +136,11 @@ int ep_paged_attention(const ep_heads *q, const ep_tokens *tokens, const ep_kv_c
 
 /*
  * The same attention for a batch whose tables begin with the same `shared`
- * pages (0 .. width; those of sequence 0 are read, whatever the other rows
- * name): these pages are computed once for the rows of the whole batch, then
- * each sequence's own, and the two are joined.  Every token's position may lie
- * in either.  At most 2^30 - 1 rows (tokens times query heads) on one cache
- * head.  Workspace: as above.
+ * pages (0 .. width; which row they are read from is not said): these pages are
+ * computed once for the rows of the whole batch, then each sequence's own, and
+ * the two are joined (a few pages are computed with the rest).  Every token's
+ * position may lie in either.  At most 2^30 - 1 rows (tokens times query
+ * heads) on one cache head.  Workspace: as above.
  */
 size_t ep_paged_attention_shared_workspace(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache,
                                            int64_t shared);

@@ -97,8 +97,10 @@ def test_paged_calls_refuse(lib):
     for shared in (-1, 5):
         assert lib.ep_paged_attention_shared(q, t, c, shared, 1.0, 0, P, P, 1 << 40, None) < 0
         assert lib.ep_paged_attention_shared_workspace(q, t, c, shared) == 0
-    assert lib.ep_paged_attention_shared(q, t, c, 2, 1.0, 0, P, None, 0, None) != 0          # workspace
-    assert lib.ep_paged_attention_shared_workspace(q, t, c, 2) > 0
+    large = cache(page=1024)
+    assert lib.ep_paged_attention_shared_workspace(q, t, large, 2) > 0
+    assert lib.ep_paged_attention_shared(q, t, large, 2, 1.0, 0, P, None, 0, None) < 0
+    assert "workspace" in _abi.last_error()
     assert lib.ep_paged_attention_blocks(q, t, c, None, 2, 1.0, 0, P, P, 1 << 40, None) < 0
     for take in (0, -1, 1 << 27):
         assert lib.ep_paged_attention_blocks(q, t, c, P, take, 1.0, 0, P, P, 1 << 40, None) != 0

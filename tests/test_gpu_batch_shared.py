@@ -90,6 +90,25 @@ def test_a_generation_behind_a_prefix_takes_its_pages_once():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", list(HELD))
+def test_a_long_prefix_gives_what_it_gives_each_sequence(cache_dtype):
+    """1040 positions in common (computed once a step) against the same tokens in
+    every sequence: twice a decoder's distance from float32."""
+    w = random_weights(CFG, seed=6, device=DEV)
+    g = torch.Generator().manual_seed(4)
+    prefix, prompts = ids(g, 1045), [ids(g, n) for n in (12, 1, 30, 4)]
+    shared, apart = (BatchDecoder(w, 4, 1200, page=16, cache_dtype=cache_dtype) for _ in range(2))
+    rest = shared.share(prefix)
+    assert len(rest) == 5 and shared.shared == 65
+    new, whole = [rest + p for p in prompts], [prefix + p for p in prompts]
+    for _ in range(4):
+        got, want = shared.forward(new), apart.forward(whole)
+        assert ((got - want).norm(dim=-1) <= 2 * tolerance(cache_dtype) * want.norm(dim=-1)).all()
+        new = whole = [ids(g, 1) for _ in range(4)]
+    assert shared.lengths == apart.lengths and len(shared.free) == shared.n_pages - 65 - sum(map(len, shared.owned))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("select", [None, 3])
 def test_drafted_tokens_stand_or_are_taken_back(select):
     """Against the oracle on the same probabilities (a twin's, taken token by
@@ -194,6 +213,8 @@ def test_refusals_change_nothing():
                         (([1, 2], [[], []], None, None, 0.0), ValueError),
                         (([1, 2], [[3], []], torch.zeros(2, 3)), ValueError),
                         (([1, 2], [[3], []], None, torch.zeros(2, 1, 49)), ValueError),
+                        (([1, 2], [[3], []], torch.zeros(2, 2).double()), TypeError),
+                        (([1, 2], [[3], []], None, torch.zeros(2, 1, 50).half()), TypeError),
                         (([1, 50], [[], []]), ValueError), (([1] * 3, [[]] * 3), ValueError),
                         (([1, 2], [[3] * 64, []]), ValueError)):
         with pytest.raises(error):

@@ -122,7 +122,7 @@ def limits(cache, table):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,S,width,page,G,heads,D,take", [
     (1, 1, 1, 16, 1, 1, 16, 1), (3, 1, 9, 16, 4, 2, 128, 4), (2, 3, 40, 16, 3, 1, 96, 7), (2, 1, 5, 32, 8, 2, 256, 9),
-    (1, 2, 300, 16, 1, 1, 48, 64), (2, 1, 150, 16, 5, 2, 80, 149), (1, 1, 33, 64, 2, 1, 144, 1), (4, 1, 7, 16, 2, 1, 64, 7)])
+    (1, 2, 300, 16, 1, 1, 48, 64), (2, 1, 700, 16, 3, 2, 80, 100), (2, 1, 150, 16, 5, 2, 80, 149), (1, 1, 33, 64, 2, 1, 144, 1), (4, 1, 7, 16, 2, 1, 64, 7)])
 def test_selection(B, S, width, page, G, heads, D, take, dtype):
     """Equal pages: scores in float64 differ by far more than their sums' rounding."""
     g = gen(width + take)

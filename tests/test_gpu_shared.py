@@ -39,7 +39,7 @@ def filled(g, B, shared, own, page, heads, D, dtype):
     k, v = normal(g, B, L, heads, D, dtype=xdt), normal(g, B, L, heads, D, dtype=xdt)
     k[:, :shared * page], v[:, :shared * page] = k[:1, :shared * page], v[:1, :shared * page]
     cache.append(k, v, torch.arange(L, device=DEV), table)
-    return cache, table, op.stands_for(k, dtype), op.stands_for(v, dtype)
+    return (cache, table, *cache.read(torch.arange(L, device=DEV).expand(B, L), table, F32))
 
 
 def check(got, q, k, v, pos, scale, window=None):
@@ -51,10 +51,11 @@ def check(got, q, k, v, pos, scale, window=None):
     assert not bad.any(), f"{bad.sum().item()} of {bad.numel()} off"
 
 
-CASES = [  # B, S, shared, own, page, G, heads, D
-    (2, 1, 1, 1, 16, 1, 1, 64), (3, 1, 2, 3, 16, 4, 2, 128), (5, 1, 9, 1, 32, 2, 1, 96), (2, 5, 3, 2, 16, 5, 2, 80),
-    (9, 3, 4, 2, 16, 3, 1, 48), (40, 1, 2, 1, 16, 2, 2, 16), (3, 1, 1, 9, 64, 8, 1, 192), (2, 2, 5, 1, 16, 20, 1, 256),
-    (17, 1, 40, 1, 32, 4, 1, 128), (6, 8, 33, 2, 32, 3, 1, 144), (70, 2, 3, 1, 16, 1, 2, 160), (2, 1, 3, 2, 128, 1, 3, 112)]
+CASES = [  # B, S, shared (1024 positions or more), own, page, G, heads, D
+    (2, 1, 64, 1, 16, 1, 1, 64), (3, 1, 65, 3, 16, 4, 2, 128), (5, 1, 34, 1, 32, 2, 1, 96), (2, 5, 66, 2, 16, 5, 2, 80),
+    (9, 3, 67, 2, 16, 3, 1, 48), (40, 1, 64, 1, 16, 2, 2, 16), (3, 1, 17, 9, 64, 8, 1, 192), (2, 2, 70, 1, 16, 20, 1, 256),
+    (17, 1, 40, 1, 32, 4, 1, 128), (6, 8, 33, 2, 32, 3, 1, 144), (20, 2, 65, 1, 16, 1, 2, 160), (2, 1, 9, 2, 128, 1, 3, 112),
+    (2, 1, 1, 1, 1024, 2, 1, 32), (3, 2, 5, 2, 16, 2, 1, 64)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, I8, E4M3])
@@ -68,56 +69,58 @@ def test_shared_pages(B, S, shared, own, page, G, heads, D, dtype):
     pos = torch.randint(0, L, (B, S), generator=g, device=DEV)
     edge = torch.tensor([P - 1, P, L - 1, 0, -1, L, P + 1], device=DEV)
     pos.view(-1)[:min(7, B * S)] = edge[:min(7, B * S)]
-    for window in (None, 1, 17, P + 3):
+    for window in (None, 17, 1024, 1029, P + 3):
         check(cache.attend(q, pos, table, window=window, shared=shared), q, k, v, pos, D ** -0.5, window)
     check(cache.attend(q, pos, table, scale=0.3, shared=shared - 1), q, k, v, pos, 0.3)
 
 
 def test_all_pages_shared_and_none():
     g = gen(2)
-    cache, table, k, v = filled(g, 4, 6, 1, 16, 2, 64, BF16)
-    q, pos = normal(g, 4, 1, 4, 64, std=2.0), torch.tensor([[95], [3], [40], [-1]], device=DEV)
-    check(cache.attend(q, pos, table[:, :6], shared=6), q, k[:, :96], v[:, :96], pos, 0.125)
+    cache, table, k, v = filled(g, 4, 70, 1, 16, 2, 64, BF16)
+    q, pos = normal(g, 4, 1, 4, 64, std=2.0), torch.tensor([[1119], [3], [1040], [-1]], device=DEV)
+    check(cache.attend(q, pos, table[:, :70], shared=70), q, k[:, :1120], v[:, :1120], pos, 0.125)
     assert torch.equal(cache.attend(q, pos, table, shared=0), cache.attend(q, pos, table))
     # one sequence shares with nobody
-    assert torch.equal(cache.attend(q[:1], pos[:1], table[:1], shared=6), cache.attend(q[:1], pos[:1], table[:1]))
+    assert torch.equal(cache.attend(q[:1], pos[:1], table[:1], shared=70), cache.attend(q[:1], pos[:1], table[:1]))
 
 
 @pytest.mark.parametrize("dtype", [BF16, I8])
 def test_pages_that_the_pool_lacks_and_values_that_are_not_finite(dtype):
     """A missing page is a NaN to who sees a position on it; so is a value that is not finite, and to nobody else."""
     g = gen(3)
-    cache, table, k, v = filled(g, 40, 4, 2, 16, 1, 64, dtype)
+    at = 63 * 16
+    cache, table, k, v = filled(g, 40, 67, 2, 16, 1, 64, dtype)
     q = normal(g, 40, 1, 2, 64, std=2.0)
-    pos = (torch.arange(40, device=DEV) * 2 + 16)[:, None]         # 16 .. 94
-    table[:, 2] = 1 << 20           # positions 32 .. 47, shared
-    table[20, 4] = -1               # 64 .. 79 of sequence 20 (position 56: not seen), 30 (76: seen)
-    table[30, 4] = -1
-    got = cache.attend(q, pos, table, shared=4)
-    want = ((pos >= 32) | (torch.arange(40, device=DEV)[:, None] == 30))[..., None, None].expand_as(got)
+    pos = (torch.arange(40, device=DEV) * 2 + 16)[:, None] + at    # 16 .. 94 behind 1008
+    table[:, 65] = 1 << 20           # positions 32 .. 47, shared
+    table[20, 67] = -1               # 64 .. 79 of sequence 20 (position 56: not seen), 30 (76: seen)
+    table[30, 67] = -1
+    got = cache.attend(q, pos, table, shared=67)
+    want = ((pos >= at + 32) | (torch.arange(40, device=DEV)[:, None] == 30))[..., None, None].expand_as(got)
     assert torch.equal(got.isnan(), want)
-    assert torch.equal(cache.attend(q, pos, table, shared=4, window=5).isnan()[:, 0, 0, 0].cpu(),
-                       torch.tensor([any(32 <= j < 48 or (i == 30 and 64 <= j < 80) for j in range(p - 4, p + 1))
-                                     for i, p in enumerate(pos[:, 0].tolist())]))
-    cache, table, k, v = filled(g, 40, 4, 2, 16, 1, 64, dtype)
-    page, row = int(table[0, 1]), 5                                 # position 21
+    for window in (5, 1030):
+        assert torch.equal(cache.attend(q, pos, table, shared=67, window=window).isnan()[:, 0, 0, 0].cpu(), torch.tensor(
+            [any(32 <= j - at < 48 or (i == 30 and 64 <= j - at < 80) for j in range(max(p - window + 1, 0), p + 1))
+             for i, p in enumerate(pos[:, 0].tolist())]))
+    cache, table, k, v = filled(g, 40, 67, 2, 16, 1, 64, dtype)
+    page, row = int(table[0, 64]), 5                                # position 1029
     if dtype == BF16:
         cache.v[page, 0, row, 7] = float("inf")
         cache.k[page, 0, row + 1] = float("nan")
     else:
         cache.v_scale[page, 0, row] = float("inf")
         cache.k_scale[page, 0, row + 1] = float("nan")
-    got = cache.attend(q, pos, table, shared=4)
-    assert not got[:3].isnan().any() and not got[:3].isinf().any()          # positions 16, 18, 20
+    got = cache.attend(q, pos, table, shared=67)
+    assert not got[:3].isnan().any() and not got[:3].isinf().any()          # positions 1024, 1026, 1028
     assert got[3:].isnan().any(-1).all()
 
 
 def test_strided_queries_and_other_streams_and_graphs():
     g = gen(4)
-    cache, table, k, v = filled(g, 6, 5, 2, 16, 2, 128, BF16)
+    cache, table, k, v = filled(g, 6, 66, 2, 16, 2, 128, BF16)
     q = normal(g, 6, 2, 8, 128, std=2.0)
-    pos = torch.randint(0, 112, (6, 2), generator=g, device=DEV)
-    want = cache.attend(q, pos, table, shared=5)
+    pos = torch.randint(0, 68 * 16, (6, 2), generator=g, device=DEV)
+    want = cache.attend(q, pos, table, shared=66)
     check(want, q, k, v, pos, 128 ** -0.5)
     wide = torch.empty(6, 2, 8, 136, dtype=BF16, device=DEV)
     wide[..., :128] = q
@@ -125,21 +128,21 @@ def test_strided_queries_and_other_streams_and_graphs():
     odd.copy_(q)
     for x in (wide[..., :128], odd, q.transpose(0, 1).contiguous().transpose(0, 1),
               q.transpose(1, 2).contiguous().transpose(1, 2)):
-        assert torch.equal(cache.attend(x, pos, table, shared=5), want)
-    assert torch.equal(cache.attend(q, pos.T.contiguous().T, torch.cat((table, table), 1)[:, :7], shared=5), want)
+        assert torch.equal(cache.attend(x, pos, table, shared=66), want)
+    assert torch.equal(cache.attend(q, pos.T.contiguous().T, torch.cat((table, table), 1)[:, :68], shared=66), want)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        other = cache.attend(q, pos, table, shared=5)
+        other = cache.attend(q, pos, table, shared=66)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(other, want)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        out = cache.attend(q, pos, table, shared=5)
+        out = cache.attend(q, pos, table, shared=66)
     for i in range(3):
-        pos.copy_(torch.randint(-1, 113, (6, 2), generator=g, device=DEV))
+        pos.copy_(torch.randint(-1, 68 * 16 + 1, (6, 2), generator=g, device=DEV))
         q.copy_(normal(g, 6, 2, 8, 128, std=2.0))
-        want = cache.attend(q, pos, table, shared=5)
+        want = cache.attend(q, pos, table, shared=66)
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0))
