@@ -84,7 +84,8 @@ struct AttendArgs {
 //     from there.  Every output stays a part: the join adds them up (more than
 //     32 rows a cache head over the shared pages are attend_front.h's);
 //   kBlocks: a unit is up to 16 rows of one token, and tile after tile goes
-//     over the `take` pages that a list names for it, in `cuts` equal pieces.
+//     over the `take` pages that a list names for it, in `cuts` equal pieces
+//     (8 tokens of 64 pages of 64 positions, 8 heads of 128 in bf16, 134 MB: 23 us).
 enum AttendMode { kWhole, kParts, kBlocks };
 
 struct AttendWhole : AttendArgs {
