@@ -18,16 +18,20 @@
 // heads of 128 (bf16, 67 MB) take 17 us and the choice of 64 of them 8, a chain
 // of steps over LDS.  Up to kFewPages pages a row one workgroup does both in one
 // launch (44 pages on 8 heads: 7.4 us; 60 tokens of up to 282 pages on 4: 12.8).
-// The bounds of 64 appended tokens take 6.2 us, a chain of loads, and those of
-// 2 x 4096 (8 heads, pages of 64) 10.4, beside 14.4 for the rows themselves.
+// The bounds of 64 appended tokens take 5.8 us, a chain of loads, and those of
+// 2 x 4096 (8 heads, pages of 64) 10.6, beside 14.5 for the rows themselves.
 #include "ep_common.h"
 #include "ep_internal.h"
 #include "ep_paged.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace ep {
 namespace {
 
-constexpr int kChunkTokens = 64;    // tokens a workgroup of the bounds looks over
+constexpr int kGroupTokens = 64;    // tokens that a wave looks over at a time for the bounds
+constexpr int kRowChunks = 64;      // workgroups that share a row of tokens for them, at most
 constexpr int kChunkPages = 128;    // pages a workgroup scores
 constexpr int kHeldKeys = 4096;     // scores that the choice keeps in LDS (32 KiB)
 constexpr int kFewPages = 512;      // of a table whose rows one workgroup each scores and chooses from
@@ -36,7 +40,7 @@ struct BoundsArgs {
     PagedTokens tok;
     PagedCache c;
     void *bounds;
-    uint32_t first_wg, chunks;
+    uint32_t first_wg, chunks, each;     // workgroups a sequence, of `each` groups of tokens
 };
 
 // Eight adjacent values of a cache row as f32.
@@ -65,91 +69,153 @@ EP_DEV void row_values(const PagedCache &c, int64_t row, int d, float *v)
 EP_DEV float least(float a, float b) { return b < a || b != b ? b : a; }
 EP_DEV float largest(float a, float b) { return b > a || b != b ? b : a; }
 
-// One workgroup looks over 64 tokens of a sequence and one cache head.  Of the
-// tokens on one page the one at the largest position (of two there, the later
-// in the call) rebuilds the page's bounds from its rows up to that position:
+// The next lane's value (the last lane's: anything).
+EP_DEV int64_t next_lane(int64_t v)
+{
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)v, 0x130, 0xf, 0xf, false);     // wave_shl:1
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(v >> 32), 0x130, 0xf, 0xf, false);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// One workgroup looks over `each` times 64 tokens of a sequence and one cache head.
+// Of the tokens on one page the one at the largest position (of two there, the
+// later in the call) rebuilds the page's bounds from its rows up to that position:
 // what the page held before the call counts as the new rows do, nothing that it
 // held for an earlier sequence does, and it does not matter how often it is done.
-template <int CODE>
+// Where positions ascend (then, in a padded row, none) that token is the one
+// whose successor lies elsewhere; in any other order the whole row is searched
+// for a later one, once a page.
+// WAVES waves share a page: all four, or one; 0: all four, and rows are of one
+// token (code for several, fetched cold, took 0.7 us more).
+template <int CODE, int WAVES>
 __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
 {
+    constexpr bool ONE = WAVES == 0;
+    constexpr int TEAMS = WAVES == 1 ? 4 : 1, TEAM = 256 / TEAMS, kOrder = WAVES == 1 ? 16 : 8;
     __shared__ float s_lo[256 * 8], s_hi[256 * 8];
     const uint32_t at = a.first_wg + blockIdx.x, H = a.c.heads;
-    const uint32_t part = at / H, h = at - part * H, b = part / a.chunks, chunk = part - b * a.chunks;
-    const int tid = threadIdx.x, lane = tid & 63, D = a.c.D;
+    const uint32_t part = at / H, h = at - part * H, b = ONE ? part : part / a.chunks, chunk = part - b * a.chunks;
+    const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM, lane = tid & 63, D = a.c.D;
     const int64_t *pos = a.tok.pos + (int64_t)b * a.tok.pos_sb;
-    const int64_t s = (int64_t)chunk * kChunkTokens + lane, ps = a.tok.pos_ss;
-    const int64_t p = s < a.tok.S ? pos[s * ps] : -1, after = s + 1 < a.tok.S ? pos[(s + 1) * ps] : -1;
-    const int64_t index = p >> a.c.page_shift;
-    int32_t id = -1;
-    if (p >= 0 && index < a.tok.width)
-        id = a.tok.table[b * a.tok.table_stride + index];
-    // the next token is the next row of the page: not the last one there
-    const bool inner = after == p + 1 && after >> a.c.page_shift == index;
-    uint64_t left = __ballot(id >= 0 && id < a.c.n_pages && !inner);
-    const int lanes = D / 8, group = tid / lanes, u = tid - group * lanes, groups = 256 / lanes;
-    for (; left; left &= left - 1) {
-        const int l = __builtin_ctzll(left);
-        const int64_t mine = __shfl(p, l, 64), page = mine >> a.c.page_shift, who = (int64_t)chunk * kChunkTokens + l;
-        if (a.tok.S > 1) {
-            int later = 0;
-            for (int64_t t0 = tid; t0 < a.tok.S; t0 += 8 * 256) {
-                int64_t o[8];
+    const int64_t ps = a.tok.pos_ss, s_begin = (int64_t)chunk * a.each * kGroupTokens;
+    const int64_t s_end = s_begin + a.each * kGroupTokens < a.tok.S ? s_begin + a.each * kGroupTokens : a.tok.S;
+    bool ascend = true;
+    if constexpr (!ONE) {
+        int wrong = 0;
+        for (int64_t t0 = threadIdx.x; t0 < a.tok.S; t0 += kOrder * 256) {
+            int64_t o[kOrder], after[kOrder];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)      // eight loads in flight; past the end the first again
-                    o[i] = pos[(t0 + 256 * i < a.tok.S ? t0 + 256 * i : t0) * ps];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int64_t t = t0 + 256 * i < a.tok.S ? t0 + 256 * i : t0;
-                    later |= o[i] >= 0 && o[i] >> a.c.page_shift == page && (o[i] > mine || (o[i] == mine && t > who));
-                }
+            for (int i = 0; i < kOrder; ++i) {      // all in flight; past the end the first again
+                const int64_t t = t0 + 256 * i < a.tok.S ? t0 + 256 * i : t0;
+                o[i] = pos[t * ps];
+                after[i] = -1;
+                if (lane == 63 && t + 1 < a.tok.S)
+                    after[i] = pos[(t + 1) * ps];
             }
-            if (__syncthreads_or(later))
-                continue;
+#pragma unroll
+            for (int i = 0; i < kOrder; ++i) {
+                const int64_t next = next_lane(o[i]), t = t0 + 256 * i < a.tok.S ? t0 + 256 * i : t0;
+                after[i] = lane == 63 ? after[i] : t + 1 < a.tok.S ? next : -1;
+                wrong |= after[i] >= 0 && (o[i] < 0 || after[i] <= o[i]);
+            }
         }
-        const int64_t row0 = ((int64_t)__shfl(id, l, 64) * H + h) * a.c.page;
-        const int rows = (int)(mine & (a.c.page - 1)) + 1;
-        float lo[8], hi[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            lo[i] = INFINITY;
-            hi[i] = -INFINITY;
+        ascend = !__syncthreads_or(wrong);
+    }
+    // LDS of a team of one wave: its own accesses stay in order
+    auto team_sync = [&]() {
+        if constexpr (TEAMS == 1)
+            __syncthreads();
+        else {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+            __builtin_amdgcn_wave_barrier();
         }
-        if (group < groups)
-            for (int r = group; r < rows; r += 4 * groups) {
-                float v[4][8];
+    };
+    auto team_any = [&](int x) {
+        if constexpr (TEAMS == 1)
+            return __syncthreads_or(x);
+        else
+            return __any(x);
+    };
+    float *const t_lo = s_lo + 8 * TEAM * team, *const t_hi = s_hi + 8 * TEAM * team;
+    const int lanes = D / 8, group = tid / lanes, u = tid - group * lanes, groups = TEAM / lanes;
+    for (int64_t s0 = s_begin + kGroupTokens * team; s0 < s_end; s0 += kGroupTokens * TEAMS) {
+        const int64_t s = s0 + lane;
+        const int64_t p = ONE ? pos[0] : s < a.tok.S ? pos[s * ps] : -1, after = !ONE && s + 1 < a.tok.S ? pos[(s + 1) * ps] : -1;
+        const int64_t index = p >> a.c.page_shift;
+        int32_t id = -1;
+        if (p >= 0 && index < a.tok.width)
+            id = a.tok.table[b * a.tok.table_stride + index];
+        // not the last one there: where positions ascend, any on the page that follows; else
+        // the next token on the next row
+        const bool inner = after >> a.c.page_shift == index && (ascend ? after >= 0 : after == p + 1);
+        uint64_t left = __ballot(id >= 0 && id < a.c.n_pages && !inner);
+        for (; left; left &= left - 1) {
+            const int l = ONE ? 0 : __builtin_ctzll(left);
+            const int64_t mine = __shfl(p, l, 64), page = mine >> a.c.page_shift, who = s0 + l;
+            if (!ONE && !ascend) {
+                int later = 0;
+                for (int64_t t0 = tid; t0 < a.tok.S; t0 += 8 * TEAM) {
+                    int64_t o[8];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)      // four rows in flight; past the end the last again
-                    row_values<CODE>(a.c, row0 + min(r + k * groups, rows - 1), 8 * u, v[k]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
+                    for (int i = 0; i < 8; ++i)      // eight loads in flight; past the end the first again
+                        o[i] = pos[(t0 + TEAM * i < a.tok.S ? t0 + TEAM * i : t0) * ps];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        lo[i] = least(lo[i], v[k][i]);
-                        hi[i] = largest(hi[i], v[k][i]);
+                        const int64_t t = t0 + TEAM * i < a.tok.S ? t0 + TEAM * i : t0;
+                        later |= o[i] >= 0 && o[i] >> a.c.page_shift == page && (o[i] > mine || (o[i] == mine && t > who));
                     }
+                }
+                if (team_any(later))
+                    continue;
             }
-        __syncthreads();         // the buffers' last readers are done
+            const int64_t row0 = ((int64_t)__shfl(id, l, 64) * H + h) * a.c.page;
+            const int rows = (int)(mine & (a.c.page - 1)) + 1;
+            float lo[8], hi[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            s_lo[8 * tid + i] = lo[i];      // [group][D], as 8 (group lanes + u) + i = group D + 8 u + i
-            s_hi[8 * tid + i] = hi[i];
+            for (int i = 0; i < 8; ++i) {
+                lo[i] = INFINITY;
+                hi[i] = -INFINITY;
+            }
+            if (group < groups)
+                for (int r = group; r < rows; r += 4 * groups) {
+                    float v[4][8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)      // four rows in flight; past the end the last again
+                        row_values<CODE>(a.c, row0 + min(r + k * groups, rows - 1), 8 * u, v[k]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            lo[i] = least(lo[i], v[k][i]);
+                            hi[i] = largest(hi[i], v[k][i]);
+                        }
+                }
+            team_sync();         // the buffers' last readers are done
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                t_lo[8 * tid + i] = lo[i];      // [group][D], as 8 (group lanes + u) + i = group D + 8 u + i
+                t_hi[8 * tid + i] = hi[i];
+            }
+            team_sync();
+            const int64_t out = ((int64_t)__shfl(id, l, 64) * H + h) * 2 * D;
+            for (int e = tid; e < 2 * D; e += TEAM) {
+                const bool top = e >= D;
+                const int d = top ? e - D : e;
+                float x = top ? t_hi[d] : t_lo[d];
+                for (int k = 1; k < groups; ++k)
+                    x = top ? largest(x, t_hi[k * D + d]) : least(x, t_lo[k * D + d]);
+                if constexpr (CODE == EP_F16)
+                    ((f16_t *)a.bounds)[out + e] = (f16_t)x;
+                else if constexpr (CODE == EP_BF16)
+                    ((uint16_t *)a.bounds)[out + e] = f32_to_bf16(x);
+                else
+                    ((float *)a.bounds)[out + e] = x;
+            }
+            if (ONE)
+                return;
         }
-        __syncthreads();
-        const int64_t out = ((int64_t)__shfl(id, l, 64) * H + h) * 2 * D;
-        for (int e = tid; e < 2 * D; e += 256) {
-            const bool top = e >= D;
-            const int d = top ? e - D : e;
-            float x = top ? s_hi[d] : s_lo[d];
-            for (int k = 1; k < groups; ++k)
-                x = top ? largest(x, s_hi[k * D + d]) : least(x, s_lo[k * D + d]);
-            if constexpr (CODE == EP_F16)
-                ((f16_t *)a.bounds)[out + e] = (f16_t)x;
-            else if constexpr (CODE == EP_BF16)
-                ((uint16_t *)a.bounds)[out + e] = f32_to_bf16(x);
-            else
-                ((float *)a.bounds)[out + e] = x;
-        }
+        if (ONE)
+            return;
     }
 }
 
@@ -516,21 +582,38 @@ int in_launches(int64_t grid, unsigned threads, ARGS a, F launch)
 
 int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, hipStream_t stream)
 {
-    const int64_t chunks = (tok.S + kChunkTokens - 1) / kChunkTokens;
+    // From 1024 pages and heads on a wave rebuilds a page alone.  With four / one,
+    // 8 heads of 128 in bf16, append included: 2 x 512 tokens on pages of 64, 128 of
+    // them, 11.4 / 17.1 us; 2 x 4096, 1024, 28.1 / 26.7; on pages of 16 40 / 32;
+    // 65536 332 / 171.
+    const bool alone = tok.S > 1 && tok.B * c.heads * ((tok.S + c.page - 1) >> c.page_shift) >= 1024;
+    // Every workgroup looks at its whole row for the positions' order: long rows
+    // have no more than kRowChunks of them a head.
+    const int64_t tokens = (tok.S + kGroupTokens - 1) / kGroupTokens;
+    const int64_t each = std::max<int64_t>((tokens + kRowChunks - 1) / kRowChunks, alone ? 4 : 1);
+    const int64_t chunks = (tokens + each - 1) / each;
     const int64_t parts = tok.B * chunks;
     if (parts > 0x7fffffff / c.heads)
         return set_error(EP_DECLINE_SHAPE, "bounds of %lld x %lld tokens are more than one call takes", (long long)tok.B,
                          (long long)tok.S);
-    return in_launches(parts * c.heads, 256, BoundsArgs{tok, c, bounds, 0, (uint32_t)chunks}, [&](const BoundsArgs &a, unsigned n) {
-        if (c.dtype == EP_BF16)
-            bounds_kernel<EP_BF16><<<n, 256, 0, stream>>>(a);
-        else if (c.dtype == EP_F16)
-            bounds_kernel<EP_F16><<<n, 256, 0, stream>>>(a);
-        else if (c.dtype == EP_I8)
-            bounds_kernel<EP_I8><<<n, 256, 0, stream>>>(a);
-        else
-            bounds_kernel<EP_E4M3><<<n, 256, 0, stream>>>(a);
-    });
+    const BoundsArgs args{tok, c, bounds, 0, (uint32_t)chunks, (uint32_t)each};
+    auto run = [&](auto code) {
+        constexpr int CODE = decltype(code)::value;
+        return in_launches(parts * c.heads, 256, args, [&](const BoundsArgs &a, unsigned n) {
+            if (tok.S == 1)
+                bounds_kernel<CODE, 0><<<n, 256, 0, stream>>>(a);
+            else if (alone)
+                bounds_kernel<CODE, 1><<<n, 256, 0, stream>>>(a);
+            else
+                bounds_kernel<CODE, 4><<<n, 256, 0, stream>>>(a);
+        });
+    };
+    switch (c.dtype) {
+    case EP_BF16: return run(std::integral_constant<int, EP_BF16>());
+    case EP_F16: return run(std::integral_constant<int, EP_F16>());
+    case EP_I8: return run(std::integral_constant<int, EP_I8>());
+    default: return run(std::integral_constant<int, EP_E4M3>());
+    }
 }
 
 // No scores in memory where every page is taken, or pages are few.

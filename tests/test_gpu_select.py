@@ -81,6 +81,26 @@ def test_bounds_of_prompts_then_tokens(B, width, page, heads, D, dtype):
     step(torch.randperm(L, generator=g, device=DEV).expand(B, L))
 
 
+@pytest.mark.parametrize("dtype,page,D", [(BF16, 16, 48), (I8, 32, 80), (F16, 16, 256), (E4M3, 64, 128)])
+def test_bounds_of_rows_that_more_workgroups_share(dtype, page, D):
+    """Rows of more than 64 groups of 64 tokens, past 1024 pages: one in order, one in order with gaps that ends
+    early, one in order but for its last token, one that begins with none, one backwards."""
+    S, B, heads = 4200, 5, 16 if page == 64 else 4
+    g = gen(page)
+    cache, table = made(g, B, -(-S // page) + 2, page, heads, D, dtype)
+    pos = torch.arange(S, device=DEV).repeat(B, 1)
+    pos[1] = (pos[1] + pos[1] // 5).where(pos[1] < 3000, -1)
+    pos[2, -1] = 7
+    pos[3] = torch.where(pos[3] < 70, -1, pos[3] - 70)
+    pos[4] = pos[4].flip(0)
+    xdt = dtype if dtype.itemsize == 2 else BF16
+    for _ in range(2):
+        before = cache.k_bounds.clone()
+        cache.append(normal(g, B, S, heads, D, dtype=xdt), normal(g, B, S, heads, D, dtype=xdt), pos, table)
+        check_bounds(cache, before, table.cpu(), pos.cpu(), page)
+        pos = pos[:, torch.randperm(S, generator=g, device=DEV)]        # then in no order at all
+
+
 def test_bounds_through_a_rotation_with_queries_and_without_the_native_path(monkeypatch):
     from epure.kernels import _abi
     g = gen(3)
