@@ -82,9 +82,9 @@ EP_DEV int64_t next_lane(int64_t v)
 // later in the call) rebuilds the page's bounds from its rows up to that position:
 // what the page held before the call counts as the new rows do, nothing that it
 // held for an earlier sequence does, and it does not matter how often it is done.
-// Where positions ascend (then, in a padded row, none) that token is the one
-// whose successor lies elsewhere; in any other order the whole row is searched
-// for a later one, once a page.
+// Where positions ascend (padded at either end) that token is the one whose
+// successor lies elsewhere; in any other order the whole row is searched for a
+// later one, once a page.
 // WAVES waves share a page: all four, or one; 0: all four, and rows are of one
 // token (code for several, fetched cold, took 0.7 us more).
 template <int CODE, int WAVES>
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
     const int64_t s_end = s_begin + a.each * kGroupTokens < a.tok.S ? s_begin + a.each * kGroupTokens : a.tok.S;
     bool ascend = true;
     if constexpr (!ONE) {
-        int wrong = 0;
+        int wrong = 0, begins = 0;
         for (int64_t t0 = threadIdx.x; t0 < a.tok.S; t0 += kOrder * 256) {
             int64_t o[kOrder], after[kOrder];
 #pragma unroll
@@ -116,10 +116,13 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
             for (int i = 0; i < kOrder; ++i) {
                 const int64_t next = next_lane(o[i]), t = t0 + 256 * i < a.tok.S ? t0 + 256 * i : t0;
                 after[i] = lane == 63 ? after[i] : t + 1 < a.tok.S ? next : -1;
-                wrong |= after[i] >= 0 && (o[i] < 0 || after[i] <= o[i]);
+                wrong |= after[i] >= 0 && after[i] <= o[i];
+                begins += o[i] < 0 && after[i] >= 0 && t0 + 256 * i < a.tok.S;
             }
         }
-        ascend = !__syncthreads_or(wrong);
+        // behind a token that is none they may begin once, where the first is none
+        const int threads = __syncthreads_count(begins);
+        ascend = !__syncthreads_or(wrong || begins > 1) && threads <= (pos[0] < 0);
     }
     // LDS of a team of one wave: its own accesses stay in order
     auto team_sync = [&]() {
