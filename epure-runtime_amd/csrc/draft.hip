@@ -8,12 +8,12 @@
 // 2^-50: the answers are whole numbers and must not hang on the order of sums.
 //
 // Bound by the bytes of one row of the vocabulary a sequence (of p, and of q
-// where a token was turned down): a row is cut into pieces of 4096 values, and
-// as many workgroups sum them; a second launch finds the piece in which the sum
-// is passed and looks at it again.  Which tokens stand every workgroup of the
-// first launch finds out by itself (a few loads).  64 sequences of 7 drafted tokens
-// over 128256 (f32, 66 MB of p and q): 13.6 us and 9.1; one of 4 over 32000 (f32):
-// 5.4 and 7.6, a chain of loads and steps over LDS each.
+// where a token was turned down): a row is cut into pieces of 1024 values,
+// summed side by side; a second launch finds the piece in which the sum is passed
+// and looks at it again.  Which tokens stand every workgroup of the first launch
+// finds out by itself (a few loads).  64 sequences of 7 drafted tokens over 128256
+// (f32, 66 MB of p and q): 13.7 us and 5.1 (8.6 with pieces of 4096); one of 4 over
+// 32000: 4.0 and 4.7, a chain of loads and steps over LDS each (5.4 and 7.6).
 #include "ep_common.h"
 #include "ep_draft.h"
 #include "ep_internal.h"
@@ -21,14 +21,14 @@
 namespace ep {
 namespace {
 
-constexpr int kPiece = 4096;
+constexpr int kPiece = 1024;
 
 struct DraftArgs {
     DraftTensors t;
     int64_t *accepted, *tokens;
     double2 *part;           // [B][pieces]: sum of r, sum of p
     int64_t *ends;           // [B][2]: drafted tokens that stand; the one turned down, or -1
-    uint32_t first_wg, pieces;
+    uint32_t first_wg, pieces, groups;       // groups: workgroups a sequence of the sums
 };
 
 template <typename T>
@@ -93,31 +93,38 @@ EP_DEV double2 wave_sums(double2 v)
     return v;
 }
 
-template <typename T>
+// A workgroup sums a piece, or (EACH) each of its waves one: what a workgroup
+// begins with is then paid for four.
+template <typename T, bool EACH>
 __global__ void __launch_bounds__(256) sum_kernel(DraftArgs a)
 {
     __shared__ double2 s_sum[4];
-    const uint32_t at = a.first_wg + blockIdx.x, b = at / a.pieces, piece = at - b * a.pieces;
+    const int tid = EACH ? threadIdx.x & 63 : threadIdx.x;
+    const uint32_t at = a.first_wg + blockIdx.x, b = at / a.groups, group = at - b * a.groups;
+    const uint32_t piece = EACH ? 4 * group + (threadIdx.x >> 6) : group;
     int64_t x;
     const int k = stand<T>(a.t, b, x);
     const int64_t v0 = (int64_t)piece * kPiece;
     const int n = (int)(a.t.V - v0 < kPiece ? a.t.V - v0 : kPiece);
     double2 sum = make_double2(0.0, 0.0);
 #pragma unroll 8
-    for (int i = threadIdx.x; i < n; i += 256) {
+    for (int i = tid; i < n; i += EACH ? 64 : 256) {
         const double2 w = weight<T>(a.t, b, k, x, v0 + i);
         sum.x += w.x;
         sum.y += w.y;
     }
     sum = wave_sums(sum);
-    if ((threadIdx.x & 63) == 0)
-        s_sum[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 4; ++w) {
-            sum.x += s_sum[w].x;
-            sum.y += s_sum[w].y;
-        }
+    if constexpr (!EACH) {
+        if ((threadIdx.x & 63) == 0)
+            s_sum[threadIdx.x >> 6] = sum;
+        __syncthreads();
+        if (tid == 0)
+            for (int w = 1; w < 4; ++w) {
+                sum.x += s_sum[w].x;
+                sum.y += s_sum[w].y;
+            }
+    }
+    if (tid == 0 && n > 0) {
         a.part[(int64_t)b * a.pieces + piece] = sum;
         if (piece == 0) {
             a.ends[2 * (int64_t)b] = k;
@@ -259,10 +266,18 @@ __global__ void __launch_bounds__(256) pick_kernel(DraftArgs a)
 template <typename T>
 int launch_typed(DraftArgs a, int64_t B, hipStream_t stream)
 {
-    const int64_t most = 0xffffffff / 256, grid = B * a.pieces;
+    // With more pieces than workgroups that the compute units hold at once a wave
+    // sums one alone (64 rows of 126 pieces: 21.3 -> 13.7 us; one row of 32: 3.9, 5.4 so).
+    const bool each = B * a.pieces > 2048;
+    a.groups = each ? (a.pieces + 3) / 4 : a.pieces;
+    const int64_t most = 0xffffffff / 256, grid = B * a.groups;
     for (int64_t at = 0; at < grid; at += most) {
         a.first_wg = (uint32_t)at;
-        sum_kernel<T><<<(unsigned)(grid - at < most ? grid - at : most), 256, 0, stream>>>(a);
+        const unsigned n = (unsigned)(grid - at < most ? grid - at : most);
+        if (each)
+            sum_kernel<T, true><<<n, 256, 0, stream>>>(a);
+        else
+            sum_kernel<T, false><<<n, 256, 0, stream>>>(a);
         EP_HIP_CHECK(hipGetLastError());
     }
     for (int64_t at = 0; at < B; at += most) {
@@ -286,7 +301,7 @@ int launch_verify(const DraftTensors &t, int64_t B, int dtype, int64_t *accepted
     if (ws_bytes < want || !ws)
         return set_error(EP_ERR_WORKSPACE, "verification: workspace of %zu bytes, %zu wanted", ws_bytes, want);
     double2 *const part = (double2 *)ws;
-    DraftArgs a{t, accepted, tokens, part, (int64_t *)(part + B * pieces_of(t.V)), 0, (uint32_t)pieces_of(t.V)};
+    DraftArgs a{t, accepted, tokens, part, (int64_t *)(part + B * pieces_of(t.V)), 0, (uint32_t)pieces_of(t.V), 0};
     if (B > 0x7fffffff / (int64_t)a.pieces)
         return set_error(EP_DECLINE_SHAPE, "%lld sequences over %lld tokens are more than one call takes", (long long)B,
                          (long long)t.V);

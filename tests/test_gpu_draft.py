@@ -35,6 +35,16 @@ def same(got, want):
     assert got[0].tolist() == want[0] and got[1].tolist() == want[1]
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,n,V", [(41, 2, 51201), (1050, 1, 1500), (700, 2, 3077), (3, 1, 1024), (2, 2, 1025)])
+def test_verification_of_more_pieces_than_workgroups_at_once(B, n, V, dtype):
+    """Rows of 51, 2, 4 and, for one workgroup each, 1 and 2 pieces."""
+    g = gen(B + V)
+    target, drafted, u, draft = made(g, B, n, V, dtype)
+    same(epure.verify_draft(target, drafted, u, draft=draft), od.verify(target, drafted, u, draft))
+    same(epure.verify_draft(target, drafted, u), od.verify(target, drafted, u))
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("B,n,V", [(1, 1, 1), (1, 1, 2), (3, 4, 1000), (2, 2, 4096), (2, 3, 4097), (5, 1, 8191), (70, 5, 63),
                                    (1, 70, 300), (2, 4, 20001)])

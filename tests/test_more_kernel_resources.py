@@ -54,7 +54,7 @@ def test_shared_pages_through_lds_fit_two_workgroups():
 
 def test_small_kernels_keep_everything_in_registers():
     made = found(r"((?:bounds|score|choose|select|sum|pick|join_parts|join_blocks)_kernel.*)")
-    assert len(made) == 12 + 2 + 1 + 2 + 3 + 3 + 2 + 2
+    assert len(made) == 12 + 2 + 1 + 2 + 6 + 3 + 2 + 2
     for k in made.values():
         assert k[".vgpr_spill_count"] == 0 and k[".private_segment_fixed_size"] == 0, k[".name"]
         assert k[".vgpr_count"] <= 128, k[".name"]
