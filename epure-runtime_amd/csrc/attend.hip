@@ -246,11 +246,14 @@ struct PartsPlan {
 
 // Pieces that the shared positions are cut into for `groups` row groups of all
 // cache heads: the fewest that fill the room for workgroups, round by round (else
-// those that fill it best), of two stages at least.
+// those that fill it best), of four stages at least, as every row of every piece is
+// written and joined (32 x 4 rows on 8 heads over 8192 positions: 32 pieces of
+// four 26.8 us, 64 of two 33.7), or of two up to 128 workgroups (16 x 4 over 2048:
+// 8 pieces of four 18.4 us, 16 of two 15.7).
 int64_t front_splits(int64_t groups, int64_t stages)
 {
     const int64_t room = 256 * kFrontOccupancy;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(stages / 2, 256));
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(std::max(stages / 4, std::min(stages / 2, (127 + groups) / groups)), 256));
     int64_t best = 1;
     double best_full = 0.0;
     for (int64_t s = 1; s <= most; ++s) {
@@ -266,18 +269,23 @@ int64_t front_splits(int64_t groups, int64_t stages)
     return best;
 }
 
-// Whether the shared pages go through LDS (attend_front.h).  That costs a launch
-// and some 14 us more before and behind the products, which then go 2.5 times
-// as fast (8-bit rows 1.6): 32 x 4 rows on 8 heads over 8192 positions, 8192 tiles
-// of 32 by 32, take 38 us as units and 41 so; 128 x 4 over 16384 int8 positions,
-// 65536 tiles, 134 and 101; 64 x 4 over 65536, 131072 tiles, 351 and 180.
+// Whether the shared pages go through LDS (attend_front.h): from 33 rows a cache
+// head on.  Up to 32 rows of one sequence go in the same launch as those pages do
+// (16 x 4 rows on 8 heads over 1024 positions 18.0 us as units, 14.0 so; 32 x 4
+// over 8192 37.8 and 28.2; 64 x 4 over 65536 351 and 157; 9 x 25 on 4 of 80 over 2992
+// 22.2 and 22.6; 2 x 4 over 8192, where most of a workgroup's rows are none,
+// 18.3 and 19.9).  More of them go in a launch of its own behind it, which takes 32
+// at a time: 14 us more, that 16384 tiles of 32 by 32 are worth.
+constexpr int kTogetherRows = 32;
+constexpr int64_t kTogether = 0x800000;      // workgroups of one launch of both kinds
 bool through_lds(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, int64_t shared, int64_t window)
 {
-    const int64_t all = tok.B * tok.S * (q->heads / c.heads);
+    const int64_t rows = tok.S * (q->heads / c.heads), all = tok.B * rows;
     int64_t seen = shared << c.page_shift;
     if (window > 0)
         seen = std::min(seen, window);
-    return all > 32 && c.D <= kFrontWidest && (all + 31) / 32 * c.heads >= 16384 / std::max<int64_t>(seen / kAttTile, 1);
+    return all > 32 && c.D <= kFrontWidest &&
+           (rows <= kTogetherRows || (all + 31) / 32 * c.heads >= 16384 / std::max<int64_t>(seen / kAttTile, 1));
 }
 
 // Units of the whole batch over the shared pages, then the sequences' own:
@@ -287,7 +295,7 @@ PartsPlan plan_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache
 {
     PartsPlan p{};
     const int64_t rows = tok.S * (q->heads / c.heads), all = tok.B * rows;
-    p.mt = (dense ? rows : all) <= 16 ? 1 : 2;
+    p.mt = (dense ? rows <= kTogetherRows : all <= 16) ? 1 : 2;
     const int64_t rm = 16 * p.mt;
     p.blocks = (rows + rm - 1) / rm;
     p.front = dense ? 0 : (all + rm - 1) / rm;
@@ -301,7 +309,7 @@ PartsPlan plan_parts(const ep_heads *q, const PagedTokens &tok, const PagedCache
     const int64_t most = window > 0 && window <= tiles * kAttTile
                              ? std::min(tiles, (window + tok.S) / kAttTile + 2) : tiles;
     if (most > std::min<int64_t>(16 + p.segments / 8, 32) && p.segments < 0x40000000 && tiles + kMostPiece < 0x7fff0000 / p.segments)
-        p.workers = 256 * attend_occupancy(attend_columns(c.D), p.mt, c.dtype != EP_I8);
+        p.workers = 256 * (dense && p.mt == 1 ? 1 : attend_occupancy(attend_columns(c.D), p.mt, c.dtype != EP_I8));
     p.slots = ((int64_t)2 * p.workers + p.segments) * p.slot_rows;
     const size_t part_rows = (size_t)p.slots + (size_t)p.groups * c.heads * p.splits * kFrontRows;
     p.desc = p.workers ? up16(p.segments * sizeof(int2)) : 0;
@@ -338,9 +346,9 @@ BlocksPlan plan_blocks(const ep_heads *q, const PagedTokens &tok, const PagedCac
 }
 
 // Sharing pays where there is more than one sequence, and from 1024 positions
-// seen on (16 x 4 rows on 8 heads behind 512 and 1024: 11.8 and 19.3 us each for
-// itself, 15.5 and 18.0 shared; 64 x 4 behind 1024: 49 and 42; 32 x 4 behind 2048:
-// 45 and 37).
+// seen on (16 x 4 rows on 8 heads behind 512 and 1024: 12.0 and 19.6 us each for
+// itself, 14.0 and 14.3 shared; 64 x 4 behind 1024: 36 and 22; 32 x 4 with 1024 of
+// their own behind 512 and 2048: 31.7 and 46, 31.8 and 34).
 bool shares(const PagedTokens &tok, const PagedCache &c, int64_t shared, int64_t window)
 {
     return tok.B > 1 && shared << c.page_shift >= 1024 && (window <= 0 || window >= 1024);
@@ -456,6 +464,8 @@ int launch_attend_parts(const ep_heads *q, const PagedTokens &tok, const PagedCa
     a.slot_rows = p.slot_rows;
     a.front_splits = (int)p.splits;
     a.front_at = p.slots;
+    const int64_t grid = p.workers ? p.workers : p.segments;
+    bool apart = true;
     if (p.groups) {
         FrontArgs f{};
         f.q = a.q;
@@ -474,16 +484,21 @@ int launch_attend_parts(const ep_heads *q, const PagedTokens &tok, const PagedCa
         f.splits = (int)p.splits;
         f.part_ml = a.part_ml + p.slots;
         f.part_o = a.part_o + p.slots * c.D;
-        const int64_t pairs = (int64_t)c.heads * p.splits;
-        rc = in_launches((pairs + 7) / 8 * 8 * p.groups, 64 * kFrontWaves, f,
-                         [&](const FrontArgs &part, unsigned n) { attend_front(part, q->dtype, n, stream); });
+        const int64_t pairs = (int64_t)c.heads * p.splits, fronts = (pairs + 7) / 8 * 8 * p.groups;
+        if (p.mt == 1 && fronts + grid <= kTogether) {
+            attend_front_tails(FrontTails{f, a, (uint32_t)fronts}, q->dtype, (unsigned)(fronts + grid), stream);
+            EP_HIP_CHECK(hipGetLastError());
+            apart = false;
+        } else
+            rc = in_launches(fronts, 64 * kFrontWaves, f,
+                             [&](const FrontArgs &part, unsigned n) { attend_front(part, q->dtype, n, stream); });
         if (rc != EP_OK)
             return rc;
     }
-    const int64_t grid = p.workers ? p.workers : p.segments;
-    rc = in_launches(grid, 64 * kAttWaves, a, [&](const AttendParts &part, unsigned n) {
-        attend_parts(part, q->dtype, p.mt, n, stream);
-    });
+    if (apart)
+        rc = in_launches(grid, 64 * kAttWaves, a, [&](const AttendParts &part, unsigned n) {
+            attend_parts(part, q->dtype, p.mt, n, stream);
+        });
     if (rc == EP_OK) {
         const unsigned threads = join_threads(p.segments, p.workers);
         rc = in_launches(out_rows, threads, a, [&](const AttendParts &part, unsigned n) {

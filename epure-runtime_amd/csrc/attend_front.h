@@ -1,5 +1,5 @@
 // Attention of a whole batch's rows over the pages that its tables begin with
-// (attend.hip plans and joins; attend_gen_front.hip instantiates).
+// (attend.hip plans and joins; attend_gen_front.hip and attend_gen_tails.hip instantiate).
 //
 // Many rows meet every key here, so a stage of 64 positions' keys and values is
 // brought to LDS once a workgroup and read from there by all of its four waves:
@@ -20,7 +20,8 @@
 // 8 cache heads over 65536 positions of 128 (bf16: 268 MB, 103 GFLOP of products
 // with the second term): 120 us, 106 with nothing loaded; 182 with
 // one workgroup of eight waves a compute unit and stages of 128.  128 such sequences over 16384 positions
-// in int8: 75.
+// in int8: 75.  Registers and LDS of
+// two workgroups are why wider heads are not taken here.
 #pragma once
 
 #include "attend_kernel.h"
@@ -46,8 +47,7 @@ struct FrontArgs {
 
 constexpr int kFrontWaves = 4, kFrontStage = 64;
 
-// Workgroups that a compute unit holds: by registers and LDS, which is why
-// wider heads are not taken here.
+// Workgroups that a compute unit holds, and the widest heads.
 constexpr int kFrontOccupancy = 2, kFrontWidest = 128;
 
 // How far (in powers of two) a row's weights may outgrow the maximum that they
@@ -73,16 +73,43 @@ EP_DEV void lds_rows(const void *p, uint32_t bytes, uint16_t *lds, int off)
     __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_rsrc(p, bytes), (__attribute__((address_space(3))) void *)lds, 16, off, 0, 0, 0);
 }
 
+// Output columns a lane that attend_kernel.h takes for heads of up to 32 KS values.
+constexpr int front_columns(int KS) { return KS == 2 ? 4 : 8; }
+
+// A workgroup's two stages: keys, then values.  They are arrays of their own: the
+// compiler waits for rows on their way into an array before it reads from it.
+// Where the workgroup is one of attend_body's, it joins its waves' outputs in them.
+template <int KS>
+struct FrontShared {
+    typedef AttendShared<16, 16 * front_columns(KS)> Body;
+    static constexpr int kValues = 2 * kFrontStage * 32 * KS, kOutputs = sizeof(typename Body::Outputs) / 2;
+    typedef uint16_t Even[kValues > kOutputs ? kValues : kOutputs];
+    typedef uint16_t Odd[kValues];
+    static EP_DEV Even &even()
+    {
+        __shared__ __attribute__((aligned(16))) Even s;
+        return s;
+    }
+    static EP_DEV Odd &odd()
+    {
+        __shared__ __attribute__((aligned(16))) Odd s;
+        return s;
+    }
+    static EP_DEV typename Body::Outputs &outputs() { return *(typename Body::Outputs *)even(); }
+    static EP_DEV typename Body::Rows &maxima() { return *(typename Body::Rows *)odd(); }
+    static EP_DEV typename Body::Rows &sums() { return *(typename Body::Rows *)(odd() + 1024); }
+    static EP_DEV typename Body::Positions &positions() { return *(typename Body::Positions *)(odd() + 2048); }
+};
+
 template <typename QOP, int CODE, int KS>
-__global__ void __launch_bounds__(64 * kFrontWaves, kFrontOccupancy) front_kernel(FrontArgs a)
+EP_DEV void front_body(const FrontArgs &a, uint32_t at)
 {
     constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
     constexpr int ES = k8 ? 1 : 2, NC = 2 * KS, DM = 32 * KS, TP = kFrontStage, NT = TP / 16;
     constexpr int NK = KS;           // chunks of a stage's keys, and of its values, that a lane brings
     using VOP = typename std::conditional<k8, OpBf16, QOP>::type;
-    // A stage's keys, then its values.  The two stages are arrays of their own: the
-    // compiler waits for rows on their way into an array before it reads from it.
-    __shared__ __attribute__((aligned(16))) uint16_t s_even[2 * TP * DM], s_odd[2 * TP * DM];
+    auto &s_even = FrontShared<KS>::even();
+    auto &s_odd = FrontShared<KS>::odd();
     __shared__ float s_ks[2][k8 ? TP : 1], s_vs[2][k8 ? TP : 1];
     __shared__ int s_id[2][kFrontWaves], s_lo[4], s_hi[4];     // page ids of the stages, 16 positions each
 
@@ -95,7 +122,7 @@ __global__ void __launch_bounds__(64 * kFrontWaves, kFrontOccupancy) front_kerne
     const uint32_t pairs = (uint32_t)H * a.splits;
     uint32_t pair, group;
     {
-        const uint32_t wg = a.first_wg + blockIdx.x, x = wg & 7, y = wg >> 3;
+        const uint32_t x = at & 7, y = at >> 3;
         pair = (y / a.groups) * 8 + x;
         group = y % a.groups;
     }
@@ -510,6 +537,32 @@ __global__ void __launch_bounds__(64 * kFrontWaves, kFrontOccupancy) front_kerne
     }
 }
 
+template <typename QOP, int CODE, int KS>
+__global__ void __launch_bounds__(64 * kFrontWaves, kFrontOccupancy) front_kernel(FrontArgs a)
+{
+    front_body<QOP, CODE, KS>(a, a.first_wg + blockIdx.x);
+}
+
+// And the sequences' own pages in the same launch (up to 16 rows of one sequence on
+// a cache head).  The shared pages' workgroups come first and the others where
+// those leave room: they wait for memory while the former multiply, and there is
+// no end of one launch and beginning of another between them (the calls above:
+// 176 -> 157 us and 91 -> 87; in turns 170 and 117, the others first 163 and 91).
+struct FrontTails {
+    FrontArgs front;
+    AttendParts tails;
+    uint32_t fronts;         // workgroups of the former, a multiple of eight
+};
+template <typename QOP, int CODE, int KS>
+__global__ void __launch_bounds__(64 * kFrontWaves, kFrontOccupancy) front_tails_kernel(FrontTails a)
+{
+    constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
+    if (blockIdx.x < a.fronts)
+        front_body<QOP, CODE, KS>(a.front, blockIdx.x);
+    else
+        attend_body<QOP, CODE, k8 && KS == 3 ? 4 : KS, front_columns(KS), 1, true, FrontShared<KS>>(a.tails, blockIdx.x - a.fronts);
+}
+
 template <typename QOP, int CODE>
 void front_by_size(const FrontArgs &a, unsigned grid, hipStream_t st)
 {
@@ -521,6 +574,18 @@ void front_by_size(const FrontArgs &a, unsigned grid, hipStream_t st)
         front_kernel<QOP, CODE, 4><<<grid, 64 * kFrontWaves, 0, st>>>(a);
 }
 
+template <typename QOP, int CODE>
+void front_tails_by_size(const FrontTails &a, unsigned grid, hipStream_t st)
+{
+    if (a.front.c.D <= 64)
+        front_tails_kernel<QOP, CODE, 2><<<grid, 64 * kFrontWaves, 0, st>>>(a);
+    else if (a.front.c.D <= 96)
+        front_tails_kernel<QOP, CODE, 3><<<grid, 64 * kFrontWaves, 0, st>>>(a);
+    else
+        front_tails_kernel<QOP, CODE, 4><<<grid, 64 * kFrontWaves, 0, st>>>(a);
+}
+
+void attend_front_tails(const FrontTails &a, int q_dtype, unsigned grid, hipStream_t st);
 void attend_front(const FrontArgs &a, int q_dtype, unsigned grid, hipStream_t st);
 
 }  // namespace ep

@@ -343,20 +343,51 @@ constexpr int attend_occupancy(int CW, int MT, bool lookout)
 // 16 columns; 192 bf16 values 36.8 and 37.8, 32 rows a key head 45.8 and 48.7).
 constexpr int attend_columns(int D) { return D <= 64 ? 4 : D <= 128 ? 8 : D <= 192 && D % 12 == 0 ? 12 : 16; }
 
+// What a workgroup joins its waves' outputs by: outputs, maxima and sums, the
+// rows' positions.
+template <int RM, int DP>
+struct AttendShared {
+    typedef float Outputs[kAttWaves][RM][DP + 4];
+    typedef float Rows[kAttWaves][RM];
+    typedef int Positions[RM];
+    static EP_DEV Outputs &outputs()
+    {
+        __shared__ Outputs s;
+        return s;
+    }
+    static EP_DEV Rows &maxima()
+    {
+        __shared__ Rows s;
+        return s;
+    }
+    static EP_DEV Rows &sums()
+    {
+        __shared__ Rows s;
+        return s;
+    }
+    static EP_DEV Positions &positions()
+    {
+        __shared__ Positions s;
+        return s;
+    }
+};
+
+// wg: the workgroup's number, of those that this body is for.
 // QOP: type of the queries; CODE: EP_I8, EP_E4M3, or QOP's type.  KS: steps of
 // 32 values of a head, CW: output columns a lane (16 CW >= D), MT: 16-row
 // tiles of query rows.  RAGGED: rows of a unit may differ in what they see.
-template <typename QOP, int CODE, int KS, int CW, int MT, bool RAGGED, typename ARGS>
-EP_DEV void attend_body(const ARGS &a)
+template <typename QOP, int CODE, int KS, int CW, int MT, bool RAGGED, typename SHARED = AttendShared<16 * MT, 16 * CW>, typename ARGS>
+EP_DEV void attend_body(const ARGS &a, uint32_t wg)
 {
     constexpr AttendMode MODE = ARGS::kMode;
     constexpr bool k8 = CODE == EP_I8 || CODE == EP_E4M3;
     constexpr int ES = k8 ? 1 : 2, KL = k8 ? KS / 2 : KS, RM = 16 * MT, DP = 16 * CW, VW = CW * ES / 4;
     static_assert(!k8 || KS % 2 == 0, "8-bit keys are read in chunks of two steps");
     using VOP = typename std::conditional<k8, OpBf16, QOP>::type;
-    __shared__ float s_o[kAttWaves][RM][DP + 4];
-    __shared__ float s_m[kAttWaves][RM], s_l[kAttWaves][RM];
-    __shared__ int s_p[RM];
+    auto &s_o = SHARED::outputs();
+    auto &s_m = SHARED::maxima();
+    auto &s_l = SHARED::sums();
+    auto &s_p = SHARED::positions();
     // Queries of more than one row tile stay in LDS: their registers are what
     // a second wave on the SIMD needs.
     constexpr bool kQueriesInLds = MT > 1;
@@ -839,7 +870,7 @@ EP_DEV void attend_body(const ARGS &a)
 
     // ---- a list's segment, cut into equal pieces
     if constexpr (MODE == kBlocks) {
-        const uint32_t at = a.first_wg + blockIdx.x, seg = at / (uint32_t)a.cuts, cut = at - seg * a.cuts;
+        const uint32_t at = a.first_wg + wg, seg = at / (uint32_t)a.cuts, cut = at - seg * a.cuts;
         const int tiles = (int)(((int64_t)a.take * a.c.page + kAttTile - 1) / kAttTile);
         const uint32_t u = seg / (uint32_t)H;
         piece(u, (int)(seg - u * H), (int)((int64_t)tiles * cut / a.cuts), (int)((int64_t)tiles * (cut + 1) / a.cuts),
@@ -852,7 +883,7 @@ EP_DEV void attend_body(const ARGS &a)
     // itself, 64 units at a time; the host bounds all counts to 32 bits.
     const uint32_t units = a.units;
     auto at_lane = [](uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); };
-    const uint32_t segment = a.first_wg + blockIdx.x;
+    const uint32_t segment = a.first_wg + wg;
     uint32_t u = segment / (uint32_t)H;
     int h = (int)(segment - u * H), t0 = -1, t1 = 0, slot = MODE == kParts ? (int)segment : -1;
     uint32_t f = 0, begin = 0, stop = 1, per = 1, total = 0;
@@ -882,7 +913,7 @@ EP_DEV void attend_body(const ARGS &a)
             const uint32_t shares = total > 16u * a.few ? a.few : a.workers;
             per = max((total + shares - 1) / shares,
                       min(max((total + 255) / 256, (uint32_t)kAttWaves), 2u * kAttWaves));
-            f = begin = min(blockIdx.x * per, total);
+            f = begin = min(wg * per, total);
             stop = min(begin + per, total);
             u0 = 0;
             load = units > 64;
@@ -917,12 +948,12 @@ EP_DEV void attend_body(const ARGS &a)
             // worker's first slot, else in its second; a whole segment that has
             // to stay a part, in one of its own behind them.
             const bool whole = f0 == head0 && f1 == next;
-            slot = 2 * (int)blockIdx.x + (head0 - a.piece >= begin);
+            slot = 2 * (int)wg + (head0 - a.piece >= begin);
             if (MODE == kParts && whole)
                 slot = 2 * a.workers + (int)(u * H) + h;
             if (f0 == head0 && threadIdx.x == 0) {
                 const uint32_t w1 = min((next - 1) / per, (uint32_t)a.workers - 1);
-                a.desc[u * H + h] = make_int2(slot, (int)(w1 - blockIdx.x + 1));
+                a.desc[u * H + h] = make_int2(slot, (int)(w1 - wg + 1));
             }
             if (MODE == kWhole && whole)
                 slot = -1;
@@ -935,17 +966,17 @@ EP_DEV void attend_body(const ARGS &a)
 template <typename QOP, int CODE, int KS, int CW, int MT, bool RAGGED>
 __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, RAGGED && CODE != EP_I8)) attend_kernel(AttendWhole a)
 {
-    attend_body<QOP, CODE, KS, CW, MT, RAGGED>(a);
+    attend_body<QOP, CODE, KS, CW, MT, RAGGED>(a, blockIdx.x);
 }
 template <typename QOP, int CODE, int KS, int CW, int MT>
 __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, MT, CODE != EP_I8)) attend_parts_kernel(AttendParts a)
 {
-    attend_body<QOP, CODE, KS, CW, MT, true>(a);
+    attend_body<QOP, CODE, KS, CW, MT, true>(a, blockIdx.x);
 }
 template <typename QOP, int CODE, int KS, int CW>
 __global__ void __launch_bounds__(64 * kAttWaves, attend_occupancy(CW, 1, false)) attend_blocks_kernel(AttendBlocks a)
 {
-    attend_body<QOP, CODE, KS, CW, 1, false>(a);
+    attend_body<QOP, CODE, KS, CW, 1, false>(a, blockIdx.x);
 }
 
 // Instantiations of one pair of types, by D and rows (attend_gen_*.hip).

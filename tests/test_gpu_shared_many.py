@@ -99,6 +99,38 @@ def test_many_rows(B, S, shared, own, page, G, heads, D, dtype):
             check(cache.attend(q, pos, table, shared=shared, window=window), reference(q, parts, pos, D ** -0.5, window))
 
 
+def three_ways(B, S, shared, own, page, G, heads, D, dtype):
+    g = gen(B * D + S)
+    cache, table, parts = filled(g, B, shared, own, page, heads, D, dtype)
+    q = normal(g, B, S, G * heads, D, dtype=dtype if dtype.itemsize == 2 else F16 if D % 48 == 0 else BF16, std=2.0)
+    P, L = shared * page, (shared + own) * page
+    pos = torch.randint(P, L, (B, S), generator=g, device=DEV)
+    check(cache.attend(q, pos, table, shared=shared), reference(q, parts, pos, D ** -0.5))
+    pos.view(-1)[:7] = torch.tensor([P - 1, P, L - 1, 0, -1, L, P // 2], device=DEV)[:B * S]
+    check(cache.attend(q, pos, table, shared=shared, scale=-0.21), reference(q, parts, pos, -0.21))
+    check(cache.attend(q, pos, table, shared=shared, window=P - 3), reference(q, parts, pos, D ** -0.5, P - 3))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, I8, E4M3])
+@pytest.mark.parametrize("B,S,shared,own,page,G,heads,D", [
+    (8, 5, 130, 1, 64, 8, 8, 128), (3, 33, 200, 2, 32, 3, 32, 64), (4, 12, 90, 1, 64, 4, 16, 96), (2, 70, 600, 5, 16, 1, 12, 48),
+    (2, 70, 500, 5, 16, 1, 12, 48)])
+def test_many_rows_of_each_sequence(B, S, shared, own, page, G, heads, D, dtype):
+    """More than 32 on a cache head: the sequences' own pages in a launch of their own (the last case: no LDS)."""
+    assert S * G > 32 and (tiles(B, S, shared, page, G, heads) >= 16384) == (shared != 500)
+    three_ways(B, S, shared, own, page, G, heads, D, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, I8, E4M3])
+@pytest.mark.parametrize("B,S,shared,own,page,G,heads,D", [
+    (33, 1, 65, 1, 16, 1, 1, 64), (17, 1, 17, 40, 64, 2, 3, 128), (7, 1, 2, 1, 1024, 5, 2, 96), (4, 4, 9, 3, 128, 8, 2, 112),
+    (2, 1, 33, 90, 32, 17, 1, 16), (40, 1, 33, 300, 32, 4, 8, 128), (300, 1, 17, 1, 64, 1, 2, 80), (9, 2, 80, 2, 16, 16, 1, 128)])
+def test_few_tiles_and_long_contexts_behind_them(B, S, shared, own, page, G, heads, D, dtype):
+    """33 rows on and few positions in common; own pages in one piece a sequence, or cut into shares."""
+    assert B * S * G > 32 >= S * G and tiles(B, S, shared, page, G, heads) < 16384
+    three_ways(B, S, shared, own, page, G, heads, D, dtype)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, I8, E4M3])
 def test_missing_pages_and_values_that_are_not_finite(dtype):
     """They reach who sees them, and nobody else."""

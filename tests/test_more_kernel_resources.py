@@ -42,13 +42,14 @@ def test_lists_of_pages_fit_the_registers():
 
 
 def test_shared_pages_through_lds_fit_two_workgroups():
-    """kFrontOccupancy of attend_front.h.  Rows of 128 e4m3 values put one register away."""
-    made = found(r"front_kernel<ep::Op(Bf16|F16), (\d+), (\d+)>")
-    assert {(q, int(c)) for q, c, _ in made} == TYPES and len(made) == 6 * 3
-    for (_, code, steps), k in made.items():
-        away = 1 if int(code) == E4M3 and int(steps) == 4 else 0
+    """kFrontOccupancy of attend_front.h, for the shared pages alone and with the others'.  Heads of 128 values take
+    all registers and put up to three more away."""
+    made = found(r"front(_tails)?_kernel<ep::Op(Bf16|F16), (\d+), (\d+)>")
+    assert {(q, int(c)) for _, q, c, _ in made} == TYPES and len(made) == 2 * 6 * 3
+    for (_, _, _, steps), k in made.items():
+        away = 3 if int(steps) == 4 else 0
         assert k[".vgpr_count"] <= 512 // 2, k[".name"]
-        assert k[".vgpr_spill_count"] <= away and k[".private_segment_fixed_size"] <= 8 * away, k[".name"]
+        assert k[".vgpr_spill_count"] <= away and k[".private_segment_fixed_size"] <= 4 * away, k[".name"]
         assert k[".group_segment_fixed_size"] <= 160 * 1024 // 2, k[".name"]
 
 
