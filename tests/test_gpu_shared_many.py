@@ -72,7 +72,7 @@ def check(got, want):
 
 
 def tiles(B, S, shared, page, G, heads, window=None):
-    """Of 32 rows by 32 positions: from 16384 on the shared pages go through LDS."""
+    """Of 32 rows by 32 positions: from 16384 on the shared pages always go through LDS."""
     return -(-B * S * G // 32) * heads * (min(shared * page, window or shared * page) // 32)
 
 
