@@ -12,16 +12,16 @@
 // O^T = V^T P^T if its index 8 g + 4 t + i means position 16 t + 4 g + i: what a
 // transposing LDS read of four rows gives.  16-bit rows go from memory to LDS
 // past the registers; codes of 8 bits become 16-bit values on the way, once for
-// all rows.  Rounding as there: the weights' second term costs more here (28
-// of the 120 us below), and is kept so that a
-// token's answer does not lose bits with the company that it is computed in.
+// all rows.  Rounding as there: the weights' second term costs more here (28 of
+// the 120 us below), and is kept so that a token's answer does not lose bits with
+// the company that it is computed in.
 //
-// Bound by the issue of instructions.  64 sequences of 4 query heads on each of
-// 8 cache heads over 65536 positions of 128 (bf16: 268 MB, 103 GFLOP of products
-// with the second term): 120 us, 106 with nothing loaded; 182 with
-// one workgroup of eight waves a compute unit and stages of 128.  128 such sequences over 16384 positions
-// in int8: 75.  Registers and LDS of
-// two workgroups are why wider heads are not taken here.
+// Bound by the issue of instructions.  64 sequences of 4 query heads on each of 8
+// cache heads over 65536 positions of 128 (bf16: 268 MB, 103 GFLOP of products
+// with the second term): 120 us, 106 with nothing loaded; 182 with one workgroup of
+// eight waves a compute unit and stages of 128 positions.  128 such sequences over
+// 16384 positions in int8: 75.  Registers and LDS of two workgroups are why wider
+// heads are not taken here.
 #pragma once
 
 #include "attend_kernel.h"
