@@ -84,7 +84,10 @@ EP_DEV int64_t next_lane(int64_t v)
 // held for an earlier sequence does, and it does not matter how often it is done.
 // Where positions ascend (padded at either end) that token is the one whose
 // successor lies elsewhere; in any other order the whole row is searched for a
-// later one, once a page.
+// later one, once a page.  A page may be in other sequences' tables too, at the
+// same place: the rows of those are searched as well (a load a sequence finds that
+// there are none, as a rule; 16 x 4096 tokens in chunks over one table of pages of
+// 64, 8 heads of 128, append included: 334 us, of which 227 are that search).
 // WAVES waves share a page: all four, or one; 0: all four, and rows are of one
 // token (code for several, fetched cold, took 0.7 us more).
 template <int CODE, int WAVES>
@@ -139,6 +142,23 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
         else
             return __any(x);
     };
+    // This thread's share of a look for a token on `page` behind position `mine` among
+    // the positions o of a sequence; at `mine`: behind token `who`.
+    auto later_in = [&](const int64_t *o, int64_t page, int64_t mine, int64_t who) {
+        int later = 0;
+        for (int64_t t0 = tid; t0 < a.tok.S; t0 += 8 * TEAM) {
+            int64_t p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)      // eight loads in flight; past the end the first again
+                p[i] = o[(t0 + TEAM * i < a.tok.S ? t0 + TEAM * i : t0) * ps];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t t = t0 + TEAM * i < a.tok.S ? t0 + TEAM * i : t0;
+                later |= p[i] >> a.c.page_shift == page && (p[i] > mine || (p[i] == mine && t > who));
+            }
+        }
+        return later;
+    };
     float *const t_lo = s_lo + 8 * TEAM * team, *const t_hi = s_hi + 8 * TEAM * team;
     const int lanes = D / 8, group = tid / lanes, u = tid - group * lanes, groups = TEAM / lanes;
     for (int64_t s0 = s_begin + kGroupTokens * team; s0 < s_end; s0 += kGroupTokens * TEAMS) {
@@ -155,23 +175,29 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
         for (; left; left &= left - 1) {
             const int l = ONE ? 0 : __builtin_ctzll(left);
             const int64_t mine = __shfl(p, l, 64), page = mine >> a.c.page_shift, who = s0 + l;
-            if (!ONE && !ascend) {
-                int later = 0;
-                for (int64_t t0 = tid; t0 < a.tok.S; t0 += 8 * TEAM) {
-                    int64_t o[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)      // eight loads in flight; past the end the first again
-                        o[i] = pos[(t0 + TEAM * i < a.tok.S ? t0 + TEAM * i : t0) * ps];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int64_t t = t0 + TEAM * i < a.tok.S ? t0 + TEAM * i : t0;
-                        later |= o[i] >= 0 && o[i] >> a.c.page_shift == page && (o[i] > mine || (o[i] == mine && t > who));
+            const int32_t here = __shfl(id, l, 64);
+            const int64_t row0 = ((int64_t)here * H + h) * a.c.page;
+            int later = 0;
+            if constexpr (ONE)       // the loads do not wait for `here`
+                for (int64_t o = tid; o < a.tok.B; o += 256) {
+                    const int32_t there = a.tok.table[o * a.tok.table_stride + page];
+                    const int64_t q = a.tok.pos[o * a.tok.pos_sb];
+                    later |= there == here && q >> a.c.page_shift == page && q > mine;
+                }
+            else if (!ascend || a.tok.B > 1) {
+                for (int64_t o0 = 0; o0 < a.tok.B; o0 += 64) {
+                    const int64_t o = o0 + lane;
+                    bool have = o < a.tok.B;
+                    if (have)
+                        have = o == b ? !ascend : a.tok.table[o * a.tok.table_stride + page] == here;
+                    for (uint64_t rows = __ballot(have); rows; rows &= rows - 1) {
+                        const int64_t r = o0 + __builtin_ctzll(rows);
+                        later |= later_in(a.tok.pos + r * a.tok.pos_sb, page, mine, r == b ? who : a.tok.S);
                     }
                 }
                 if (team_any(later))
                     continue;
             }
-            const int64_t row0 = ((int64_t)__shfl(id, l, 64) * H + h) * a.c.page;
             const int rows = (int)(mine & (a.c.page - 1)) + 1;
             float lo[8], hi[8];
 #pragma unroll
@@ -193,14 +219,18 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
                             hi[i] = largest(hi[i], v[k][i]);
                         }
                 }
-            team_sync();         // the buffers' last readers are done
+            if constexpr (ONE) {
+                if (a.tok.B > 1 && team_any(later))
+                    return;
+            } else
+                team_sync();     // the buffers' last readers are done
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 t_lo[8 * tid + i] = lo[i];      // [group][D], as 8 (group lanes + u) + i = group D + 8 u + i
                 t_hi[8 * tid + i] = hi[i];
             }
             team_sync();
-            const int64_t out = ((int64_t)__shfl(id, l, 64) * H + h) * 2 * D;
+            const int64_t out = ((int64_t)here * H + h) * 2 * D;
             for (int e = tid; e < 2 * D; e += TEAM) {
                 const bool top = e >= D;
                 const int d = top ? e - D : e;

@@ -375,7 +375,9 @@ class PagedKVCache:
         Bounds, where the cache keeps them, are rebuilt for each page written,
         from its rows up to the largest of the call's positions on it: a
         sequence that goes back to an earlier position and appends from there
-        leaves no trace of what it held."""
+        leaves no trace of what it held.  Sequences of a call may write a page
+        in common, at the same place of their tables: the largest position of
+        any of them counts."""
         call = _native()
         if call is not None:
             cos, sin, inter = (None, None, False) if rotary is None else \

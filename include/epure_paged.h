@@ -154,7 +154,10 @@ int ep_paged_attention_shared(const ep_heads *q, const ep_tokens *tokens, const 
  * largest value of each column over a page's rows.  After ep_kv_append of the
  * same tokens: each page that one of them lies on gets those of its rows from
  * 0 to the largest position of the call's tokens on it (a NaN among them is
- * both).  Tokens that store nothing because of the page table change nothing.
+ * both).  Sequences may have a page in common, and write it in one call: it
+ * stands at one place of their tables then, as a page does that holds the keys
+ * of some positions (where it stands at two, its bounds may be those of either).
+ * Tokens that store nothing because of the page table change nothing.
  */
 int ep_kv_bounds(const ep_tokens *tokens, const ep_kv_cache *cache, void *bounds, void *stream);
 
