@@ -55,7 +55,7 @@ size_t attend_blocks_workspace(const ep_heads *q, const PagedTokens &tok, const 
 int launch_attend_blocks(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, const int32_t *list,
                          int64_t take, float scale, int64_t window, void *out, void *ws, size_t ws_bytes,
                          hipStream_t stream);
-int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, hipStream_t stream);
+int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, int64_t limit, hipStream_t stream);
 size_t select_workspace(const PagedTokens &tok, const PagedCache &c, int64_t take);
 int launch_kv_select(const ep_heads *q, const PagedTokens &tok, const PagedCache &c, const void *bounds, int64_t take,
                      int32_t *blocks, void *ws, size_t ws_bytes, hipStream_t stream);

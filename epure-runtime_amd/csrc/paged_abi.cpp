@@ -117,6 +117,36 @@ int check_take(int64_t take, const ep_tokens *t, const PagedCache &c)
     return EP_OK;
 }
 
+int check_append(const ep_heads *q, const ep_heads *k, const ep_heads *v, const ep_rotation *rot,
+                 const ep_tokens *tokens, const ep_kv_cache *cache, const void *q_out, PagedCache &c)
+{
+    int rc = check_tokens(tokens, true);
+    if (rc == EP_OK)
+        rc = check_heads("k", k, tokens);
+    if (rc == EP_OK)
+        rc = check_heads("v", v, tokens);
+    if (rc == EP_OK && q)
+        rc = check_heads("q", q, tokens);
+    if (rc == EP_OK)
+        rc = check_cache(cache, c);
+    if (rc == EP_OK && rot)
+        rc = check_rotation(rot, c.D);
+    if (rc != EP_OK)
+        return rc;
+    if (k->dtype != v->dtype || (q && q->dtype != k->dtype))
+        return set_error(EP_ERR_ARG, "append: q, k and v differ in type");
+    if (k->heads != c.heads || v->heads != c.heads)
+        return set_error(EP_ERR_ARG, "append: %d key and %d value heads for a cache of %d", k->heads, v->heads, c.heads);
+    if (q && !q_out && tokens->B > 0 && tokens->S > 0)
+        return set_error(EP_ERR_ARG, "append: null output");
+    return EP_OK;
+}
+
+int check_bounds(const void *bounds)
+{
+    return bounds && aligned16(bounds) ? EP_OK : set_error(EP_ERR_ARG, "bounds must be 16-byte aligned storage");
+}
+
 }  // namespace
 
 extern "C" {
@@ -152,26 +182,25 @@ int ep_kv_append(const ep_heads *q, const ep_heads *k, const ep_heads *v, const 
 {
     set_error(EP_OK, "");
     PagedCache c;
-    int rc = check_tokens(tokens, true);
+    const int rc = check_append(q, k, v, rot, tokens, cache, q_out, c);
+    return rc != EP_OK ? rc : launch_kv_append(q, k, v, rot, tokens_of(tokens), c, q_out, (hipStream_t)stream);
+}
+
+int ep_kv_append_bounds(const ep_heads *q, const ep_heads *k, const ep_heads *v, const ep_rotation *rot,
+                        const ep_tokens *tokens, const ep_kv_cache *cache, void *q_out, void *bounds, void *stream)
+{
+    set_error(EP_OK, "");
+    PagedCache c;
+    int rc = check_append(q, k, v, rot, tokens, cache, q_out, c);
     if (rc == EP_OK)
-        rc = check_heads("k", k, tokens);
-    if (rc == EP_OK)
-        rc = check_heads("v", v, tokens);
-    if (rc == EP_OK && q)
-        rc = check_heads("q", q, tokens);
-    if (rc == EP_OK)
-        rc = check_cache(cache, c);
-    if (rc == EP_OK && rot)
-        rc = check_rotation(rot, c.D);
+        rc = check_bounds(bounds);
     if (rc != EP_OK)
         return rc;
-    if (k->dtype != v->dtype || (q && q->dtype != k->dtype))
-        return set_error(EP_ERR_ARG, "append: q, k and v differ in type");
-    if (k->heads != c.heads || v->heads != c.heads)
-        return set_error(EP_ERR_ARG, "append: %d key and %d value heads for a cache of %d", k->heads, v->heads, c.heads);
-    if (q && !q_out && tokens->B > 0 && tokens->S > 0)
-        return set_error(EP_ERR_ARG, "append: null output");
-    return launch_kv_append(q, k, v, rot, tokens_of(tokens), c, q_out, (hipStream_t)stream);
+    const PagedTokens tok = tokens_of(tokens);
+    rc = launch_kv_append(q, k, v, rot, tok, c, q_out, (hipStream_t)stream);
+    if (rc != EP_OK || tokens->B == 0 || tokens->S == 0)
+        return rc;
+    return launch_kv_bounds(tok, c, bounds, rot ? rot->max_pos : INT64_MAX, (hipStream_t)stream);
 }
 
 int ep_kv_read(const ep_tokens *tokens, const ep_kv_cache *cache, void *k_out, void *v_out, int out_dtype,
@@ -253,13 +282,11 @@ int ep_kv_bounds(const ep_tokens *tokens, const ep_kv_cache *cache, void *bounds
     int rc = check_tokens(tokens, true);
     if (rc == EP_OK)
         rc = check_cache(cache, c);
-    if (rc != EP_OK)
+    if (rc == EP_OK)
+        rc = check_bounds(bounds);
+    if (rc != EP_OK || tokens->B == 0 || tokens->S == 0)
         return rc;
-    if (!bounds || !aligned16(bounds))
-        return set_error(EP_ERR_ARG, "bounds must be 16-byte aligned storage");
-    if (tokens->B == 0 || tokens->S == 0)
-        return EP_OK;
-    return launch_kv_bounds(tokens_of(tokens), c, bounds, (hipStream_t)stream);
+    return launch_kv_bounds(tokens_of(tokens), c, bounds, INT64_MAX, (hipStream_t)stream);
 }
 
 size_t ep_kv_select_workspace(const ep_tokens *tokens, const ep_kv_cache *cache, int64_t take)
@@ -279,12 +306,10 @@ int ep_kv_select(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *
     int rc = check_query(q, tokens, cache, c);
     if (rc == EP_OK)
         rc = check_take(take, tokens, c);
-    if (rc != EP_OK)
+    if (rc == EP_OK)
+        rc = check_bounds(bounds);
+    if (rc != EP_OK || tokens->B == 0 || tokens->S == 0)
         return rc;
-    if (!bounds || !aligned16(bounds))
-        return set_error(EP_ERR_ARG, "bounds must be 16-byte aligned storage");
-    if (tokens->B == 0 || tokens->S == 0)
-        return EP_OK;
     if (!blocks)
         return set_error(EP_ERR_ARG, "select: null output");
     if (!aligned16(workspace))

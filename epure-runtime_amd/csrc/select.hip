@@ -40,6 +40,7 @@ struct BoundsArgs {
     PagedTokens tok;
     PagedCache c;
     void *bounds;
+    int64_t limit;           // positions from here on store nothing
     uint32_t first_wg, chunks, each;     // workgroups a sequence, of `each` groups of tokens
 };
 
@@ -82,12 +83,13 @@ EP_DEV int64_t next_lane(int64_t v)
 // later in the call) rebuilds the page's bounds from its rows up to that position:
 // what the page held before the call counts as the new rows do, nothing that it
 // held for an earlier sequence does, and it does not matter how often it is done.
-// Where positions ascend (padded at either end) that token is the one whose
-// successor lies elsewhere; in any other order the whole row is searched for a
-// later one, once a page.  A page may be in other sequences' tables too, at the
-// same place: the rows of those are searched as well (a load a sequence finds that
-// there are none, as a rule; 16 x 4096 tokens in chunks over one table of pages of
-// 64, 8 heads of 128, append included: 334 us, of which 227 are that search).
+// Where positions ascend (padded at either end, all below the limit) that token is
+// the one whose successor lies elsewhere; in any other order the whole row is
+// searched for a later one, once a page.  A page may be in other sequences' tables
+// too, at the same place: the rows of those are searched as well (a load a sequence
+// finds that there are none, as a rule; 16 x 4096 tokens in chunks over one table
+// of pages of 64, 8 heads of 128, append included: 334 us, of which 227 are that
+// search).
 // WAVES waves share a page: all four, or one; 0: all four, and rows are of one
 // token (code for several, fetched cold, took 0.7 us more).
 template <int CODE, int WAVES>
@@ -100,6 +102,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
     const uint32_t part = at / H, h = at - part * H, b = ONE ? part : part / a.chunks, chunk = part - b * a.chunks;
     const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM, lane = tid & 63, D = a.c.D;
     const int64_t *pos = a.tok.pos + (int64_t)b * a.tok.pos_sb;
+    auto stored = [&](int64_t p) { return p < a.limit ? p : -1; };
     const int64_t ps = a.tok.pos_ss, s_begin = (int64_t)chunk * a.each * kGroupTokens;
     const int64_t s_end = s_begin + a.each * kGroupTokens < a.tok.S ? s_begin + a.each * kGroupTokens : a.tok.S;
     bool ascend = true;
@@ -119,7 +122,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
             for (int i = 0; i < kOrder; ++i) {
                 const int64_t next = next_lane(o[i]), t = t0 + 256 * i < a.tok.S ? t0 + 256 * i : t0;
                 after[i] = lane == 63 ? after[i] : t + 1 < a.tok.S ? next : -1;
-                wrong |= after[i] >= 0 && after[i] <= o[i];
+                wrong |= (after[i] >= 0 && after[i] <= o[i]) || o[i] >= a.limit;
                 begins += o[i] < 0 && after[i] >= 0 && t0 + 256 * i < a.tok.S;
             }
         }
@@ -142,9 +145,9 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
         else
             return __any(x);
     };
-    // This thread's share of a look for a token on `page` behind position `mine` among
-    // the positions o of a sequence; at `mine`: behind token `who`.
-    auto later_in = [&](const int64_t *o, int64_t page, int64_t mine, int64_t who) {
+    // This thread's share of a look for a token between position `mine` and `top`
+    // among the positions o of a sequence; at `mine`: behind token `who`.
+    auto later_in = [&](const int64_t *o, int64_t mine, int64_t top, int64_t who) {
         int later = 0;
         for (int64_t t0 = tid; t0 < a.tok.S; t0 += 8 * TEAM) {
             int64_t p[8];
@@ -154,7 +157,8 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int64_t t = t0 + TEAM * i < a.tok.S ? t0 + TEAM * i : t0;
-                later |= p[i] >> a.c.page_shift == page && (p[i] > mine || (p[i] == mine && t > who));
+                const uint64_t ahead = p[i] - mine;
+                later |= ahead < (uint64_t)(top - mine) && (ahead || t > who);
             }
         }
         return later;
@@ -163,7 +167,8 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
     const int lanes = D / 8, group = tid / lanes, u = tid - group * lanes, groups = TEAM / lanes;
     for (int64_t s0 = s_begin + kGroupTokens * team; s0 < s_end; s0 += kGroupTokens * TEAMS) {
         const int64_t s = s0 + lane;
-        const int64_t p = ONE ? pos[0] : s < a.tok.S ? pos[s * ps] : -1, after = !ONE && s + 1 < a.tok.S ? pos[(s + 1) * ps] : -1;
+        const int64_t p = stored(ONE ? pos[0] : s < a.tok.S ? pos[s * ps] : -1);
+        const int64_t after = stored(!ONE && s + 1 < a.tok.S ? pos[(s + 1) * ps] : -1);
         const int64_t index = p >> a.c.page_shift;
         int32_t id = -1;
         if (p >= 0 && index < a.tok.width)
@@ -176,13 +181,14 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
             const int l = ONE ? 0 : __builtin_ctzll(left);
             const int64_t mine = __shfl(p, l, 64), page = mine >> a.c.page_shift, who = s0 + l;
             const int32_t here = __shfl(id, l, 64);
+            const int64_t end = (page + 1) << a.c.page_shift, top = end < a.limit ? end : a.limit;
             const int64_t row0 = ((int64_t)here * H + h) * a.c.page;
             int later = 0;
             if constexpr (ONE)       // the loads do not wait for `here`
                 for (int64_t o = tid; o < a.tok.B; o += 256) {
                     const int32_t there = a.tok.table[o * a.tok.table_stride + page];
                     const int64_t q = a.tok.pos[o * a.tok.pos_sb];
-                    later |= there == here && q >> a.c.page_shift == page && q > mine;
+                    later |= there == here && q > mine && q < top;
                 }
             else if (!ascend || a.tok.B > 1) {
                 for (int64_t o0 = 0; o0 < a.tok.B; o0 += 64) {
@@ -192,7 +198,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
                         have = o == b ? !ascend : a.tok.table[o * a.tok.table_stride + page] == here;
                     for (uint64_t rows = __ballot(have); rows; rows &= rows - 1) {
                         const int64_t r = o0 + __builtin_ctzll(rows);
-                        later |= later_in(a.tok.pos + r * a.tok.pos_sb, page, mine, r == b ? who : a.tok.S);
+                        later |= later_in(a.tok.pos + r * a.tok.pos_sb, mine, top, r == b ? who : a.tok.S);
                     }
                 }
                 if (team_any(later))
@@ -613,7 +619,7 @@ int in_launches(int64_t grid, unsigned threads, ARGS a, F launch)
 
 }  // namespace
 
-int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, hipStream_t stream)
+int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, int64_t limit, hipStream_t stream)
 {
     // From 1024 pages and heads on a wave rebuilds a page alone.  With four / one,
     // 8 heads of 128 in bf16, append included: 2 x 512 tokens on pages of 64, 128 of
@@ -629,7 +635,7 @@ int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, 
     if (parts > 0x7fffffff / c.heads)
         return set_error(EP_DECLINE_SHAPE, "bounds of %lld x %lld tokens are more than one call takes", (long long)tok.B,
                          (long long)tok.S);
-    const BoundsArgs args{tok, c, bounds, 0, (uint32_t)chunks, (uint32_t)each};
+    const BoundsArgs args{tok, c, bounds, limit, 0, (uint32_t)chunks, (uint32_t)each};
     auto run = [&](auto code) {
         constexpr int CODE = decltype(code)::value;
         return in_launches(parts * c.heads, 256, args, [&](const BoundsArgs &a, unsigned n) {

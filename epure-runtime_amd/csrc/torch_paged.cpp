@@ -21,7 +21,7 @@ decltype(&ep_paged_attention_workspace) fn_attend_ws;
 decltype(&ep_paged_attention) fn_attend;
 decltype(&ep_paged_attention_shared_workspace) fn_shared_ws;
 decltype(&ep_paged_attention_shared) fn_shared;
-decltype(&ep_kv_bounds) fn_bounds;
+decltype(&ep_kv_append_bounds) fn_append_bounds;
 decltype(&ep_kv_select_workspace) fn_select_ws;
 decltype(&ep_kv_select) fn_select;
 decltype(&ep_paged_attention_blocks_workspace) fn_blocks_ws;
@@ -331,20 +331,17 @@ PyObject *append_to(PyObject *const *args, PyObject *bounds_arg)
     const ep_heads qh = some_q ? heads_of(*q) : ep_heads{}, kh = heads_of(*k), vh = heads_of(*v);
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = fn_append(some_q ? &qh : nullptr, &kh, &vh, turns ? &r : nullptr, &tok, &c, some_q ? qo.data_ptr() : nullptr,
-                   stream);
+    if (bounds)
+        rc = fn_append_bounds(some_q ? &qh : nullptr, &kh, &vh, turns ? &r : nullptr, &tok, &c,
+                              some_q ? qo.data_ptr() : nullptr, bounds, stream);
+    else
+        rc = fn_append(some_q ? &qh : nullptr, &kh, &vh, turns ? &r : nullptr, &tok, &c, some_q ? qo.data_ptr() : nullptr,
+                       stream);
     Py_END_ALLOW_THREADS
     if (rc > 0)
         Py_RETURN_NOTIMPLEMENTED;
     if (rc < 0)
-        return failed("ep_kv_append", rc);
-    if (bounds) {
-        Py_BEGIN_ALLOW_THREADS
-        rc = fn_bounds(&tok, &c, bounds, stream);
-        Py_END_ALLOW_THREADS
-        if (rc != EP_OK)
-            return failed("ep_kv_bounds", rc);
-    }
+        return failed(bounds ? "ep_kv_append_bounds" : "ep_kv_append", rc);
     if (!some_q)
         Py_RETURN_NONE;
     return THPVariable_Wrap(qo);
@@ -582,7 +579,7 @@ PyObject *bind_paged(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     Py_RETURN_NONE;
 }
 
-// bind_select(shared attention's workspace and call, bounds, select's workspace
+// bind_select(shared attention's workspace and call, append with bounds, select's workspace
 // and call, listed attention's workspace and call): addresses
 PyObject *bind_select(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 {
@@ -590,7 +587,7 @@ PyObject *bind_select(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         return nullptr;
     fn_shared_ws = (decltype(fn_shared_ws))PyLong_AsVoidPtr(args[0]);
     fn_shared = (decltype(fn_shared))PyLong_AsVoidPtr(args[1]);
-    fn_bounds = (decltype(fn_bounds))PyLong_AsVoidPtr(args[2]);
+    fn_append_bounds = (decltype(fn_append_bounds))PyLong_AsVoidPtr(args[2]);
     fn_select_ws = (decltype(fn_select_ws))PyLong_AsVoidPtr(args[3]);
     fn_select = (decltype(fn_select))PyLong_AsVoidPtr(args[4]);
     fn_blocks_ws = (decltype(fn_blocks_ws))PyLong_AsVoidPtr(args[5]);

@@ -150,6 +150,7 @@ _SIGS = {
     "ep_paged_attention_shared": (_c_int, [
         _heads, _tokens, _cache, _c_i64, ctypes.c_float, _c_i64,  # q, tokens, cache, shared, scale, window
         _p, _p, _sz, _p]),                       # out, workspace, bytes, stream
+    "ep_kv_append_bounds": (_c_int, [_heads, _heads, _heads, _rotation, _tokens, _cache, _p, _p, _p]),
     "ep_kv_bounds": (_c_int, [_tokens, _cache, _p, _p]),
     "ep_kv_select_workspace": (_sz, [_tokens, _cache, _c_i64]),
     "ep_kv_select": (_c_int, [_heads, _tokens, _cache, _p, _c_i64, _p, _p, _sz, _p]),
@@ -183,7 +184,7 @@ def _load_call(handle):
              addr("ep_last_error"), getattr(torch._C, "_cuda_getCurrentRawStream", None))
     ext.bind_paged(addr("ep_rotate"), addr("ep_kv_append"), addr("ep_kv_read"),
                    addr("ep_paged_attention_workspace"), addr("ep_paged_attention"))
-    ext.bind_select(addr("ep_paged_attention_shared_workspace"), addr("ep_paged_attention_shared"), addr("ep_kv_bounds"),
+    ext.bind_select(addr("ep_paged_attention_shared_workspace"), addr("ep_paged_attention_shared"), addr("ep_kv_append_bounds"),
                     addr("ep_kv_select_workspace"), addr("ep_kv_select"),
                     addr("ep_paged_attention_blocks_workspace"), addr("ep_paged_attention_blocks"))
     ext.bind_draft(addr("ep_verify_draft_workspace"), addr("ep_verify_draft"))

@@ -377,7 +377,8 @@ class PagedKVCache:
         sequence that goes back to an earlier position and appends from there
         leaves no trace of what it held.  Sequences of a call may write a page
         in common, at the same place of their tables: the largest position of
-        any of them counts."""
+        any of them counts.  Positions past the rotation's tables are not
+        stored, and change no bounds."""
         call = _native()
         if call is not None:
             cos, sin, inter = (None, None, False) if rotary is None else \
@@ -409,13 +410,12 @@ class PagedKVCache:
         if k.numel() == 0:
             return qo
         some_q = q is not None and q.shape[2] > 0
-        _run("ep_kv_append", _abi.lib.ep_kv_append(
-            _heads(q) if some_q else None, _heads(k), _heads(v), rotary._rotation() if rotary is not None else None,
-            tok, self._cache(), qo.data_ptr() if some_q else None, _abi.stream_handle(k.device)))
-        if self.k_bounds is not None:
-            with torch.cuda.device(k.device):
-                _run("ep_kv_bounds", _abi.lib.ep_kv_bounds(tok, self._cache(), self.k_bounds.data_ptr(),
-                                                           _abi.stream_handle(k.device)))
+        which, more = ("ep_kv_append", ()) if self.k_bounds is None else \
+            ("ep_kv_append_bounds", (self.k_bounds.data_ptr(),))
+        with torch.cuda.device(k.device):
+            _run(which, getattr(_abi.lib, which)(
+                _heads(q) if some_q else None, _heads(k), _heads(v), rotary._rotation() if rotary is not None else None,
+                tok, self._cache(), qo.data_ptr() if some_q else None, *more, _abi.stream_handle(k.device)))
         return qo
 
     def read(self, positions, table, dtype=torch.bfloat16):

@@ -151,14 +151,18 @@ int ep_paged_attention_shared(const ep_heads *q, const ep_tokens *tokens, const 
 /*
  * Bounds of the keys a cache holds: bounds [n_pages][heads][2][D] (dense,
  * 16-byte aligned; the cache's type, for 8-bit caches f32), the least and the
- * largest value of each column over a page's rows.  After ep_kv_append of the
- * same tokens: each page that one of them lies on gets those of its rows from
+ * largest value of each column over a page's rows.  ep_kv_append_bounds stores
+ * as ep_kv_append does; ep_kv_bounds takes the tokens as stored, behind an append
+ * without a rotation.  Then each page that one of them lies on gets those of its rows from
  * 0 to the largest position of the call's tokens on it (a NaN among them is
  * both).  Sequences may have a page in common, and write it in one call: it
  * stands at one place of their tables then, as a page does that holds the keys
  * of some positions (where it stands at two, its bounds may be those of either).
- * Tokens that store nothing because of the page table change nothing.
+ * Tokens that store nothing (past the rotation's or the page table, or on no page
+ * of the pool) change nothing.
  */
+int ep_kv_append_bounds(const ep_heads *q, const ep_heads *k, const ep_heads *v, const ep_rotation *rot,
+                        const ep_tokens *tokens, const ep_kv_cache *cache, void *q_out, void *bounds, void *stream);
 int ep_kv_bounds(const ep_tokens *tokens, const ep_kv_cache *cache, void *bounds, void *stream);
 
 /*
