@@ -31,14 +31,17 @@ struct DraftArgs {
     uint32_t first_wg, pieces, groups;       // groups: workgroups a sequence of the sums
 };
 
+// One probability; a NaN or a negative one is none.
 template <typename T>
 EP_DEV double prob(const void *p, int64_t at)
 {
     const T v = ((const T *)p)[at];
+    float f;
     if constexpr (sizeof(T) == 2 && !__is_same(T, f16_t))
-        return (double)bf16_to_f32(v);
+        f = bf16_to_f32(v);
     else
-        return (double)(float)v;
+        f = (float)v;
+    return (double)fmaxf(f, 0.0f);
 }
 
 // How many drafted tokens of sequence b stand; turned_down: one that does not
@@ -80,7 +83,7 @@ EP_DEV double2 weight(const DraftTensors &t, int64_t b, int k, int64_t turned_do
     if (turned_down >= 0)
         q = t.draft ? prob<T>(t.draft, b * t.q_sb + k * t.q_ss + v) : v == turned_down ? 1.0 : 0.0;
     const double r = p - q;
-    return make_double2(r > 0.0 ? r : 0.0, p > 0.0 ? p : 0.0);       // a NaN weighs nothing
+    return make_double2(r > 0.0 ? r : 0.0, p);
 }
 
 EP_DEV double2 wave_sums(double2 v)

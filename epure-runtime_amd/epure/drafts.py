@@ -21,6 +21,7 @@ def verify_draft(target, drafted, uniforms, draft=None):
     of them and for the token behind the last, ``draft`` ``[B, n, V]`` those
     they were drawn from, in the same type (float32, float16 or bfloat16).
     Without ``draft`` the proposals were certain (a lookup, a greedy model).
+    Probabilities need not sum to 1; a NaN or a negative one counts as 0.
     ``uniforms`` ``[B, n + 1]`` are float32 random numbers in [0, 1).
 
     Token x of step i stands if ``uniforms[i] * draft[i, x] < target[i, x]``.

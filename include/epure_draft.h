@@ -23,7 +23,7 @@ extern "C" {
  * Probabilities of B sequences: target [B][n + 1][V], and draft [B][n][V] or
  * NULL (the drafted tokens were certain: q = 1 for each, 0 elsewhere), both of
  * one type (EP_F32 / EP_F16 / EP_BF16), strides in elements, the values of one
- * step adjacent.  They need not sum to 1; a NaN or a negative one weighs nothing.
+ * step adjacent.  They need not sum to 1; a NaN or a negative one counts as 0.
  * drafted [B][n]: token ids; one outside [0, V) ends its sequence's draft.
  * uniforms [B][n + 1]: random numbers in [0, 1).
  */
