@@ -13,7 +13,8 @@ namespace {
 // Joins `n` pieces of one output row a workgroup, piece k of it at row at(k)
 // of the parts: D / 4 lanes take a piece, the next ones the next, each with its
 // own running maximum, so that sums, maxima and outputs load together.  p: the
-// row's position; none: what a row without any weight gives.
+// row's position; none: what a row gives that sees no position (maximum -inf; NaN
+// if it has seen some and they weigh nothing).
 template <typename OP, typename AT>
 EP_DEV void join_row(const AttendArgs &a, int64_t out_row, int p, int n, AT at, float none)
 {
@@ -60,7 +61,7 @@ EP_DEV void join_row(const AttendArgs &a, int64_t out_row, int p, int n, AT at, 
     const float inv = 1.0f / l;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        y[i] = p < 0 ? 0.0f : p >= a.cap ? __uint_as_float(0x7fc00000u) : l == 0.0f ? none : y[i] * inv;
+        y[i] = p < 0 ? 0.0f : p >= a.cap ? __uint_as_float(0x7fc00000u) : l == 0.0f ? m == -INFINITY ? none : __uint_as_float(0x7fc00000u) : y[i] * inv;
     uint2 w;
     w.x = OP::pack(y[0], y[1]);
     w.y = OP::pack(y[2], y[3]);

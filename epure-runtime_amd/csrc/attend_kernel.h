@@ -600,6 +600,7 @@ EP_DEV void attend_body(const ARGS &a, uint32_t wg)
         // each, looked at in the end).  With 8 columns the bits cost some 25 more.
         constexpr bool kHitsApart = RAGGED && CODE != EP_I8 && CW >= 12;
         uint32_t hit[MT][2] = {};
+        bool named = false;      // kBlocks: a tile held positions that the rows see
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             m[mt] = -INFINITY;
@@ -632,6 +633,8 @@ EP_DEV void attend_body(const ARGS &a, uint32_t wg)
             // positions of the tile's halves
             const int j0 = MODE == kBlocks ? base[0] : j * kAttTile, j1 = MODE == kBlocks ? base[1] : j0 + 16;
             const bool bad0 = !good[0], bad1 = !good[1];
+            if constexpr (MODE == kBlocks)
+                named = named || (j0 <= hi && j0 + 15 >= lo) || (j1 <= hi && j1 + 15 >= lo);
             auto position = [&](int e) { return (e < 4 ? j0 : j1) + 4 * g + e % 4; };
             f32x4_t sc[MT][2];
 #pragma unroll
@@ -814,6 +817,10 @@ EP_DEV void attend_body(const ARGS &a, uint32_t wg)
                     for (int i = 0; i < 4; ++i)
                         o[mt][t][i] = hit[mt][t / 8] >> (4 * (t % 8) + i) & 1 ? nan : o[mt][t][i];
             l[mt] = xor32_sum(xor16_sum(l[mt]));
+            // Positions whose scores are all -inf weigh nothing, and are not none: the least
+            // finite maximum tells them from a list that names no position.
+            if constexpr (MODE == kBlocks)
+                m[mt] = named ? fmaxf(m[mt], -__FLT_MAX__) : m[mt];
             if (eg == 0) {
                 s_m[wave][16 * mt + en] = m[mt];
                 s_l[wave][16 * mt + en] = l[mt];
@@ -855,8 +862,8 @@ EP_DEV void attend_body(const ARGS &a, uint32_t wg)
             }
             const AttendToken t = attend_token(a, unit, r0 + r);
             const int p = s_p[r];
-            const float inv = 1.0f / sum;      // no weight at all (every score -inf) gives NaN; zeros where a list names no page
-            const float none = MODE == kBlocks ? 0.0f : nan;
+            const float inv = 1.0f / sum;      // no weight at all (every score -inf) gives NaN; zeros where a list names no position
+            const float none = MODE == kBlocks && mx == -INFINITY ? 0.0f : nan;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 y[i] = p < 0 ? 0.0f : p >= a.cap ? nan : sum == 0.0f ? none : y[i] * inv;

@@ -504,7 +504,8 @@ class PagedKVCache:
         these pages of its sequence, indices into its row of the table as
         ``select`` gives them, in any order; negative ones, and ones past the
         table, name none, one that is there twice counts twice, and a token
-        that sees no position gets zeros.  Not together with ``shared``."""
+        that sees no position gets zeros (one that sees some, with scores of
+        -inf throughout, NaN as without a list).  Not together with ``shared``."""
         call = _native()
         if call is not None:
             held = (self.k, self.v, self.k_scale, self.v_scale)

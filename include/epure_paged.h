@@ -186,7 +186,8 @@ int ep_kv_select(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *
  * (int32, dense, take >= 1) names for each token and cache head, in any order:
  * the positions max(0, p - window + 1) .. p on them.  An index that is
  * negative, or not below the table's width, names none; one that is there
- * twice counts twice.  A token that sees no position gets zeros.
+ * twice counts twice.  A token that sees no position gets zeros; one
+ * that sees some, whose scores are all -inf, gets NaN as there.
  */
 size_t ep_paged_attention_blocks_workspace(const ep_heads *q, const ep_tokens *tokens, const ep_kv_cache *cache,
                                            int64_t take);
