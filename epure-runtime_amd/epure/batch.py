@@ -47,7 +47,7 @@ class BatchDecoder:
         width = -(-max_len // page)
         self.n_pages = batch * width if n_pages is None else n_pages
         self.rotary = Rotary(cfg.head_dim, max_len, theta=cfg.rope_theta, scaling=scaling, device=dev)
-        self.select = select
+        self.select = None if select is None else min(select, width)     # more pages than a table has: -1 for each
         self.caches = [PagedKVCache(self.n_pages, page, cfg.n_kv, cfg.head_dim, cache_dtype, dev,
                                     bounds=select is not None) for _ in weights.layers]
         self.lin = [{name: PackedLinear(store) for name, store in layer.lin.items()} for layer in weights.layers]
