@@ -541,7 +541,7 @@ PyObject *select(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         PyErr_Clear();
         Py_RETURN_NOTIMPLEMENTED;
     }
-    if (take < 1)
+    if (take < 1 || c.page < 1 || take > 0x3fffffff / c.page)      // before the list is allocated
         Py_RETURN_NOTIMPLEMENTED;
     bool ok;
     void *stream = stream_of(*q, &ok);

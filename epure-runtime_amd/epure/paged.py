@@ -475,6 +475,8 @@ class PagedKVCache:
         n = operator.index(n)
         if n < 1:
             raise ValueError(f"select takes at least one page, got {n}")
+        if n > 0x3fffffff // self.page:     # before the list is allocated
+            raise ValueError(f"{n} pages of {self.page} rows a token: up to 2^30 positions are served")
         q = self._queries(q)
         tok, _keep = _tokens(q.shape[:2], positions, table)
         blocks = torch.empty(*q.shape[:2], self.heads, n, dtype=torch.int32, device=q.device)
