@@ -156,21 +156,26 @@ EP_DEV AttendUnit attend_unit(const ARGS &a, uint32_t u)
         return {r0, a.rows, b, 0, 0, a.cap};
 }
 
-// Token (b, s) of row `row` of a unit.
+// Token (b, s) of row `row` of a unit; its tokens count from that of row 0.
 struct AttendToken {
     int64_t b;
     int s, head;     // head: within the group
 };
 template <typename ARGS>
-EP_DEV AttendToken attend_token(const ARGS &a, const AttendUnit &u, int row)
+EP_DEV AttendToken attend_token_at(const ARGS &a, const AttendUnit &u, int t, int head)
 {
-    const int t = (uint32_t)row / (uint32_t)a.G, head = row - t * a.G;
     if constexpr (ARGS::kMode == kWhole)
         return {u.b, t, head};
     else {
         const uint32_t at = (uint32_t)(u.t0 + t), b = at / (uint32_t)a.tok.S;
         return {b, (int)(at - b * (uint32_t)a.tok.S), head};
     }
+}
+template <typename ARGS>
+EP_DEV AttendToken attend_token(const ARGS &a, const AttendUnit &u, int row)
+{
+    const int t = (uint32_t)row / (uint32_t)a.G;
+    return attend_token_at(a, u, t, row - t * a.G);
 }
 
 // What a row at position p sees of its unit's positions, counted from the
@@ -204,7 +209,7 @@ EP_DEV uint32_t unit_tiles(const ARGS &a, uint32_t u, uint32_t &first)
         int p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {    // four loads in flight; the last token again past the end
-            const AttendToken t = attend_token(a, unit, min(s + i, s1) * a.G);
+            const AttendToken t = attend_token_at(a, unit, min(s + i, s1), 0);
             p[i] = attend_position(a, t.b, t.s);
         }
 #pragma unroll
