@@ -101,3 +101,25 @@ def test_a_replayed_step_on_common_pages():
         twin.append(k, v, pos, table)
         torch.cuda.synchronize()
         assert torch.equal(cache.k_bounds, twin.k_bounds)
+
+
+@pytest.mark.parametrize("S", [1, 70])
+def test_bounds_of_rows_that_are_there_already(S):
+    """The entry point without an append, behind one into a cache that keeps none."""
+    import ctypes
+
+    from epure.kernels import _abi
+    from epure.paged import _tokens
+    g = gen(S)
+    B, page = 6, 16
+    cache = made(g, 40, page, 2, 80, F16)
+    bare = epure.PagedKVCache.of(cache.k, cache.v)
+    table = torch.arange(40, dtype=torch.int32, device=DEV)[None].expand(B, -1)
+    pos = torch.arange(B * S, device=DEV).view(B, S) + 5
+    k = normal(g, B, S, 2, 80, dtype=F16)
+    bare.append(k, k, pos, table)
+    before = cache.k_bounds.clone()
+    tok, _keep = _tokens((B, S), pos, table)
+    assert _abi.lib.ep_kv_bounds(ctypes.byref(tok), ctypes.byref(cache._cache()), cache.k_bounds.data_ptr(),
+                                 _abi.stream_handle(DEV)) == 0
+    check_bounds(cache, before, table.cpu(), pos.cpu(), page)
