@@ -273,14 +273,16 @@ int64_t front_splits(int64_t groups, int64_t stages)
 // Whether the shared pages go through LDS (attend_front.h): from 33 rows a cache
 // head on, if those of one sequence are a tile at most (16 x 4 rows on 8 heads over
 // 1024 positions 18.0 us as units, 14.0 so; 32 x 4 over 8192 37.8 and 28.2; 64 x 4
-// over 65536 351 and 157; 2 x 4 over 8192, where most of a workgroup's rows are none,
+// over 65536 351 and 157 to 164; 2 x 4 over 8192, where most of a workgroup's rows are none,
 // 18.3 and 19.9), or from 16384 tiles of 32 rows by 32 positions on (16 x 32 rows on
 // 8 heads over 4096, 16384 tiles, 45.6 and 38.8; 9 x 25 on 4 of 80 over 2992, 2992
 // tiles, 21.5 and 22.8, of e4m3 with a window 22.0 and 26.6).
 // Where a window may end among the shared pages, scores there are masked one by
 // one, and 256 rows are asked for (window 40 short of the pages, as units and so:
 // 16 x 4 over 4096 22.6 and 32.5, of e4m3 22.0 and 35.7; 64 x 4 over 2048 36.2 and
-// 35.8, 37.1 and 38.9; windows of 1100: 20.1 and 17.0, 32.9 and 25.8).
+// 35.8, of e4m3 37.1 and 38.9; windows of 1100: 20.1 and 17.0, 32.9 and 25.8; what
+// lies between 64 and 256 rows was not measured).  The host knows no positions: a
+// window shorter than the table counts, though it may be longer than any context.
 // Up to 32 rows of one sequence go in the same launch as those pages do; more go in
 // one of their own behind it, which takes 32 at a time.
 constexpr int kTogetherRows = 32;

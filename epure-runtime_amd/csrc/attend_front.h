@@ -5,7 +5,7 @@
 // brought to LDS once a workgroup and read from there by all of its four waves:
 // 128 rows (token by token, the group's query heads side by side), 32 a wave.
 // Two stages lie in LDS, one on its way while the other is read; a compute unit
-// holds two workgroups, and one's softmax runs beside the other's products.
+// holds two workgroups, so that one has something to do where the other waits.
 //
 // The products are those of attend_kernel.h: S^T = K Q^T gives lane (n, g) the
 // scores of positions 16 t + 4 g + i of query row n, which is the operand of
@@ -16,12 +16,14 @@
 // the 120 us below), and is kept so that a token's answer does not lose bits with
 // the company that it is computed in.
 //
-// Bound by the issue of instructions.  64 sequences of 4 query heads on each of 8
-// cache heads over 65536 positions of 128 (bf16: 268 MB, 103 GFLOP of products
-// with the second term): 120 us, 106 with nothing loaded; 182 with one workgroup of
-// eight waves a compute unit and stages of 128 positions.  128 such sequences over
-// 16384 positions in int8: 75.  Registers and LDS of two workgroups are why wider
-// heads are not taken here.
+// Bound by vector and matrix instructions that hardly overlap.  64 sequences of 4
+// query heads on each of 8 cache heads over 65536 positions of 128 (bf16: 268 MB,
+// 103 GFLOP of products with the second term): 120 us, 106 with nothing loaded.  The
+// instructions counted, at the clocks of each kind in a loop of its own, are some 70
+// us of vector ones and 60 of matrix ones: about their sum is what is measured.  One
+// workgroup of eight waves a compute unit and stages of 128 positions took 182.  128
+// such sequences over 16384 positions in int8: 75.  Wider heads are not taken: two
+// workgroups' stages of 64 positions, and 32 rows a wave, leave them no room.
 #pragma once
 
 #include "attend_kernel.h"
@@ -47,7 +49,9 @@ struct FrontArgs {
 
 constexpr int kFrontWaves = 4, kFrontStage = 64;
 
-// Workgroups that a compute unit holds, and the widest heads.
+// Workgroups that a compute unit holds, and the widest heads.  Those of 128 values
+// take all registers that two leave them: nine of the kernels put two or three more
+// away (12 bytes of scratch a lane).
 constexpr int kFrontOccupancy = 2, kFrontWidest = 128;
 
 // How far (in powers of two) a row's weights may outgrow the maximum that they
@@ -543,11 +547,11 @@ __global__ void __launch_bounds__(64 * kFrontWaves, kFrontOccupancy) front_kerne
     front_body<QOP, CODE, KS>(a, a.first_wg + blockIdx.x);
 }
 
-// And the sequences' own pages in the same launch (up to 16 rows of one sequence on
-// a cache head).  The shared pages' workgroups come first and the others where
+// And the sequences' own pages in the same launch (up to kTogetherRows rows of one
+// sequence on a cache head, 16 a unit).  The shared pages' workgroups come first and the others where
 // those leave room: they wait for memory while the former multiply, and there is
 // no end of one launch and beginning of another between them (the calls above:
-// 176 -> 157 us and 91 -> 87; in turns 170 and 117, the others first 163 and 91).
+// 176 -> 157 to 164 us and 91 -> 85; in turns 170 and 117, the others first 163 and 91).
 struct FrontTails {
     FrontArgs front;
     AttendParts tails;

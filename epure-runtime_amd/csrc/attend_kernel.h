@@ -81,8 +81,9 @@ struct AttendArgs {
 //   kParts: the tables' first `shared` pages are those of sequence 0.  The
 //     first `front` units are rows of the whole batch, over those pages; the
 //     rest is as in kWhole, over the pages behind them, positions counted
-//     from there.  Every output stays a part: the join adds them up (more than
-//     32 rows a cache head over the shared pages are attend_front.h's);
+//     from there.  Every output stays a part: the join adds them up (where the
+//     shared pages go through LDS, through_lds() of attend.hip, they are
+//     attend_front.h's and there are no such units);
 //   kBlocks: a unit is up to 16 rows of one token, and tile after tile goes
 //     over the `take` pages that a list names for it, in `cuts` equal pieces
 //     (8 tokens of 64 pages of 64 positions, 8 heads of 128 in bf16, 134 MB: 23 us).

@@ -12,7 +12,7 @@
 // summed side by side; a second launch finds the piece in which the sum is passed
 // and looks at it again.  Which tokens stand every workgroup of the first launch
 // finds out by itself (a few loads).  64 sequences of 7 drafted tokens over 128256
-// (f32, 66 MB of p and q): 13.7 us and 5.1 (8.6 with pieces of 4096); one of 4 over
+// (f32, 66 MB of p and q): 13.9 us and 5.2 (8.6 with pieces of 4096); one of 4 over
 // 32000: 4.0 and 4.7, a chain of loads and steps over LDS each (5.4 and 7.6).
 #include "ep_common.h"
 #include "ep_draft.h"

@@ -18,8 +18,8 @@
 // heads of 128 (bf16, 67 MB) take 17 us and the choice of 64 of them 8, a chain
 // of steps over LDS.  Up to kFewPages pages a row one workgroup does both in one
 // launch (44 pages on 8 heads: 7.4 us; 60 tokens of up to 282 pages on 4: 12.8).
-// The bounds of 64 appended tokens take 5.8 us, a chain of loads, and those of
-// 2 x 4096 (8 heads, pages of 64) 10.6, beside 14.5 for the rows themselves.
+// The bounds of 64 appended tokens take 6.1 us, a chain of loads, and those of
+// 2 x 4096 (8 heads, pages of 64) 12.0, beside 14.4 for the rows themselves.
 #include "ep_common.h"
 #include "ep_internal.h"
 #include "ep_paged.h"
@@ -623,8 +623,9 @@ int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, 
 {
     // From 1024 pages and heads on a wave rebuilds a page alone.  With four / one,
     // 8 heads of 128 in bf16, append included: 2 x 512 tokens on pages of 64, 128 of
-    // them, 11.4 / 17.1 us; 2 x 4096, 1024, 28.1 / 26.7; on pages of 16 40 / 32;
-    // 65536 332 / 171.
+    // them, 12.1 / 15.4 us; 2 x 2048, 512, 19.1 / 21.7; 3 x 2048, 768, 23.0 / 24.0;
+    // 2 x 4096, 1024, 28.5 / 26.2; on pages of 16 2 x 512, 512, 23.0 / 21.9; 2 x 4096,
+    // 4096, 43 / 33; 65536, 32768, 349 / 173.
     const bool alone = tok.S > 1 && tok.B * c.heads * ((tok.S + c.page - 1) >> c.page_shift) >= 1024;
     // Every workgroup looks at its whole row for the positions' order: long rows
     // have no more than kRowChunks of them a head.
