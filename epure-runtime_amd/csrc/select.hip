@@ -42,6 +42,7 @@ struct BoundsArgs {
     void *bounds;
     int64_t limit;           // positions from here on store nothing
     uint32_t first_wg, chunks, each;     // workgroups a sequence, of `each` groups of tokens
+    uint32_t heads, head_groups;         // that a workgroup takes one after the other; workgroups that share all
 };
 
 // Eight adjacent values of a cache row as f32.
@@ -78,7 +79,8 @@ EP_DEV int64_t next_lane(int64_t v)
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// One workgroup looks over `each` times 64 tokens of a sequence and one cache head.
+// One workgroup looks over `each` times 64 tokens of a sequence, for one cache head
+// or a few.
 // Of the tokens on one page the one at the largest position (of two there, the
 // later in the call) rebuilds the page's bounds from its rows up to that position:
 // what the page held before the call counts as the new rows do, nothing that it
@@ -99,7 +101,8 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
     constexpr int TEAMS = WAVES == 1 ? 4 : 1, TEAM = 256 / TEAMS, kOrder = WAVES == 1 ? 16 : 8;
     __shared__ float s_lo[256 * 8], s_hi[256 * 8];
     const uint32_t at = a.first_wg + blockIdx.x, H = a.c.heads;
-    const uint32_t part = at / H, h = at - part * H, b = ONE ? part : part / a.chunks, chunk = part - b * a.chunks;
+    const uint32_t part = at / a.head_groups, h0 = (at - part * a.head_groups) * a.heads, h1 = min(h0 + a.heads, H);
+    const uint32_t b = ONE ? part : part / a.chunks, chunk = part - b * a.chunks;
     const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM, lane = tid & 63, D = a.c.D;
     const int64_t *pos = a.tok.pos + (int64_t)b * a.tok.pos_sb;
     auto stored = [&](int64_t p) { return p < a.limit ? p : -1; };
@@ -182,7 +185,6 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
             const int64_t mine = __shfl(p, l, 64), page = mine >> a.c.page_shift, who = s0 + l;
             const int32_t here = __shfl(id, l, 64);
             const int64_t end = (page + 1) << a.c.page_shift, top = end < a.limit ? end : a.limit;
-            const int64_t row0 = ((int64_t)here * H + h) * a.c.page;
             int later = 0;
             if constexpr (ONE)       // the loads do not wait for `here`
                 for (int64_t o = tid; o < a.tok.B; o += 256) {
@@ -205,50 +207,53 @@ __global__ void __launch_bounds__(256) bounds_kernel(BoundsArgs a)
                     continue;
             }
             const int rows = (int)(mine & (a.c.page - 1)) + 1;
-            float lo[8], hi[8];
+            for (uint32_t h = h0; h < h1; ++h) {
+                const int64_t row0 = ((int64_t)here * H + h) * a.c.page;
+                float lo[8], hi[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                lo[i] = INFINITY;
-                hi[i] = -INFINITY;
-            }
-            if (group < groups)
-                for (int r = group; r < rows; r += 4 * groups) {
-                    float v[4][8];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)      // four rows in flight; past the end the last again
-                        row_values<CODE>(a.c, row0 + min(r + k * groups, rows - 1), 8 * u, v[k]);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            lo[i] = least(lo[i], v[k][i]);
-                            hi[i] = largest(hi[i], v[k][i]);
-                        }
+                for (int i = 0; i < 8; ++i) {
+                    lo[i] = INFINITY;
+                    hi[i] = -INFINITY;
                 }
-            if constexpr (ONE) {
-                if (a.tok.B > 1 && team_any(later))
-                    return;
-            } else
-                team_sync();     // the buffers' last readers are done
+                if (group < groups)
+                    for (int r = group; r < rows; r += 4 * groups) {
+                        float v[4][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                t_lo[8 * tid + i] = lo[i];      // [group][D], as 8 (group lanes + u) + i = group D + 8 u + i
-                t_hi[8 * tid + i] = hi[i];
-            }
-            team_sync();
-            const int64_t out = ((int64_t)here * H + h) * 2 * D;
-            for (int e = tid; e < 2 * D; e += TEAM) {
-                const bool top = e >= D;
-                const int d = top ? e - D : e;
-                float x = top ? t_hi[d] : t_lo[d];
-                for (int k = 1; k < groups; ++k)
-                    x = top ? largest(x, t_hi[k * D + d]) : least(x, t_lo[k * D + d]);
-                if constexpr (CODE == EP_F16)
-                    ((f16_t *)a.bounds)[out + e] = (f16_t)x;
-                else if constexpr (CODE == EP_BF16)
-                    ((uint16_t *)a.bounds)[out + e] = f32_to_bf16(x);
-                else
-                    ((float *)a.bounds)[out + e] = x;
+                        for (int k = 0; k < 4; ++k)      // four rows in flight; past the end the last again
+                            row_values<CODE>(a.c, row0 + min(r + k * groups, rows - 1), 8 * u, v[k]);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                lo[i] = least(lo[i], v[k][i]);
+                                hi[i] = largest(hi[i], v[k][i]);
+                            }
+                    }
+                if (ONE && h == h0) {
+                    if (a.tok.B > 1 && team_any(later))
+                        return;
+                } else
+                    team_sync();     // the buffers' last readers are done
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    t_lo[8 * tid + i] = lo[i];      // [group][D], as 8 (group lanes + u) + i = group D + 8 u + i
+                    t_hi[8 * tid + i] = hi[i];
+                }
+                team_sync();
+                const int64_t out = ((int64_t)here * H + h) * 2 * D;
+                for (int e = tid; e < 2 * D; e += TEAM) {
+                    const bool top = e >= D;
+                    const int d = top ? e - D : e;
+                    float x = top ? t_hi[d] : t_lo[d];
+                    for (int k = 1; k < groups; ++k)
+                        x = top ? largest(x, t_hi[k * D + d]) : least(x, t_lo[k * D + d]);
+                    if constexpr (CODE == EP_F16)
+                        ((f16_t *)a.bounds)[out + e] = (f16_t)x;
+                    else if constexpr (CODE == EP_BF16)
+                        ((uint16_t *)a.bounds)[out + e] = f32_to_bf16(x);
+                    else
+                        ((float *)a.bounds)[out + e] = x;
+                }
             }
             if (ONE)
                 return;
@@ -636,10 +641,17 @@ int launch_kv_bounds(const PagedTokens &tok, const PagedCache &c, void *bounds, 
     if (parts > 0x7fffffff / c.heads)
         return set_error(EP_DECLINE_SHAPE, "bounds of %lld x %lld tokens are more than one call takes", (long long)tok.B,
                          (long long)tok.S);
-    const BoundsArgs args{tok, c, bounds, limit, 0, (uint32_t)chunks, (uint32_t)each};
+    // What a workgroup finds out about its tokens holds for all heads, and a look at
+    // the other sequences grows with their number: more workgroups than 4096 take
+    // several heads each.  One head / so, 8 heads of 128 in bf16, append included:
+    // 512 x 1 tokens 19.7 / 20.6 us (the kernel's registers), 2048 x 1 68 / 60,
+    // 4096 x 1 162 / 113, 4096 x 4 358 / 128.
+    const int64_t some = std::max<int64_t>(1, std::min<int64_t>(c.heads, parts * c.heads / 4096));
+    const int64_t head_groups = (c.heads + some - 1) / some;
+    const BoundsArgs args{tok, c, bounds, limit, 0, (uint32_t)chunks, (uint32_t)each, (uint32_t)some, (uint32_t)head_groups};
     auto run = [&](auto code) {
         constexpr int CODE = decltype(code)::value;
-        return in_launches(parts * c.heads, 256, args, [&](const BoundsArgs &a, unsigned n) {
+        return in_launches(parts * head_groups, 256, args, [&](const BoundsArgs &a, unsigned n) {
             if (tok.S == 1)
                 bounds_kernel<CODE, 0><<<n, 256, 0, stream>>>(a);
             else if (alone)

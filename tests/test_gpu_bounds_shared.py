@@ -65,6 +65,20 @@ def test_one_token_each_on_common_pages(B, page, heads, D, dtype):
         step(g, cache, table, p)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, I8, E4M3])
+@pytest.mark.parametrize("B,S,heads", [(2100, 1, 5), (4200, 1, 3), (1100, 3, 8), (830, 17, 12)])
+def test_more_sequences_than_workgroups_at_once(B, S, heads, dtype):
+    """A workgroup takes two heads or three; every fifth sequence has the page of the one before."""
+    assert B * heads >= 8192
+    g = gen(B)
+    cache = made(g, B + 3, 32, heads, 16, dtype)
+    table = torch.randperm(B + 3, generator=g, device=DEV)[:B].to(torch.int32)[:, None].contiguous()
+    table[4::5] = table[3::5][:table[4::5].shape[0]]
+    start = torch.randint(-2, 32 - S + 1, (B, 1), generator=g, device=DEV)
+    step(g, cache, table, start + torch.arange(S, device=DEV))
+    step(g, cache, table, torch.where(start >= 0, start + torch.arange(S, device=DEV).flip(0), -1))
+
+
 @pytest.mark.parametrize("S", [1, 5, 90])
 def test_sequences_that_part_within_their_tables(S):
     """The first pages in common, the rest their own (or none, or nonsense): tokens on both."""
